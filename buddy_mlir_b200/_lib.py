@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(_HERE, "libbuddy_b200_kernels.so")
 
 F32, F16, BF16 = 0, 1, 2
 W_F32, W_I8, W_U4 = 0, 1, 2
+PAGES_OK, PAGES_EXHAUSTED, PAGES_TABLE, PAGES_ROWS, PAGES_STATE = range(5)
 
 (T_EMBED, T_INV_FREQ, T_FINAL_NORM, T_LM_HEAD, T_IN_NORM, T_POST_NORM, T_Q_NORM,
  T_K_NORM, T_Q, T_K, T_V, T_O, T_GATE, T_UP, T_DOWN, T_Q_BIAS, T_K_BIAS,
@@ -38,6 +39,23 @@ class ModelConfigC(C.Structure):
                  "vocab", "max_len")] + \
                [("eps", C.c_float), ("rope_theta", C.c_float)] + \
                [(n, C.c_int32) for n in ("qkv_bias", "qk_norm", "tp_rank", "tp_size")]
+
+
+class Kv4Cache(C.Structure):
+    _fields_ = [("pool", C.c_void_p)] + [(n, C.c_int32) for n in ("n_pages", "kv_heads", "head_dim", "page")]
+
+
+class PageStep(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_seqs", "page", "table_stride", "n_pages", "max_rows", "reserved")] + \
+               [(n, C.c_void_p) for n in ("held", "add", "held_out", "block_table", "free_pages", "n_free", "n_free_out",
+                                          "row_start", "slots", "row_seq", "row_pos", "status")]
+
+
+class Kv4Attention(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("dtype", C.c_int32), ("q_heads", C.c_int32),
+                ("q_ld", C.c_int64), ("out_ld", C.c_int64), ("rows", C.c_int32), ("n_seqs", C.c_int32),
+                ("row_start", C.c_void_p), ("lens", C.c_void_p), ("block_table", C.c_void_p),
+                ("table_stride", C.c_int32), ("scale", C.c_float)]
 
 
 class B200Error(RuntimeError):
@@ -91,6 +109,12 @@ def load():
         "b200_argmax_first": (i32, [vp, i64, vp, vp, vp]),
         "b200_kv_overflow": (i32, [vp, i32, i32, i32, i32, i32, i32, f32,
                                    C.POINTER(C.c_int), vp]),
+        "b200_kv4_pool_bytes": (i64, [i32, i32, i32, i32]),
+        "b200_kv4_write": (i32, [C.POINTER(Kv4Cache), vp, i64, vp, i64, i32, vp, i32, vp]),
+        "b200_kv4_read": (i32, [C.POINTER(Kv4Cache), vp, i64, vp, i64, i32, vp, i32, vp]),
+        "b200_page_step": (i32, [C.POINTER(PageStep), vp]),
+        "b200_kv4_attention_workspace_bytes": (i64, [i32, i32, i32]),
+        "b200_kv4_attention": (i32, [C.POINTER(Kv4Cache), C.POINTER(Kv4Attention), vp, i64, vp]),
         "b200_model_create": (i32, [C.POINTER(ModelConfigC), C.POINTER(vp)]),
         "b200_model_destroy": (None, [vp]),
         "b200_model_set_vector": (i32, [vp, i32, i32, vp, i64]),

@@ -1,0 +1,184 @@
+// One step of the page allocator on the device (b200_page_step): lengths in, block tables, slots and row maps out.
+//
+// Every CTA adds up all sequences (new rows, pages taken, pages given back: three prefix sums in shared memory) and then writes its share of
+// the outputs; a row, a page or a place of the stack finds its sequence by binary search.  Old values are read before the barrier, or are
+// never written (entries below a sequence's old end, places below the old top of the stack), so a step may be in place.
+#include "kv4.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+
+struct Sums {
+  long long rows, taken, given;
+};
+__device__ __forceinline__ Sums operator+(Sums a, Sums b) { return {a.rows + b.rows, a.taken + b.taken, a.given + b.given}; }
+__device__ __forceinline__ Sums up(Sums a, int o) {
+  return {__shfl_up_sync(0xffffffffu, a.rows, o), __shfl_up_sync(0xffffffffu, a.taken, o), __shfl_up_sync(0xffffffffu, a.given, o)};
+}
+
+// The last i of 0 .. n - 1 with first[i] <= x (first does not decrease, first[0] <= x < first[n]): never a sequence without any.
+__device__ __forceinline__ int owner(const int32_t *first, int n, int x) {
+  int lo = 0, hi = n;   // first[lo] <= x < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= x)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kThreads) page_step_kernel(const __grid_constant__ b200_page_step_args p) {
+  extern __shared__ int32_t s_all[];
+  __shared__ Sums s_warp[kWarps];
+  __shared__ int s_over, s_state;
+  const int n = p.n_seqs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int32_t *s_row = s_all, *s_take = s_row + n + 1, *s_give = s_take + n + 1, *s_held = s_give + n + 1;
+  kernel_go();
+  if (tid == 0)
+    s_over = s_state = 0;
+  kernel_wait();
+  __syncthreads();
+
+  // ---- this thread's sequences, then all before them ------------------------------------------------------------------------
+  const int per = (n + kThreads - 1) / kThreads, first = min(n, tid * per), last = min(n, first + per);
+  const long long room = (long long)p.table_stride * p.page;
+  Sums mine{0, 0, 0};
+  bool over = false, bad = false;
+  const int n_free = *p.n_free;
+  for (int s = first; s < last; ++s) {
+    const long long held = p.held[s], add = p.add[s];
+    bad = bad || held < 0 || held > room;
+    over = over || (add > 0 && held + add > room);
+    const long long have = (held + p.page - 1) / p.page;
+    mine = mine + (add < 0 ? Sums{0, 0, have} : Sums{add, (held + add + p.page - 1) / p.page - have, 0});
+    s_held[s] = (int32_t)held;
+  }
+  if (over)
+    s_over = 1;
+  if (bad)
+    s_state = 1;
+  Sums sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const Sums v = up(sum, o);
+    if (lane >= o)
+      sum = sum + v;
+  }
+  if (lane == 31)
+    s_warp[warp] = sum;
+  __syncthreads();
+  Sums before{0, 0, 0}, total{0, 0, 0};
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp)
+      before = total;
+    total = total + s_warp[w];
+  }
+  const int status = s_state || n_free < 0 || n_free > p.n_pages || n_free + total.given > p.n_pages ? B200_PAGES_STATE
+                     : s_over                                                                        ? B200_PAGES_TABLE
+                     : total.rows > p.max_rows                                                       ? B200_PAGES_ROWS
+                     : total.taken > n_free + total.given                                            ? B200_PAGES_EXHAUSTED
+                                                                                                     : B200_PAGES_OK;
+  const bool ok = status == B200_PAGES_OK;
+  if (ok) {   // (then all sums fit 32 bits)
+    Sums at = {before.rows + sum.rows - mine.rows, before.taken + sum.taken - mine.taken, before.given + sum.given - mine.given};
+    for (int s = first; s < last; ++s) {
+      const int held = s_held[s], add = p.add[s], have = (held + p.page - 1) / p.page;
+      s_row[s] = (int32_t)at.rows;
+      s_take[s] = (int32_t)at.taken;
+      s_give[s] = (int32_t)at.given;
+      at = at + (add < 0 ? Sums{0, 0, have} : Sums{add, (int)(((long long)held + add + p.page - 1) / p.page) - have, 0});
+    }
+    if (tid == 0) {
+      s_row[n] = (int32_t)total.rows;
+      s_take[n] = (int32_t)total.taken;
+      s_give[n] = (int32_t)total.given;
+    }
+  }
+  __syncthreads();
+  const int rows = ok ? (int)total.rows : 0, taken = ok ? (int)total.taken : 0, given = ok ? (int)total.given : 0, top = n_free + given;
+
+  // ---- outputs ------------------------------------------------------------------------------------------------------------------
+  auto returned = [&](int i) {   // the i-th page that is given back
+    const int s = owner(s_give, n, i);
+    return p.block_table[(int64_t)s * p.table_stride + i - s_give[s]];
+  };
+  auto new_page = [&](int i) {   // the i-th page that is taken
+    const int at = top - 1 - i;
+    return at < n_free ? p.free_pages[at] : returned(at - n_free);
+  };
+  for (int r = tid; r < p.max_rows; r += kThreads) {
+    int64_t slot = -1;
+    int seq = -1, pos = -1;
+    if (r < rows) {
+      seq = owner(s_row, n, r);
+      pos = s_held[seq] + r - s_row[seq];
+      const int have = (s_held[seq] + p.page - 1) / p.page, at = pos / p.page;
+      const int page = at < have ? p.block_table[(int64_t)seq * p.table_stride + at] : new_page(s_take[seq] + at - have);
+      slot = (int64_t)page * p.page + pos % p.page;
+    }
+    p.slots[r] = slot;
+    if (p.row_seq != nullptr)
+      p.row_seq[r] = seq;
+    if (p.row_pos != nullptr)
+      p.row_pos[r] = pos;
+  }
+  for (int i = tid; i < taken; i += kThreads) {
+    const int s = owner(s_take, n, i), have = (s_held[s] + p.page - 1) / p.page;
+    p.block_table[(int64_t)s * p.table_stride + have + i - s_take[s]] = new_page(i);
+  }
+  for (int i = tid; i < given - taken; i += kThreads)   // what stays on the stack of them
+    p.free_pages[n_free + i] = returned(i);
+  for (int s = tid; s < n; s += kThreads) {
+    const int add = p.add[s];
+    p.held_out[s] = !ok ? s_held[s] : add < 0 ? 0 : s_held[s] + add;
+  }
+  for (int s = tid; s <= n; s += kThreads)
+    p.row_start[s] = ok ? s_row[s] : 0;
+  if (tid == 0) {
+    *p.n_free_out = ok ? top - taken : n_free;
+    *p.status = status;
+  }
+}
+
+RaisedOn g_raised;
+
+} // namespace
+
+int page_step_launch(const b200_page_step_args &a, cudaStream_t st) {
+  const int bytes = 4 * (4 * a.n_seqs + 3);
+  if (int rc = raise_shared_limit(g_raised, (const void *)page_step_kernel, 4 * (4 * B200_PAGE_STEP_MAX_SEQS + 3)))
+    return rc;
+  return launch_after(page_step_kernel, dim3(1), kThreads, bytes, st, a);
+}
+
+} // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_page_step(const b200_page_step_args *a, void *stream) {
+  if (!a || !a->held || !a->add || !a->held_out || !a->block_table || !a->free_pages || !a->n_free || !a->n_free_out || !a->row_start || !a->status ||
+      (a->max_rows > 0 && !a->slots))
+    return fail(B200_EINVAL, "page_step: null pointer");
+  if (a->n_seqs < 1 || a->page < 1 || a->table_stride < 1 || a->n_pages < 1 || a->max_rows < 0)
+    return fail(B200_EINVAL, "page_step: %d sequences, pages of %d, tables of %d, %d pages, %d rows", a->n_seqs, a->page, a->table_stride, a->n_pages,
+                a->max_rows);
+  if ((int64_t)a->table_stride * a->page > INT32_MAX)
+    return fail(B200_EINVAL, "page_step: a table of %d pages of %d positions: more than 2^31 - 1 positions", a->table_stride, a->page);
+  if (a->n_seqs > B200_PAGE_STEP_MAX_SEQS)
+    return fail(B200_ELIMIT, "page_step: %d sequences (at most %d)", a->n_seqs, B200_PAGE_STEP_MAX_SEQS);
+  if (a->add == a->held_out || (const void *)a->slots == a->held || a->row_start == a->held_out)
+    return fail(B200_EINVAL, "page_step: arrays overlap");
+  if (((uintptr_t)a->held | (uintptr_t)a->add | (uintptr_t)a->held_out | (uintptr_t)a->block_table | (uintptr_t)a->free_pages | (uintptr_t)a->n_free |
+       (uintptr_t)a->n_free_out | (uintptr_t)a->row_start | (uintptr_t)a->row_seq | (uintptr_t)a->row_pos | (uintptr_t)a->status) &
+          3 ||
+      (uintptr_t)a->slots & 7)
+    return fail(B200_EINVAL, "page_step: a pointer is not aligned to its elements");
+  if (int rc = ensure_device())
+    return rc;
+  return page_step_launch(*a, (cudaStream_t)stream);
+}

@@ -253,6 +253,138 @@ int b200_kv_overflow(float **kv_dev, int n_buffers, int kv_heads, int max_len,
                      int *new_position, void *stream);
 
 /* ------------------------------------------------------------------------
+ * A paged KV cache held in 4 bits: its pages, writes, reads and attention.
+ * (No counterpart in buddy-mlir, whose caches are contiguous floats.)
+ *
+ * Format.  A page holds `page` positions (a multiple of 16) of every kv head, K
+ * and V.  A position's K row (and V row) of one head is cut into groups of 64
+ * dims.  With x' = x clamped to +-65504 (the largest f16), a group has
+ *   lo = f16(min x'),  scale = f16((max x' - lo) / 15)
+ *   code = rint((x' - lo) / scale) within 0..15 (0 where the scale is 0)
+ * each operation rounded to f32 (nearest, ties to even), and stands for
+ *   value = lo + scale * code            (rounded to f32 once).
+ * So |value - x'| is at most half a step and what lo's rounding adds, and the
+ * bytes are the same wherever they are computed.  Infinities are held as
+ * +-65504; a NaN makes its group NaN.  4.5 bits a value.
+ *
+ * Layout.  Sixteen positions of a head are a tile of 16 * (D + D / 8) bytes; the
+ * pool is [n_pages][kv_heads][page / 16] tiles.  In a tile, in this order:
+ *   K codes [16][D / 2]: dim 32 i + 8 t + 4 a + 2 b + h of a position is the low
+ *     (b = 0) or high nibble of byte t * (D / 8) + 4 i + 2 h + a of its row;
+ *   V codes [8 D]: dim 64 j + 16 i + 8 w + g of position 8 u + 2 t + h is the low
+ *     (w = 0) or high nibble of byte 512 j + 64 g + 16 t + 4 i + 2 h + u;
+ *   K pairs, then V pairs [16][D / 64]: (scale, lo), two f16.
+ * (Words of eight codes lie as the tensor cores' operand registers want them.)
+ * A slot, page id * page + offset in the page, names a position of the pool in
+ * all heads; it is 64 bits wide, since a pool of one head of 64 dims can hold more
+ * than 2^31 positions.
+ *
+ * All calls are asynchronous on `stream`, read their inputs there, use no memory
+ * but what they are given, and can be captured into a graph. Strides (_ld) are
+ * in elements; rows need no alignment beyond their elements'. */
+typedef struct {
+  void *pool;          /* b200_kv4_pool_bytes() bytes, 16-byte aligned       */
+  int32_t n_pages, kv_heads;
+  int32_t head_dim;    /* 64 or 128                                          */
+  int32_t page;        /* positions of a page, a multiple of 16              */
+} b200_kv4_cache;
+
+/* Bytes of a pool, or B200_EINVAL for sizes that no pool has. Host function. */
+int64_t b200_kv4_pool_bytes(int n_pages, int kv_heads, int head_dim, int page);
+
+/* Quantise rows of K and V ([rows][ld], kv heads side by side, of element type
+ * `dtype`) into the cache, row r at slots[r].  A row whose slot is negative or
+ * beyond the pool is left out.  No slot twice in one call. */
+int b200_kv4_write(const b200_kv4_cache *c, const void *k, int64_t k_ld,
+                   const void *v, int64_t v_ld, int dtype, const int64_t *slots,
+                   int rows, void *stream);
+/* The values that the cache holds at `slots`, rounded to `dtype`, into rows of k and v
+ * (zero for a slot outside the pool). */
+int b200_kv4_read(const b200_kv4_cache *c, void *k, int64_t k_ld, void *v,
+                  int64_t v_ld, int dtype, const int64_t *slots, int rows,
+                  void *stream);
+
+/* One step of a page allocator that lives on the device: block tables and slot
+ * maps from the sequences' lengths, with no word from the host.  Sequence s
+ * holds held[s] positions, in the pages block_table[s][0 .. ceil(held / page));
+ * it grows by add[s] >= 0 of them, or ends (add[s] < 0) and gives its pages
+ * back.  free_pages is a stack of the n_free[0] free pages: first the pages of the
+ * sequences that end are put on it, sequence by sequence, page by page; then
+ * each growing sequence, in order, takes its new pages from the top.  Results:
+ *   held_out[s]    the positions it holds then (0 when it has ended);
+ *   block_table    the new pages' entries (others stay as they are);
+ *   free_pages, n_free_out[0]  the stack;
+ *   row_start[n_seqs + 1]  the new rows of sequence s are row_start[s] ..;
+ *   slots, row_seq, row_pos [max_rows]  of every new row: its slot, its sequence, its
+ *                  position; -1 in all rows behind the last (row_seq and row_pos
+ *                  may be NULL);
+ *   status[0]      0, or why nothing was done: B200_PAGES_*.  Then held_out is held,
+ *                  n_free_out is n_free, tables and stack stay as they are, and there
+ *                  are no rows.
+ * held_out may be held, and n_free_out n_free (a step in place); no other two
+ * arrays may overlap. With arrays of their own the inputs stay, and the step can be
+ * taken again.  Free entries above the stack's top are scratch.  n_seqs up to
+ * B200_PAGE_STEP_MAX_SEQS. */
+#define B200_PAGE_STEP_MAX_SEQS 8192
+enum {
+  B200_PAGES_OK = 0,
+  B200_PAGES_EXHAUSTED = 1, /* more new pages than the stack holds           */
+  B200_PAGES_TABLE = 2,     /* a sequence would not fit its row of the table */
+  B200_PAGES_ROWS = 3,      /* more new rows than max_rows                   */
+  B200_PAGES_STATE = 4      /* held or n_free are not what a step leaves     */
+};
+typedef struct {
+  int32_t n_seqs, page, table_stride, n_pages, max_rows, reserved;
+  const int32_t *held, *add;
+  int32_t *held_out;
+  int32_t *block_table;      /* [n_seqs][table_stride]                       */
+  int32_t *free_pages;       /* [n_pages]                                    */
+  const int32_t *n_free;
+  int32_t *n_free_out, *row_start;
+  int64_t *slots;
+  int32_t *row_seq, *row_pos, *status;
+} b200_page_step_args;
+int b200_page_step(const b200_page_step_args *a, void *stream);
+
+/* Attention of query rows over the cache: the rows row_start[s] .. row_start[s + 1]
+ * (not decreasing, within 0 .. rows) of q are the newest positions of sequence s,
+ * which holds lens[s] of them: row i of n sits at position lens[s] - n + i and
+ * sees the positions 0 .. its own (written before this call).  One row of every
+ * sequence is a decode step, several are drafted tokens, many a chunk of a prompt;
+ * all can stand in one call.  q head h reads kv head h / (q_heads / kv_heads).
+ *   out = softmax(scale * q K^T) V   with the values of the cache,
+ * scores, sums and products with f32 accumulators, rounded to `dtype` once.
+ * dtype f32: both products as exact as f32 (the other operand is split into bf16
+ * terms, codes are exact); bf16 and f16: q exactly, the weights to 2^-9 and
+ * 2^-17 of themselves.  A row that sees no position is zero, and so are the rows
+ * before row_start[0] and behind the last sequence's.  Positions beyond
+ * table_stride * page, and those whose table entry is no page of the pool, are
+ * not seen.  Nothing that a row does not see (infinities and NaN included)
+ * changes it.  workspace: b200_kv4_attention_workspace_bytes() bytes, 256-byte
+ * aligned, zeroed once by the caller (every call leaves its counters zero);
+ * calls that can overlap on the GPU need one each.  Results do not depend on what runs
+ * beside them: the same inputs on the same device give the same bits.  q and out must not overlap.
+ * n_seqs up to B200_KV4_ATTENTION_MAX_SEQS. */
+#define B200_KV4_ATTENTION_MAX_SEQS 4096
+typedef struct {
+  const void *q;             /* [rows][q_ld], heads side by side             */
+  void *out;                 /* [rows][out_ld]                               */
+  int32_t dtype, q_heads;
+  int64_t q_ld, out_ld;
+  int32_t rows, n_seqs;
+  const int32_t *row_start;  /* [n_seqs + 1]                                 */
+  const int32_t *lens;       /* [n_seqs]                                     */
+  const int32_t *block_table; /* [n_seqs][table_stride]                      */
+  int32_t table_stride;
+  float scale;               /* of the scores: 1 / sqrt(head_dim), commonly  */
+} b200_kv4_attention_args;
+int64_t b200_kv4_attention_workspace_bytes(int q_heads, int kv_heads,
+                                           int head_dim);
+int b200_kv4_attention(const b200_kv4_cache *c,
+                       const b200_kv4_attention_args *a, void *workspace,
+                       int64_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
  * Device-resident decode session.
  * ---------------------------------------------------------------------- */
 typedef struct {
