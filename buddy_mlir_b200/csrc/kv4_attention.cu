@@ -1,83 +1,672 @@
 // Attention over the 4-bit KV cache (b200_kv4_attention).
+//
+// Codes go to the tensor cores as they are: with k = lo + s c per group of 64 dims, a score is  q.k = sum over groups of s (q.c) + lo sum(q),  and
+// an output  sum p v = sum (p s) c + sum p lo,  so that scales meet scores and weights (a handful per key) instead of 64 codes each.  A code is one
+// bf16 exactly; the other operand is split into as many bf16 terms as its type needs.  Codes are the operand with M rows (mma.m16n8k16: sixteen
+// positions, or sixteen dims), the query rows that share a kv head the eight columns; words of eight codes lie in the cache as the
+// operand's registers want them, and one and-or makes a pair of codes a pair of bf16 (16 + c: the code in the mantissa's upper bits).
 #include "kv4.cuh"
+
+#include <algorithm>
 
 namespace b200 {
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kWarps = 8, kThreads = 32 * kWarps, kCtas = 296;
+constexpr int kRows = 8;            // query rows of an item: a position's heads (several positions', if they are few)
+constexpr int kStages = 3;          // tiles that a warp has in flight or in hand
+constexpr float kLag = 8.f;         // a row's maximum is renewed when a score is this far above it (powers of two)
 
 struct AttentionParams {
   const uint8_t *pool;
   int n_pages, kv_heads, page;
   b200_kv4_attention_args a;
+  int G, heads, tokens, subs;       // q heads of a kv head, of an item; positions of an item; items that share a kv head's q heads
+  float log2_scale;
+  int *counters;                    // [kCtas]
+  float *parts;                     // [kCtas][2][part floats]
 };
 
-__device__ __forceinline__ int clamp(int x, int lo, int hi) { return min(max(x, lo), hi); }
+__host__ __device__ constexpr int part_floats(int D) { return kRows * (D + 4) + 2 * kRows; }   // sums in rows of D + 4, maxima, totals
 
-// A warp per row and q head, a key after the other.
-template <int D> __global__ void __launch_bounds__(kThreads) kv4_attention_kernel(const __grid_constant__ AttentionParams p) {
-  constexpr int E = D / 32;   // dims 32 e + lane of a lane
+__device__ __forceinline__ int clamp(long long x, int lo, int hi) { return (int)(x < lo ? lo : x > hi ? hi : x); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float low_of(uint32_t pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float high_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void copy16(void *to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// Codes 0..15 of nibbles p and p + 4 as a pair of bf16: 16 + c, or (CENTRED) c - 7.5.  Both exact.  Centred operands keep a sum of n
+// weighted codes as small as the values' own spread: the tensor cores' sums round towards zero, and would lose 5 sqrt(n) times as much.
+constexpr float kOffset = 16.f, kCentre = 7.5f;
+template <bool CENTRED> __device__ __forceinline__ uint32_t codes(uint32_t w, int p) {
+  const uint32_t x = ((p == 0 ? w << 3 : w >> (4 * p - 3)) & 0x00780078u) | 0x41804180u;
+  if constexpr (!CENTRED)
+    return x;
+  uint32_t y;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(0x3f803f80u), "r"(0xc1bcc1bcu));   // * 1 - 23.5
+  return y;
+}
+
+// x as TERMS bf16 that add up to it (f16: two are exact, f32: three), pairs of two values
+template <int TERMS> __device__ __forceinline__ void split(float x, float y, uint32_t (&t)[TERMS]) {
+#pragma unroll
+  for (int i = 0; i < TERMS; ++i) {
+    t[i] = pack_bf16(x, y);
+    if (i + 1 < TERMS) {
+      x -= low_of(t[i]);
+      y -= high_of(t[i]);
+    }
+  }
+}
+
+// A sequence as its items: its rows `tokens` at a time and, for each kv head (or part of its q heads), a range of keys that ends at the last
+// row's own position.  Cost of an item: its keys; of all items before it in a head: before().
+struct Sequence {
+  int r0, n;            // rows
+  int base;             // position of the first row (negative: rows before it see nothing), at most the table's room
+  int past, tiles;      // max(base, 0); row tiles
+  __device__ __forceinline__ Sequence(const AttentionParams &p, int s, int room) {
+    r0 = clamp(p.a.row_start[s], 0, p.a.rows);
+    n = clamp(p.a.row_start[s + 1], r0, p.a.rows) - r0;
+    base = clamp((long long)p.a.lens[s] - n, -n, room);
+    past = max(base, 0);
+    tiles = (n + p.tokens - 1) / p.tokens;
+  }
+  __device__ __forceinline__ long long before(int rt, int tokens) const {
+    return rt < tiles ? (long long)rt * past + (long long)tokens * rt * (rt + 1) / 2
+                      : tiles == 0 ? 0 : (long long)(tiles - 1) * past + (long long)tokens * tiles * (tiles - 1) / 2 + past + n;
+  }
+};
+
+template <int D, int TERMS> struct Tile {   // of a warp: one item's sums
+  static constexpr int GROUPS = D / kKv4Group, STEPS = D / 16;
+  static constexpr bool K_CENTRED = TERMS == 3;
+  uint32_t q[TERMS][STEPS][2];
+  float qs[GROUPS][2];                      // sums of q over a group, scaled, of rows 2 t and 2 t + 1 (t: lane % 4)
+  float o[STEPS][4];                        // dims 16 i + g (+ 8), rows 2 t (+ 1) (g: lane / 4)
+  float bias[GROUPS][2], m[2], l[2];        // sums over this lane's keys: p (lo + 7.5 s), p
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        o[i][e] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m[e] = -INFINITY;
+      l[e] = 0.f;
+#pragma unroll
+      for (int gr = 0; gr < GROUPS; ++gr)
+        bias[gr][e] = 0.f;
+    }
+  }
+
+  // q of this lane's row (lane / 4), or none
+  __device__ __forceinline__ void load_q(const AttentionParams &p, bool live, int64_t at) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    float sum[GROUPS] = {};
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+      const int d = 32 * (k / 2) + 8 * t + 4 * (k & 1);
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = live ? load_as_float(p.a.q, p.a.dtype, at + d + e) : 0.f;
+        sum[k * 16 / kKv4Group] += x[e];
+      }
+      uint32_t lo[TERMS], hi[TERMS];
+      split<TERMS>(x[0], x[1], lo);
+      split<TERMS>(x[2], x[3], hi);
+#pragma unroll
+      for (int i = 0; i < TERMS; ++i) {
+        q[i][k][0] = lo[i];
+        q[i][k][1] = hi[i];
+      }
+    }
+#pragma unroll
+    for (int gr = 0; gr < GROUPS; ++gr) {
+      float s = sum[gr];
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      s = s - s == 0.f ? s * p.log2_scale : NAN;   // (a row with an infinity has no scores)
+      qs[gr][0] = __shfl_sync(0xffffffffu, s, 8 * t);
+      qs[gr][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+    }
+  }
+
+  // sixteen keys from j0 on; limit: keys that rows 2 t and 2 t + 1 see (only where MASKED)
+  template <bool MASKED> __device__ __forceinline__ void keys(const uint8_t *tile, float scale, int j0, const int (&limit)[2]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float s[4] = {}, vs[GROUPS][2], vb[GROUPS][2];
+    uint32_t kw[2][D / 32];
+    if constexpr (D == 128) {
+      *reinterpret_cast<uint4 *>(kw[0]) = *reinterpret_cast<const uint4 *>(tile + g * 64 + t * 16);
+      *reinterpret_cast<uint4 *>(kw[1]) = *reinterpret_cast<const uint4 *>(tile + (g + 8) * 64 + t * 16);
+    } else {
+      *reinterpret_cast<uint2 *>(kw[0]) = *reinterpret_cast<const uint2 *>(tile + g * 32 + t * 8);
+      *reinterpret_cast<uint2 *>(kw[1]) = *reinterpret_cast<const uint2 *>(tile + (g + 8) * 32 + t * 8);
+    }
+#pragma unroll
+    for (int gr = 0; gr < GROUPS; ++gr) {
+      float c[4] = {};
+#pragma unroll
+      for (int i = 2 * gr; i < 2 * gr + 2; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t a[4] = {codes<K_CENTRED>(kw[0][i], 2 * u), codes<K_CENTRED>(kw[1][i], 2 * u), codes<K_CENTRED>(kw[0][i], 2 * u + 1),
+                                 codes<K_CENTRED>(kw[1][i], 2 * u + 1)};
+#pragma unroll
+          for (int e = TERMS - 1; e >= 0; --e)
+            mma(c, a, q[e][2 * i + u][0], q[e][2 * i + u][1]);
+        }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int pair = ((g + 8 * h) * GROUPS + gr) * 4;
+        const float2 kp = __half22float2(*reinterpret_cast<const __half2 *>(tile + kv4_k_pairs(D) + pair));
+        const float2 vp = __half22float2(*reinterpret_cast<const __half2 *>(tile + kv4_v_pairs(D) + pair));
+        const float lo = fmaf(K_CENTRED ? kCentre : -kOffset, kp.x, kp.y), sc = kp.x * scale;
+        vs[gr][h] = vp.x;
+        vb[gr][h] = fmaf(kCentre, vp.x, vp.y);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          s[2 * h + e] = fmaf(c[2 * h + e], sc, fmaf(lo, qs[gr][e], s[2 * h + e]));
+      }
+    }
+    bool out[4];   // not seen
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        out[e] = j0 + g + 8 * (e >> 1) >= limit[e & 1];
+        s[e] = out[e] ? -INFINITY : s[e];
+      }
+    }
+    if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > m[0] + kLag || fmaxf(s[1], s[3]) > m[1] + kLag)) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = fmaxf(s[e], s[2 + e]);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1)
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        top = fmaxf(top, m[e]);
+        const float keep = m[e] == -INFINITY ? (l[e] == 0.f ? 0.f : 1.f) : ex2(m[e] - top);   // (a total that is NaN stays)
+        m[e] = top;
+        l[e] *= keep;
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr)
+          bias[gr][e] *= keep;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+          o[i][e] *= keep;
+          o[i][2 + e] *= keep;
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s[e] = ex2(s[e] - (m[e & 1] == -INFINITY ? 0.f : m[e & 1]));
+      l[e & 1] += s[e];
+    }
+#pragma unroll
+    for (int gr = 0; gr < GROUPS; ++gr) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = s[e] * vs[gr][e >> 1];
+        float b = fmaf(s[e], vb[gr][e >> 1], bias[gr][e & 1]);
+        if constexpr (MASKED) {   // (what is not seen may be NaN)
+          w[e] = out[e] ? 0.f : w[e];
+          b = out[e] ? bias[gr][e & 1] : b;
+        }
+        bias[gr][e & 1] = b;
+      }
+      uint32_t b0[TERMS], b1[TERMS];
+      split<TERMS>(w[0], w[1], b0);
+      split<TERMS>(w[2], w[3], b1);
+#pragma unroll
+      for (int e = 0; e < TERMS; ++e) {
+        b0[e] = transpose8(b0[e]);
+        b1[e] = transpose8(b1[e]);
+      }
+      uint32_t vw[4];
+      *reinterpret_cast<uint4 *>(vw) = *reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + gr * 512 + lane * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a[4] = {codes<true>(vw[i], 0), codes<true>(vw[i], 1), codes<true>(vw[i], 2), codes<true>(vw[i], 3)};
+        if constexpr (TERMS < 3) {
+#pragma unroll
+          for (int e = TERMS - 1; e >= 0; --e)
+            mma(o[4 * gr + i], a, b0[e], b1[e]);
+        } else {   // f32: a sum of its own, added with rounding to nearest
+          float c[4] = {};
+#pragma unroll
+          for (int e = TERMS - 1; e >= 0; --e)
+            mma(c, a, b0[e], b1[e]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[4 * gr + i][e] += c[e];
+        }
+      }
+    }
+  }
+
+  // sums over all keys of the warp
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr)
+          bias[gr][e] += __shfl_xor_sync(0xffffffffu, bias[gr][e], x);
+      }
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        o[i][e] += bias[i * 16 / kKv4Group][e];
+        o[i][2 + e] += bias[i * 16 / kKv4Group][e];
+      }
+    }
+  }
+
+  __device__ __forceinline__ void store(float *part) const {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        part[(2 * t + (e & 1)) * (D + 4) + 16 * i + g + 8 * (e >> 1)] = o[i][e];
+    if (g == 0)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        part[kRows * (D + 4) + 2 * t + e] = m[e];
+        part[kRows * (D + 4) + kRows + 2 * t + e] = l[e];
+      }
+  }
+};
+
+__device__ __forceinline__ void put(const AttentionParams &p, int64_t at, float x) {
+  if (p.a.dtype == B200_F32)
+    ((float *)p.a.out)[at] = x;
+  else if (p.a.dtype == B200_F16)
+    ((__half *)p.a.out)[at] = __float2half_rn(x);
+  else
+    ((__nv_bfloat16 *)p.a.out)[at] = __float2bfloat16_rn(x);
+}
+// element of an item's row in q (ld: q's) or out, before its dims
+__device__ __forceinline__ int64_t row_at(const AttentionParams &p, int r0, int rt, int slot, int row, int64_t ld, int D) {
+  return (r0 + (int64_t)rt * p.tokens + row / p.heads) * ld + (int64_t)((slot / p.subs) * p.G + slot % p.subs * p.heads + row % p.heads) * D;
+}
+__device__ __forceinline__ int rows_of(const AttentionParams &p, const Sequence &q, int rt, int slot) {   // of an item
+  const int tokens = min(p.tokens, q.n - rt * p.tokens);
+  return p.subs == 1 ? tokens * p.heads : min(p.heads, p.G - slot % p.subs * p.heads);
+}
+__device__ __forceinline__ float weight_of(float m, float l, float top) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(m - top); }
+
+// Where a warp stands: an item and the next of its tiles.
+struct Place {
+  int s, slot, rt, tile;
+};
+
+// A chain of parts of an item that ends in this CTA, or leaves it (by its last warp).
+struct Chain {
+  Place at;          // the item
+  int first, last;   // warps with its parts
+  bool opened;       // here: the first part is that warp's second one
+  bool ends;
+};
+
+template <int D, int TERMS> __global__ void __launch_bounds__(kThreads, 2) kv4_attention_kernel(const __grid_constant__ AttentionParams p) {
+  constexpr int BYTES = kv4_tile_bytes(D), PART = part_floats(D), RING = kStages * BYTES;
+  static_assert(RING >= PART * 4, "the second part of a warp lies in its ring");
+  extern __shared__ __align__(128) uint8_t s_all[];
+  uint8_t *s_ring = s_all;
+  float *s_part = reinterpret_cast<float *>(s_all + kWarps * RING);                                // first parts
+  long long *s_cost = reinterpret_cast<long long *>(s_all + kWarps * (RING + PART * 4));          // [n_seqs + 1]
+  __shared__ long long s_sum[kWarps];
+  __shared__ Chain s_chain[kWarps + 1];
+  __shared__ bool s_has_a[kWarps], s_a_ends[kWarps], s_has_b[kWarps];
+  __shared__ Place s_a[kWarps], s_b[kWarps];
+  __shared__ int s_n_chains, s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.a.n_seqs, room = p.a.table_stride * p.page, slots = p.kv_heads * p.subs;
   kernel_go();
   kernel_wait();
-  const b200_kv4_attention_args &a = p.a;
-  const int lane = threadIdx.x & 31;
-  const int64_t at = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (at >= (int64_t)a.rows * a.q_heads)
-    return;
-  const int row = (int)(at / a.q_heads), head = (int)(at % a.q_heads), kv = head / (a.q_heads / p.kv_heads);
-  // the last sequence that begins at or before the row
-  int lo = -1, hi = a.n_seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.row_start[mid] <= row)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  int seen = 0;
-  if (lo >= 0 && row < a.row_start[lo + 1])
-    seen = clamp((int)min((int64_t)a.lens[lo] - a.row_start[lo + 1] + row + 1, (int64_t)a.table_stride * p.page), 0, a.table_stride * p.page);
-  float q[E], acc[E] = {}, m = -INFINITY, l = 0.f;
-  bool any = false;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    q[e] = load_as_float(a.q, a.dtype, (int64_t)row * a.q_ld + (int64_t)head * D + 32 * e + lane);
-  for (int j = 0; j < seen; ++j) {
-    const int id = a.block_table[(int64_t)lo * a.table_stride + j / p.page], off = j % p.page, jj = off % kKv4Tile;
-    if (id < 0 || id >= p.n_pages)
-      continue;
-    const uint8_t *tile = p.pool + (((int64_t)id * p.kv_heads + kv) * (p.page / kKv4Tile) + off / kKv4Tile) * kv4_tile_bytes(D);
-    float s = 0.f, v[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = 32 * e + lane, pair = (jj * (D / kKv4Group) + d / kKv4Group) * 4;
-      const __half2 kp = *reinterpret_cast<const __half2 *>(tile + kv4_k_pairs(D) + pair), vp = *reinterpret_cast<const __half2 *>(tile + kv4_v_pairs(D) + pair);
-      const int kc = tile[jj * (D / 2) + d / 8 % 4 * (D / 8) + d / 32 * 4 + d % 2 * 2 + d % 8 / 4] >> (d % 4 / 2 * 4) & 15;
-      const int vc = tile[kv4_v_codes(D) + d / 64 * 512 + d % 8 * 64 + jj % 8 / 2 * 16 + d / 16 % 4 * 4 + jj % 2 * 2 + jj / 8] >> (d % 16 / 8 * 4) & 15;
-      s = fmaf(q[e], fmaf(__low2float(kp), (float)kc, __high2float(kp)), s);
-      v[e] = fmaf(__low2float(vp), (float)vc, __high2float(vp));
+
+  // ---- costs of all sequences, added up --------------------------------------------------------------------------------------
+  {
+    const int per = (n + kThreads - 1) / kThreads, first = min(n, tid * per), last = min(n, first + per);
+    long long sum = 0;
+    for (int s = first; s < last; ++s) {
+      const Sequence q(p, s, room);
+      s_cost[s] = sum;
+      sum += slots * q.before(q.tiles, p.tokens);
     }
-    s = warp_sum(s) * a.scale;
-    const float top = fmaxf(m, s), w = expf(s - top), keep = m == -INFINITY ? 0.f : expf(m - top);
-    l = fmaf(l, keep, w);
+    long long upto = sum;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      acc[e] = fmaf(acc[e], keep, w * v[e]);
-    m = top;
-    any = true;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o)
+        upto += v;
+    }
+    if (lane == 31)
+      s_sum[warp] = upto;
+    __syncthreads();
+    long long before = upto - sum;
+    for (int w = 0; w < warp; ++w)
+      before += s_sum[w];
+    for (int s = first; s < last; ++s)
+      s_cost[s] += before;
+    if (tid == kThreads - 1)
+      s_cost[n] = before + sum;
+    __syncthreads();
   }
+  // rows of no sequence
+  {
+    const int lo = clamp(p.a.row_start[0], 0, p.a.rows), hi = clamp(p.a.row_start[n], lo, p.a.rows), none = lo + p.a.rows - hi, cols = p.a.q_heads * D;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < (int64_t)none * cols; i += (int64_t)gridDim.x * kThreads) {
+      const int r = (int)(i / cols);
+      put(p, (int64_t)(r < lo ? r : hi + r - lo) * p.a.out_ld + i % cols, 0.f);
+    }
+  }
+  const long long total = s_cost[n];
+  if (total == 0)
+    return;
+  // the warps that work: sixteen keys each at least (then each begins a tile)
+  const long long workers = max(1ll, min((long long)gridDim.x * kWarps, total / 16));
+  const long long me = (long long)blockIdx.x * kWarps + warp;
+  if ((long long)blockIdx.x * kWarps >= workers)
+    return;
+  auto place = [&](long long x) {   // the first tile that begins at x or behind it
+    Place at;
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_cost[mid] <= x)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    at.s = lo;
+    const Sequence q(p, lo, room);
+    x -= s_cost[lo];
+    const long long head = q.before(q.tiles, p.tokens);
+    at.slot = (int)(x / head);
+    x -= at.slot * head;
+    int a = 0, b = q.tiles;
+    while (b - a > 1) {
+      const int mid = (a + b) >> 1;
+      if (q.before(mid, p.tokens) <= x)
+        a = mid;
+      else
+        b = mid;
+    }
+    at.rt = a;
+    at.tile = (int)((x - q.before(a, p.tokens) + 15) >> 4);
+    return at;
+  };
+  auto item_tiles = [&](const Sequence &q, int rt) { return (q.past + min((rt + 1) * p.tokens, q.n) + 15) >> 4; };
+  auto next_item = [&](Place &at, const Sequence &q) {   // (leaves the sequence: true)
+    at.tile = 0;
+    if (++at.rt < q.tiles)
+      return false;
+    at.rt = 0;
+    if (++at.slot < slots)
+      return false;
+    at.slot = 0;
+    do
+      ++at.s;
+    while (at.s < n && s_cost[at.s + 1] == s_cost[at.s]);
+    return true;
+  };
+  if (lane == 0)
+    s_has_a[warp] = s_has_b[warp] = false;
+
+  if (me < workers) {
+    Place at = place(total * me / workers);
+    const long long end = total * (me + 1) / workers;
+    Place stop{n, 0, 0, 0};
+    if (end < total)
+      stop = place(end);
+    Tile<D, TERMS> tile;
+    uint8_t *ring = s_ring + warp * RING;
+    while (at.s < n) {
+      const Sequence q(p, at.s, room);
+      const int T = item_tiles(q, at.rt);
+      if (at.tile >= T) {   // (a boundary behind an item's last tile)
+        next_item(at, q);
+        continue;
+      }
+      const bool here = stop.s == at.s && stop.slot == at.slot && stop.rt == at.rt;
+      const int t0 = at.tile, t1 = here ? min(stop.tile, T) : T;
+      if (t0 >= t1)
+        break;
+      // ---- this warp's tiles of the item ----------------------------------------------------------------------------------------
+      const int live = rows_of(p, q, at.rt, at.slot), first_token = at.rt * p.tokens, tokens = min(p.tokens, q.n - first_token);
+      const int least = clamp((long long)q.base + first_token + 1, 0, room), most = clamp((long long)q.base + first_token + tokens, 0, room);
+      const int kv = at.slot / p.subs, per_page = p.page / kKv4Tile;
+      auto source = [&](int t) {   // of lane's tile: its number in the pool, or -1
+        if (t >= t1 || t * kKv4Tile >= most)
+          return -1;
+        const int id = p.a.block_table[(int64_t)at.s * p.a.table_stride + t / per_page];
+        return id < 0 || id >= p.n_pages ? -1 : (id * p.kv_heads + kv) * per_page + t % per_page;
+      };
+      int now = source(t0 + lane), next = source(t0 + 32 + lane);
+      tile.clear();
+      uint32_t none = 0;   // bit of a stage: nothing to see in its tile
+      auto request = [&](int i) {   // tile t0 + i
+        if (i > 0 && (i & 31) == 0) {
+          now = next;
+          next = source(t0 + i + 32 + lane);
+        }
+        const int from = __shfl_sync(0xffffffffu, now, i & 31), stage = i % kStages;
+        none = from < 0 ? none | 1u << stage : none & ~(1u << stage);
+        if (from >= 0)
+          for (int c = lane; c < BYTES / 16; c += 32)
+            copy16(ring + stage * BYTES + c * 16, p.pool + (int64_t)from * BYTES + c * 16);
+        copies_commit();
+      };
+      const int count = t1 - t0;
+      __syncwarp();
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float o = any ? acc[e] / l : 0.f;
-    const int64_t to = (int64_t)row * a.out_ld + (int64_t)head * D + 32 * e + lane;
-    if (a.dtype == B200_F32)
-      ((float *)a.out)[to] = o;
-    else if (a.dtype == B200_F16)
-      ((__half *)a.out)[to] = __float2half_rn(o);
-    else
-      ((__nv_bfloat16 *)a.out)[to] = __float2bfloat16_rn(o);
+      for (int i = 0; i < kStages - 1; ++i)
+        request(i);
+      tile.load_q(p, lane / 4 < live, lane / 4 < live ? row_at(p, q.r0, at.rt, at.slot, lane / 4, p.a.q_ld, D) : 0);
+#pragma unroll 1
+      for (int i = 0; i < count; ++i) {
+        copies_wait<kStages - 2>();
+        __syncwarp();
+        const bool skip = none >> (i % kStages) & 1;
+        request(i + kStages - 1);
+        if (skip)
+          continue;
+        const int j0 = (t0 + i) * kKv4Tile;
+        const uint8_t *bytes = ring + i % kStages * BYTES;
+        int limit[2] = {0, 0};
+        if (j0 + kKv4Tile <= least) {
+          tile.template keys<false>(bytes, p.log2_scale, j0, limit);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = 2 * (lane & 3) + e;
+            limit[e] = row < live ? clamp((long long)q.base + first_token + row / p.heads + 1, 0, room) : 0;
+          }
+          tile.template keys<true>(bytes, p.log2_scale, j0, limit);
+        }
+      }
+      copies_wait<0>();
+      __syncwarp();
+      tile.finish();
+      // ---- whole, or a part -------------------------------------------------------------------------------------------------------
+      if (t0 == 0 && t1 == T) {
+        float over[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          over[e] = tile.l[e] == 0.f ? 0.f : 1.f / tile.l[e];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = 2 * (lane & 3) + e;
+          if (row < live) {
+            const int64_t to = row_at(p, q.r0, at.rt, at.slot, row, p.a.out_ld, D) + lane / 4;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              put(p, to + 16 * i, tile.l[e] == 0.f ? 0.f : tile.o[i][e] * over[e]);
+              put(p, to + 16 * i + 8, tile.l[e] == 0.f ? 0.f : tile.o[i][2 + e] * over[e]);
+            }
+          }
+        }
+      } else if (t0 > 0) {   // (only a warp's first item)
+        tile.store(s_part + warp * PART);
+        if (lane == 0) {
+          s_has_a[warp] = true;
+          s_a_ends[warp] = t1 == T;
+          s_a[warp] = at;
+        }
+      } else {               // (only its last)
+        tile.store(reinterpret_cast<float *>(ring));
+        if (lane == 0) {
+          s_has_b[warp] = true;
+          s_b[warp] = at;
+        }
+      }
+      if (here)
+        break;
+      next_item(at, q);
+    }
   }
+  __syncthreads();
+
+  // ---- parts of items: over the warps of this CTA, then over CTAs ----------------------------------------------------------------
+  if (tid == 0) {
+    int k = 0;
+    const int act = (int)min((long long)kWarps, workers - (long long)blockIdx.x * kWarps);
+    for (int w = -1; w < act; ++w) {
+      if (w < 0 ? !s_has_a[0] : !s_has_b[w])
+        continue;
+      Chain c;
+      c.opened = w >= 0;
+      c.at = w < 0 ? s_a[0] : s_b[w];
+      c.first = max(w, 0);
+      c.last = c.first;
+      c.ends = w < 0 && s_a_ends[0];
+      while (!c.ends && c.last + 1 < act) {
+        ++c.last;
+        c.ends = s_a_ends[c.last];
+      }
+      s_chain[k++] = c;
+    }
+    s_n_chains = k;
+  }
+  __syncthreads();
+  auto part_of = [&](const Chain &c, int w) { return c.opened && w == c.first ? reinterpret_cast<const float *>(s_ring + w * RING) : s_part + w * PART; };
+  for (int k = 0; k < s_n_chains; ++k) {
+    const Chain c = s_chain[k];
+    const Sequence q(p, c.at.s, room);
+    const int live = rows_of(p, q, c.at.rt, c.at.slot);
+    const bool whole = c.opened && c.ends;
+    float *mine = p.parts + ((int64_t)blockIdx.x * 2 + c.opened) * PART;
+    for (int i = tid; i < kRows * D / 4; i += kThreads) {
+      const int row = i / (D / 4), d = i % (D / 4) * 4;
+      float top = -INFINITY, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = c.first; w <= c.last; ++w)
+        top = fmaxf(top, part_of(c, w)[kRows * (D + 4) + row]);
+      for (int w = c.first; w <= c.last; ++w) {
+        const float *part = part_of(c, w), pl = part[kRows * (D + 4) + kRows + row], f = weight_of(part[kRows * (D + 4) + row], pl, top);
+        const float4 v = *reinterpret_cast<const float4 *>(part + row * (D + 4) + d);
+        l = fmaf(pl, f, l);
+        o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+      }
+      if (whole) {
+        if (row < live) {
+          const int64_t to = row_at(p, q.r0, c.at.rt, c.at.slot, row, p.a.out_ld, D) + d;
+          const float over = l == 0.f ? 0.f : 1.f / l;
+          put(p, to, l == 0.f ? 0.f : o.x * over);
+          put(p, to + 1, l == 0.f ? 0.f : o.y * over);
+          put(p, to + 2, l == 0.f ? 0.f : o.z * over);
+          put(p, to + 3, l == 0.f ? 0.f : o.w * over);
+        }
+      } else {
+        *reinterpret_cast<float4 *>(mine + row * (D + 4) + d) = o;
+        if (d == 0) {
+          mine[kRows * (D + 4) + row] = top;
+          mine[kRows * (D + 4) + kRows + row] = l;
+        }
+      }
+    }
+    if (whole)
+      continue;
+    // the CTAs with parts of this item: those of its first and last tile's workers
+    const long long begin = s_cost[c.at.s] + c.at.slot * q.before(q.tiles, p.tokens) + q.before(c.at.rt, p.tokens);
+    const long long final = begin + 16ll * (item_tiles(q, c.at.rt) - 1);
+    const int from = (int)((((begin + 1) * workers - 1) / total) / kWarps), to = (int)((((final + 1) * workers - 1) / total) / kWarps);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      const int before = atomicAdd(p.counters + from, 1);
+      s_last = before == to - from;
+      if (s_last)
+        p.counters[from] = 0;
+    }
+    __syncthreads();
+    if (!s_last)
+      continue;
+    __threadfence();
+    for (int i = tid; i < kRows * D / 4; i += kThreads) {
+      const int row = i / (D / 4), d = i % (D / 4) * 4;
+      if (row >= live)
+        continue;
+      auto part = [&](int b) { return p.parts + ((int64_t)b * 2 + (b == from)) * PART; };
+      float top = -INFINITY, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int b = from; b <= to; ++b)
+        top = fmaxf(top, __ldcg(part(b) + kRows * (D + 4) + row));
+      for (int b = from; b <= to; ++b) {
+        const float pl = __ldcg(part(b) + kRows * (D + 4) + kRows + row), f = weight_of(__ldcg(part(b) + kRows * (D + 4) + row), pl, top);
+        const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(b) + row * (D + 4) + d));
+        l = fmaf(pl, f, l);
+        o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+      }
+      const int64_t at = row_at(p, q.r0, c.at.rt, c.at.slot, row, p.a.out_ld, D) + d;
+      const float over = l == 0.f ? 0.f : 1.f / l;
+      put(p, at, l == 0.f ? 0.f : o.x * over);
+      put(p, at + 1, l == 0.f ? 0.f : o.y * over);
+      put(p, at + 2, l == 0.f ? 0.f : o.z * over);
+      put(p, at + 3, l == 0.f ? 0.f : o.w * over);
+    }
+  }
+}
+
+RaisedOn g_raised[6];
+
+template <int D, int TERMS> int attention_launch(RaisedOn &raised, const AttentionParams &p, cudaStream_t st) {
+  const int fixed = kWarps * (kStages * kv4_tile_bytes(D) + part_floats(D) * 4);
+  if (int rc = raise_shared_limit(raised, (const void *)kv4_attention_kernel<D, TERMS>, fixed + 8 * (B200_KV4_ATTENTION_MAX_SEQS + 1)))
+    return rc;
+  return launch_after(kv4_attention_kernel<D, TERMS>, dim3(kCtas), kThreads, fixed + 8 * (p.a.n_seqs + 1), st, p);
 }
 
 } // namespace
@@ -91,7 +680,7 @@ extern "C" {
 int64_t b200_kv4_attention_workspace_bytes(int q_heads, int kv_heads, int head_dim) {
   if (kv_heads < 1 || kv_heads > 1024 || q_heads < 1 || q_heads % kv_heads != 0 || (head_dim != 64 && head_dim != 128))
     return B200_EINVAL;
-  return 256;
+  return 2048 + (int64_t)kCtas * 2 * part_floats(head_dim) * 4;
 }
 
 int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a, void *workspace, int64_t workspace_bytes, void *stream) {
@@ -121,10 +710,21 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
                 (long long)b200_kv4_attention_workspace_bytes(a->q_heads, c->kv_heads, c->head_dim));
   if (int rc = ensure_device())
     return rc;
-  const AttentionParams p{(const uint8_t *)c->pool, c->n_pages, c->kv_heads, c->page, *a};
-  const dim3 grid((unsigned)(((int64_t)a->rows * a->q_heads + kThreads / 32 - 1) / (kThreads / 32)));
-  return c->head_dim == 128 ? launch_after(kv4_attention_kernel<128>, grid, kThreads, 0, (cudaStream_t)stream, p)
-                            : launch_after(kv4_attention_kernel<64>, grid, kThreads, 0, (cudaStream_t)stream, p);
+  AttentionParams p{(const uint8_t *)c->pool, c->n_pages, c->kv_heads, c->page, *a};
+  p.G = a->q_heads / c->kv_heads;
+  p.subs = (p.G + kRows - 1) / kRows;
+  p.heads = std::min(p.G, kRows);
+  p.tokens = p.subs == 1 ? kRows / p.G : 1;
+  p.log2_scale = a->scale * 1.4426950408889634f;
+  p.counters = (int *)workspace;
+  p.parts = (float *)((char *)workspace + 2048);
+  cudaStream_t st = (cudaStream_t)stream;
+#define B200_D(D_)                                                                                                                    \
+  (a->dtype == B200_F32   ? attention_launch<D_, 3>(g_raised[D_ / 64 - 1], p, st)                                                     \
+   : a->dtype == B200_F16 ? attention_launch<D_, 2>(g_raised[D_ / 64 + 1], p, st)                                                     \
+                          : attention_launch<D_, 1>(g_raised[D_ / 64 + 3], p, st))
+  return c->head_dim == 128 ? B200_D(128) : B200_D(64);
+#undef B200_D
 }
 
 } // extern "C"

@@ -214,10 +214,10 @@ def bound(kind, S, V, n):
     """Of an output's error.  S: the largest sum of |q||k| of a score; V: the largest |v|; n: keys.
     A score: at most 2^-20 S (f32 sums of sixteen terms at a time that round towards zero, 2^-23 each, six in a row for a group, three products
     where an operand is split; parameters' products), so weights 2^-19 S, in the sum and the total.  A sum of n weighted values: 2^-23 for every
-    sixteen keys, at most 64 times in a row before it goes to another sum.  Weights as operands: half a step of the type (f16: two bf16 terms),
+    sixteen keys, and some for the sums of warps and CTAs.  Weights as operands: half a step of the type (f16: two bf16 terms),
     exponentials 2^-21.  The output's own rounding.  All relative to V, which bounds each sum of weighted values over the sum of weights."""
     weight = {"f32": 2.0 ** -22, "f16": 2.0 ** -16, "bf16": 2.0 ** -8}[kind]
-    sums = min(n / 16 + 8, 80) * 2.0 ** -23
+    sums = (n / 16 + 16) * 2.0 ** -23
     return V * (2.0 ** -18 * S + 2 * sums + 2.0 ** -20 + weight) + V * HALF[kind] + 2.0 ** -25
 
 
