@@ -2,9 +2,13 @@
 //
 // Codes go to the tensor cores as they are: with k = lo + s c per group of 64 dims, a score is  q.k = sum over groups of s (q.c) + lo sum(q),  and
 // an output  sum p v = sum (p s) c + sum p lo,  so that scales meet scores and weights (a handful per key) instead of 64 codes each.  A code is one
-// bf16 exactly; the other operand is split into as many bf16 terms as its type needs.  Codes are the operand with M rows (mma.m16n8k16: sixteen
-// positions, or sixteen dims), the query rows that share a kv head the eight columns; words of eight codes lie in the cache as the
-// operand's registers want them, and one and-or makes a pair of codes a pair of bf16 (16 + c: the code in the mantissa's upper bits).
+// f16 exactly; the other operand is one f16 (f32: two, 22 bits of it) after a power of two of its row that puts the row's largest near f16's.
+// Codes are the operand with M rows (mma.m16n8k16: sixteen positions, or sixteen dims), the query rows that share a kv head the eight
+// columns; words of eight codes lie in the cache as the operand's registers want them, and one and-or makes a pair of codes a pair of
+// f16 (1024 + c, or 1024 + 16 c: the code in the mantissa's low bits).
+//
+// The reference r of a row's weights is not its largest score but the largest of score + log2 of the key's larger V scale, so that the weights
+// that meet codes, p s, are at most 2^12 and near 2^8 where they count, whatever the scales are; sums and totals carry the same factor.
 #include "kv4.cuh"
 
 #include <algorithm>
@@ -16,7 +20,10 @@ namespace {
 constexpr int kWarps = 8, kThreads = 32 * kWarps, kCtas = 296;
 constexpr int kRows = 8;            // query rows of an item: a position's heads (several positions', if they are few)
 constexpr int kStages = 3;          // tiles that a warp has in flight or in hand
-constexpr float kLag = 8.f;         // a row's maximum is renewed when a score is this far above it (powers of two)
+constexpr float kTop = 8.f;          // powers of two: what the largest weight p s is at when a row's reference is set,
+constexpr float kLag = 4.f;          // and how far above that one may come before it is set again
+constexpr float kSeed = -1.0e30f;
+constexpr float kLeastScale = 5.9604645e-8f;   // (f16's smallest: a group of equal values has the scale 0)
 
 struct AttentionParams {
   const uint8_t *pool;
@@ -36,20 +43,24 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ float low_of(uint32_t pair) { return __uint_as_float(pair << 16); }
-__device__ __forceinline__ float high_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
+__device__ __forceinline__ float2 halves(uint32_t pair) { return __half22float2(*reinterpret_cast<const __half2 *>(&pair)); }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -59,26 +70,28 @@ __device__ __forceinline__ void copy16(void *to, const void *from) {
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// Codes 0..15 of nibbles p and p + 4 as a pair of bf16: 16 + c, or (CENTRED) c - 7.5.  Both exact.  Centred operands keep a sum of n
-// weighted codes as small as the values' own spread: the tensor cores' sums round towards zero, and would lose 5 sqrt(n) times as much.
-constexpr float kOffset = 16.f, kCentre = 7.5f;
-template <bool CENTRED> __device__ __forceinline__ uint32_t codes(uint32_t w, int p) {
-  const uint32_t x = ((p == 0 ? w << 3 : w >> (4 * p - 3)) & 0x00780078u) | 0x41804180u;
-  if constexpr (!CENTRED)
-    return x;
-  uint32_t y;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(0x3f803f80u), "r"(0xc1bcc1bcu));   // * 1 - 23.5
-  return y;
+// Codes of nibbles p and p + 4 of w >> 8 * (p / 2), p = 0 and 1, as pairs of f16: 1024 + c and 1024 + 16 c as they come, or (CENTRED) c - 8.  All exact.
+// Centred operands keep a sum of n weighted codes as small as the values' own spread: the tensor cores' sums round towards zero.
+constexpr float kCentre = 8.f;
+constexpr float kOffset = 1024.f;   // not centred: of the products with q (lo), and with q / 16 (hi)
+template <bool CENTRED> __device__ __forceinline__ void codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  lo = (w & 0x000f000fu) | 0x64006400u;
+  hi = (w & 0x00f000f0u) | 0x64006400u;
+  if constexpr (CENTRED) {
+    asm("add.rn.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(0xe408e408u));                                   // - 1032
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(hi) : "r"(0x2c002c00u), "r"(0xd480d480u));             // / 16 - 72
+  }
 }
 
-// x as TERMS bf16 that add up to it (f16: two are exact, f32: three), pairs of two values
+// x and y as TERMS f16 each
 template <int TERMS> __device__ __forceinline__ void split(float x, float y, uint32_t (&t)[TERMS]) {
 #pragma unroll
   for (int i = 0; i < TERMS; ++i) {
-    t[i] = pack_bf16(x, y);
+    t[i] = pack_f16(x, y);
     if (i + 1 < TERMS) {
-      x -= low_of(t[i]);
-      y -= high_of(t[i]);
+      const float2 f = halves(t[i]);
+      x -= f.x;
+      y -= f.y;
     }
   }
 }
@@ -102,13 +115,16 @@ struct Sequence {
   }
 };
 
-template <int D, int TERMS> struct Tile {   // of a warp: one item's sums
-  static constexpr int GROUPS = D / kKv4Group, STEPS = D / 16;
-  static constexpr bool K_CENTRED = TERMS == 3;
+template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
+  static constexpr int GROUPS = D / kKv4Group, STEPS = D / 16, TERMS = TYPE == B200_F32 ? 2 : 1;
+  // K's codes: a score of bf16 queries does not notice that 1024 + c costs it 2^-13 of the sum of |q s|; f16 would
+  static constexpr bool K_CENTRED = TYPE != B200_BF16;
   uint32_t q[TERMS][STEPS][2];
-  float qs[GROUPS][2];                      // sums of q over a group, scaled, of rows 2 t and 2 t + 1 (t: lane % 4)
+  float qs[GROUPS][2];                      // sums of q over a group, times the scores' scale, of rows 2 t and 2 t + 1 (t: lane % 4)
+  float minus[K_CENTRED ? 1 : GROUPS][2];   // what the offsets of codes add up to, negative
+  float unit[2];                            // the scores' scale over the row's power of two
   float o[STEPS][4];                        // dims 16 i + g (+ 8), rows 2 t (+ 1) (g: lane / 4)
-  float bias[GROUPS][2], m[2], l[2];        // sums over this lane's keys: p (lo + 7.5 s), p
+  float bias[GROUPS][2], r[2], l[2];        // sums over this lane's keys: p (lo + 8 s), p
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -118,7 +134,7 @@ template <int D, int TERMS> struct Tile {   // of a warp: one item's sums
         o[i][e] = 0.f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      m[e] = -INFINITY;
+      r[e] = kSeed;
       l[e] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < GROUPS; ++gr)
@@ -129,92 +145,146 @@ template <int D, int TERMS> struct Tile {   // of a warp: one item's sums
   // q of this lane's row (lane / 4), or none
   __device__ __forceinline__ void load_q(const AttentionParams &p, bool live, int64_t at) {
     const int lane = threadIdx.x & 31, t = lane & 3;
-    float sum[GROUPS] = {};
+    float x[STEPS][4], most = 0.f;
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) {
       const int d = 32 * (k / 2) + 8 * t + 4 * (k & 1);
-      float x[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[e] = live ? load_as_float(p.a.q, p.a.dtype, at + d + e) : 0.f;
-        sum[k * 16 / kKv4Group] += x[e];
-      }
-      uint32_t lo[TERMS], hi[TERMS];
-      split<TERMS>(x[0], x[1], lo);
-      split<TERMS>(x[2], x[3], hi);
-#pragma unroll
-      for (int i = 0; i < TERMS; ++i) {
-        q[i][k][0] = lo[i];
-        q[i][k][1] = hi[i];
+        x[k][e] = live ? load_as_float(p.a.q, TYPE, at + d + e) : 0.f;
+        most = fmaxf(most, fabsf(x[k][e]));
       }
     }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    // 2^up: the row's largest comes to 2^14 .. 2^15 (a row below 2^-86 not as far)
+    const int up = min(max(14 + 127 - (int)(__float_as_uint(most) >> 23), -113), 100);
+    const float factor = __uint_as_float((uint32_t)(127 + up) << 23), over = p.log2_scale * __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      unit[e] = __shfl_sync(0xffffffffu, over, 8 * t + 4 * e);
 #pragma unroll
     for (int gr = 0; gr < GROUPS; ++gr) {
-      float s = sum[gr];
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      s = s - s == 0.f ? s * p.log2_scale : NAN;   // (a row with an infinity has no scores)
-      qs[gr][0] = __shfl_sync(0xffffffffu, s, 8 * t);
-      qs[gr][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+      float sum = 0.f, off = 0.f;
+#pragma unroll
+      for (int k = 4 * gr; k < 4 * gr + 4; ++k) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sum += x[k][e];
+          y[e] = x[k][e] * factor;
+          if constexpr (!K_CENTRED) {
+            y[e] = __half2float(__float2half_rn(e / 2 == 0 ? y[e] : y[e] * 0.0625f));
+            off = fmaf(kOffset, y[e], off);
+          }
+        }
+        uint32_t lo[TERMS], hi[TERMS];
+        split<TERMS>(y[0], y[1], lo);
+        split<TERMS>(y[2], y[3], hi);
+#pragma unroll
+        for (int i = 0; i < TERMS; ++i) {
+          q[i][k][0] = lo[i];
+          q[i][k][1] = hi[i];
+        }
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum = sum - sum == 0.f ? sum * p.log2_scale : NAN;   // (a row with an infinity has no scores)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        qs[gr][e] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
+      if constexpr (!K_CENTRED) {
+        off += __shfl_xor_sync(0xffffffffu, off, 1);
+        off += __shfl_xor_sync(0xffffffffu, off, 2);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          minus[gr][e] = -__shfl_sync(0xffffffffu, off, 8 * t + 4 * e);
+      }
     }
   }
 
   // sixteen keys from j0 on; limit: keys that rows 2 t and 2 t + 1 see (only where MASKED)
-  template <bool MASKED> __device__ __forceinline__ void keys(const uint8_t *tile, float scale, int j0, const int (&limit)[2]) {
+  template <bool MASKED> __device__ __forceinline__ void keys(const uint8_t *tile, int j0, const int (&limit)[2]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    float s[4] = {}, vs[GROUPS][2], vb[GROUPS][2];
-    uint32_t kw[2][D / 32];
-    if constexpr (D == 128) {
-      *reinterpret_cast<uint4 *>(kw[0]) = *reinterpret_cast<const uint4 *>(tile + g * 64 + t * 16);
-      *reinterpret_cast<uint4 *>(kw[1]) = *reinterpret_cast<const uint4 *>(tile + (g + 8) * 64 + t * 16);
-    } else {
-      *reinterpret_cast<uint2 *>(kw[0]) = *reinterpret_cast<const uint2 *>(tile + g * 32 + t * 8);
-      *reinterpret_cast<uint2 *>(kw[1]) = *reinterpret_cast<const uint2 *>(tile + (g + 8) * 32 + t * 8);
+    uint32_t kw[2][D / 32], kp[2][GROUPS], vp[2][GROUPS];   // of keys g and g + 8
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = g + 8 * h;
+      if constexpr (D == 128) {
+        *reinterpret_cast<uint4 *>(kw[h]) = *reinterpret_cast<const uint4 *>(tile + j * 64 + t * 16);
+        *reinterpret_cast<uint2 *>(kp[h]) = *reinterpret_cast<const uint2 *>(tile + kv4_k_pairs(D) + j * 8);
+        *reinterpret_cast<uint2 *>(vp[h]) = *reinterpret_cast<const uint2 *>(tile + kv4_v_pairs(D) + j * 8);
+      } else {
+        *reinterpret_cast<uint2 *>(kw[h]) = *reinterpret_cast<const uint2 *>(tile + j * 32 + t * 8);
+        kp[h][0] = *reinterpret_cast<const uint32_t *>(tile + kv4_k_pairs(D) + j * 4);
+        vp[h][0] = *reinterpret_cast<const uint32_t *>(tile + kv4_v_pairs(D) + j * 4);
+      }
     }
+    float dot[4] = {}, low[4] = {};
 #pragma unroll
     for (int gr = 0; gr < GROUPS; ++gr) {
-      float c[4] = {};
+      float c[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        c[e] = K_CENTRED ? 0.f : minus[K_CENTRED ? 0 : gr][e & 1];
 #pragma unroll
       for (int i = 2 * gr; i < 2 * gr + 2; ++i)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const uint32_t a[4] = {codes<K_CENTRED>(kw[0][i], 2 * u), codes<K_CENTRED>(kw[1][i], 2 * u), codes<K_CENTRED>(kw[0][i], 2 * u + 1),
-                                 codes<K_CENTRED>(kw[1][i], 2 * u + 1)};
+          uint32_t a[4];
+          codes<K_CENTRED>(kw[0][i] >> (8 * u), a[0], a[2]);
+          codes<K_CENTRED>(kw[1][i] >> (8 * u), a[1], a[3]);
 #pragma unroll
           for (int e = TERMS - 1; e >= 0; --e)
             mma(c, a, q[e][2 * i + u][0], q[e][2 * i + u][1]);
         }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int pair = ((g + 8 * h) * GROUPS + gr) * 4;
-        const float2 kp = __half22float2(*reinterpret_cast<const __half2 *>(tile + kv4_k_pairs(D) + pair));
-        const float2 vp = __half22float2(*reinterpret_cast<const __half2 *>(tile + kv4_v_pairs(D) + pair));
-        const float lo = fmaf(K_CENTRED ? kCentre : -kOffset, kp.x, kp.y), sc = kp.x * scale;
-        vs[gr][h] = vp.x;
-        vb[gr][h] = fmaf(kCentre, vp.x, vp.y);
+        const float2 pair = halves(kp[h][gr]);
+        const float lo = K_CENTRED ? fmaf(kCentre, pair.x, pair.y) : pair.y;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          s[2 * h + e] = fmaf(c[2 * h + e], sc, fmaf(lo, qs[gr][e], s[2 * h + e]));
+        for (int e = 0; e < 2; ++e) {
+          dot[2 * h + e] = fmaf(c[2 * h + e], pair.x, dot[2 * h + e]);
+          low[2 * h + e] = fmaf(lo, qs[gr][e], low[2 * h + e]);
+        }
       }
     }
+    float s[4], at[4], vs[GROUPS][2], vb[GROUPS][2];
     bool out[4];   // not seen
-    if constexpr (MASKED) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        out[e] = j0 + g + 8 * (e >> 1) >= limit[e & 1];
-        s[e] = out[e] ? -INFINITY : s[e];
+    for (int h = 0; h < 2; ++h) {
+      float largest = kLeastScale;
+#pragma unroll
+      for (int gr = 0; gr < GROUPS; ++gr) {
+        const float2 pair = halves(vp[h][gr]);
+        vs[gr][h] = pair.x;
+        vb[gr][h] = fmaf(kCentre, pair.x, pair.y);
+        largest = fmaxf(largest, pair.x);
       }
-    }
-    if (__any_sync(0xffffffffu, fmaxf(s[0], s[2]) > m[0] + kLag || fmaxf(s[1], s[3]) > m[1] + kLag)) {
+      const float height = lg2(largest);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float top = fmaxf(s[e], s[2 + e]);
+        const int k = 2 * h + e;
+        s[k] = fmaf(dot[k], unit[e], low[k]);
+        if constexpr (MASKED) {
+          out[k] = j0 + g + 8 * h >= limit[e];
+          s[k] = out[k] ? -INFINITY : s[k];
+        }
+        at[k] = s[k] + height;
+        if constexpr (MASKED)
+          at[k] = out[k] ? -INFINITY : at[k];
+      }
+    }
+    if (__any_sync(0xffffffffu, fmaxf(at[0], at[2]) > r[0] + (kTop + kLag) || fmaxf(at[1], at[3]) > r[1] + (kTop + kLag))) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = fmaxf(at[e], at[2 + e]);
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1)
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        top = fmaxf(top, m[e]);
-        const float keep = m[e] == -INFINITY ? (l[e] == 0.f ? 0.f : 1.f) : ex2(m[e] - top);   // (a total that is NaN stays)
-        m[e] = top;
+        top = fmaxf(top - kTop, r[e]);
+        const float keep = ex2(r[e] - top);
+        r[e] = top;
         l[e] *= keep;
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr)
@@ -228,7 +298,7 @@ template <int D, int TERMS> struct Tile {   // of a warp: one item's sums
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      s[e] = ex2(s[e] - (m[e & 1] == -INFINITY ? 0.f : m[e & 1]));
+      s[e] = ex2(s[e] - r[e & 1]);
       l[e & 1] += s[e];
     }
 #pragma unroll
@@ -256,11 +326,11 @@ template <int D, int TERMS> struct Tile {   // of a warp: one item's sums
       *reinterpret_cast<uint4 *>(vw) = *reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + gr * 512 + lane * 16);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t a[4] = {codes<true>(vw[i], 0), codes<true>(vw[i], 1), codes<true>(vw[i], 2), codes<true>(vw[i], 3)};
-        if constexpr (TERMS < 3) {
-#pragma unroll
-          for (int e = TERMS - 1; e >= 0; --e)
-            mma(o[4 * gr + i], a, b0[e], b1[e]);
+        uint32_t a[4];
+        codes<true>(vw[i], a[0], a[1]);
+        codes<true>(vw[i] >> 8, a[2], a[3]);
+        if constexpr (TERMS == 1) {
+          mma(o[4 * gr + i], a, b0[0], b1[0]);
         } else {   // f32: a sum of its own, added with rounding to nearest
           float c[4] = {};
 #pragma unroll
@@ -303,7 +373,7 @@ template <int D, int TERMS> struct Tile {   // of a warp: one item's sums
     if (g == 0)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        part[kRows * (D + 4) + 2 * t + e] = m[e];
+        part[kRows * (D + 4) + 2 * t + e] = r[e];
         part[kRows * (D + 4) + kRows + 2 * t + e] = l[e];
       }
   }
@@ -325,8 +395,6 @@ __device__ __forceinline__ int rows_of(const AttentionParams &p, const Sequence 
   const int tokens = min(p.tokens, q.n - rt * p.tokens);
   return p.subs == 1 ? tokens * p.heads : min(p.heads, p.G - slot % p.subs * p.heads);
 }
-__device__ __forceinline__ float weight_of(float m, float l, float top) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(m - top); }
-
 // Where a warp stands: an item and the next of its tiles.
 struct Place {
   int s, slot, rt, tile;
@@ -340,7 +408,7 @@ struct Chain {
   bool ends;
 };
 
-template <int D, int TERMS> __global__ void __launch_bounds__(kThreads, 2) kv4_attention_kernel(const __grid_constant__ AttentionParams p) {
+template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 2) kv4_attention_kernel(const __grid_constant__ AttentionParams p) {
   constexpr int BYTES = kv4_tile_bytes(D), PART = part_floats(D), RING = kStages * BYTES;
   static_assert(RING >= PART * 4, "the second part of a warp lies in its ring");
   extern __shared__ __align__(128) uint8_t s_all[];
@@ -451,7 +519,7 @@ template <int D, int TERMS> __global__ void __launch_bounds__(kThreads, 2) kv4_a
     Place stop{n, 0, 0, 0};
     if (end < total)
       stop = place(end);
-    Tile<D, TERMS> tile;
+    Tile<D, TYPE> tile;
     uint8_t *ring = s_ring + warp * RING;
     while (at.s < n) {
       const Sequence q(p, at.s, room);
@@ -477,17 +545,25 @@ template <int D, int TERMS> __global__ void __launch_bounds__(kThreads, 2) kv4_a
       int now = source(t0 + lane), next = source(t0 + 32 + lane);
       tile.clear();
       uint32_t none = 0;   // bit of a stage: nothing to see in its tile
+      int ahead = 0, hand = 0;      // stages: of the next tile to ask for, of the tile in hand
       auto request = [&](int i) {   // tile t0 + i
         if (i > 0 && (i & 31) == 0) {
           now = next;
           next = source(t0 + i + 32 + lane);
         }
-        const int from = __shfl_sync(0xffffffffu, now, i & 31), stage = i % kStages;
-        none = from < 0 ? none | 1u << stage : none & ~(1u << stage);
-        if (from >= 0)
-          for (int c = lane; c < BYTES / 16; c += 32)
-            copy16(ring + stage * BYTES + c * 16, p.pool + (int64_t)from * BYTES + c * 16);
+        const int from = __shfl_sync(0xffffffffu, now, i & 31);
+        none = from < 0 ? none | 1u << ahead : none & ~(1u << ahead);
+        if (from >= 0) {
+          const uint8_t *src = p.pool + (int64_t)from * BYTES + lane * 16;
+          uint8_t *to = ring + ahead * BYTES + lane * 16;
+#pragma unroll
+          for (int c = 0; c < BYTES / 512; ++c)
+            copy16(to + c * 512, src + c * 512);
+          if (BYTES % 512 != 0 && lane < BYTES % 512 / 16)
+            copy16(to + BYTES / 512 * 512, src + BYTES / 512 * 512);
+        }
         copies_commit();
+        ahead = ahead == kStages - 1 ? 0 : ahead + 1;
       };
       const int count = t1 - t0;
       __syncwarp();
@@ -499,22 +575,23 @@ template <int D, int TERMS> __global__ void __launch_bounds__(kThreads, 2) kv4_a
       for (int i = 0; i < count; ++i) {
         copies_wait<kStages - 2>();
         __syncwarp();
-        const bool skip = none >> (i % kStages) & 1;
+        const bool skip = none >> hand & 1;
+        const uint8_t *bytes = ring + hand * BYTES;
+        hand = hand == kStages - 1 ? 0 : hand + 1;
         request(i + kStages - 1);
         if (skip)
           continue;
         const int j0 = (t0 + i) * kKv4Tile;
-        const uint8_t *bytes = ring + i % kStages * BYTES;
         int limit[2] = {0, 0};
         if (j0 + kKv4Tile <= least) {
-          tile.template keys<false>(bytes, p.log2_scale, j0, limit);
+          tile.template keys<false>(bytes, j0, limit);
         } else {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int row = 2 * (lane & 3) + e;
             limit[e] = row < live ? clamp((long long)q.base + first_token + row / p.heads + 1, 0, room) : 0;
           }
-          tile.template keys<true>(bytes, p.log2_scale, j0, limit);
+          tile.template keys<true>(bytes, j0, limit);
         }
       }
       copies_wait<0>();
@@ -590,12 +667,12 @@ template <int D, int TERMS> __global__ void __launch_bounds__(kThreads, 2) kv4_a
     float *mine = p.parts + ((int64_t)blockIdx.x * 2 + c.opened) * PART;
     for (int i = tid; i < kRows * D / 4; i += kThreads) {
       const int row = i / (D / 4), d = i % (D / 4) * 4;
-      float top = -INFINITY, l = 0.f;
+      float top = kSeed, l = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int w = c.first; w <= c.last; ++w)
         top = fmaxf(top, part_of(c, w)[kRows * (D + 4) + row]);
       for (int w = c.first; w <= c.last; ++w) {
-        const float *part = part_of(c, w), pl = part[kRows * (D + 4) + kRows + row], f = weight_of(part[kRows * (D + 4) + row], pl, top);
+        const float *part = part_of(c, w), pl = part[kRows * (D + 4) + kRows + row], f = ex2(part[kRows * (D + 4) + row] - top);
         const float4 v = *reinterpret_cast<const float4 *>(part + row * (D + 4) + d);
         l = fmaf(pl, f, l);
         o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
@@ -640,12 +717,12 @@ template <int D, int TERMS> __global__ void __launch_bounds__(kThreads, 2) kv4_a
       if (row >= live)
         continue;
       auto part = [&](int b) { return p.parts + ((int64_t)b * 2 + (b == from)) * PART; };
-      float top = -INFINITY, l = 0.f;
+      float top = kSeed, l = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int b = from; b <= to; ++b)
         top = fmaxf(top, __ldcg(part(b) + kRows * (D + 4) + row));
       for (int b = from; b <= to; ++b) {
-        const float pl = __ldcg(part(b) + kRows * (D + 4) + kRows + row), f = weight_of(__ldcg(part(b) + kRows * (D + 4) + row), pl, top);
+        const float pl = __ldcg(part(b) + kRows * (D + 4) + kRows + row), f = ex2(__ldcg(part(b) + kRows * (D + 4) + row) - top);
         const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(b) + row * (D + 4) + d));
         l = fmaf(pl, f, l);
         o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
@@ -662,11 +739,11 @@ template <int D, int TERMS> __global__ void __launch_bounds__(kThreads, 2) kv4_a
 
 RaisedOn g_raised[6];
 
-template <int D, int TERMS> int attention_launch(RaisedOn &raised, const AttentionParams &p, cudaStream_t st) {
+template <int D, int TYPE> int attention_launch(RaisedOn &raised, const AttentionParams &p, cudaStream_t st) {
   const int fixed = kWarps * (kStages * kv4_tile_bytes(D) + part_floats(D) * 4);
-  if (int rc = raise_shared_limit(raised, (const void *)kv4_attention_kernel<D, TERMS>, fixed + 8 * (B200_KV4_ATTENTION_MAX_SEQS + 1)))
+  if (int rc = raise_shared_limit(raised, (const void *)kv4_attention_kernel<D, TYPE>, fixed + 8 * (B200_KV4_ATTENTION_MAX_SEQS + 1)))
     return rc;
-  return launch_after(kv4_attention_kernel<D, TERMS>, dim3(kCtas), kThreads, fixed + 8 * (p.a.n_seqs + 1), st, p);
+  return launch_after(kv4_attention_kernel<D, TYPE>, dim3(kCtas), kThreads, fixed + 8 * (p.a.n_seqs + 1), st, p);
 }
 
 } // namespace
@@ -720,9 +797,9 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
   p.parts = (float *)((char *)workspace + 2048);
   cudaStream_t st = (cudaStream_t)stream;
 #define B200_D(D_)                                                                                                                    \
-  (a->dtype == B200_F32   ? attention_launch<D_, 3>(g_raised[D_ / 64 - 1], p, st)                                                     \
-   : a->dtype == B200_F16 ? attention_launch<D_, 2>(g_raised[D_ / 64 + 1], p, st)                                                     \
-                          : attention_launch<D_, 1>(g_raised[D_ / 64 + 3], p, st))
+  (a->dtype == B200_F32   ? attention_launch<D_, B200_F32>(g_raised[D_ / 64 - 1], p, st)                                              \
+   : a->dtype == B200_F16 ? attention_launch<D_, B200_F16>(g_raised[D_ / 64 + 1], p, st)                                              \
+                          : attention_launch<D_, B200_BF16>(g_raised[D_ / 64 + 3], p, st))
   return c->head_dim == 128 ? B200_D(128) : B200_D(64);
 #undef B200_D
 }

@@ -354,9 +354,8 @@ int b200_page_step(const b200_page_step_args *a, void *stream);
  * all can stand in one call.  q head h reads kv head h / (q_heads / kv_heads).
  *   out = softmax(scale * q K^T) V   with the values of the cache,
  * scores, sums and products with f32 accumulators, rounded to `dtype` once.
- * dtype f32: both products as exact as f32 (the other operand is split into bf16
- * terms, codes are exact); bf16 and f16: q exactly, the weights to 2^-8 and
- * 2^-16 of themselves.  A row that sees no position is zero, and so are the rows
+ * codes exactly.  dtype f32: q and the weights to 2^-22 of themselves; bf16 and
+ * f16: q exactly (elements down to 2^-28 of their row's largest), the weights to 2^-11.  A row that sees no position is zero, and so are the rows
  * before row_start[0] and behind the last sequence's.  Positions beyond
  * table_stride * page, and those whose table entry is no page of the pool, are
  * not seen.  Nothing that a row does not see (infinities and NaN included)
