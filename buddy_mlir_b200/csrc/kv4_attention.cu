@@ -4,8 +4,8 @@
 // an output  sum p v = sum (p s) c + sum p lo,  so that scales meet scores and weights (a handful per key) instead of 64 codes each.  A code is one
 // f16 exactly; the other operand is one f16 (f32: two, 22 bits of it) after a power of two of its row that puts the row's largest near f16's.
 // Codes are the operand with M rows (mma.m16n8k16: sixteen positions, or sixteen dims), the query rows that share a kv head the eight
-// columns; words of eight codes lie in the cache as the operand's registers want them, and one and-or makes a pair of codes a pair of
-// f16 (1024 + c, or 1024 + 16 c: the code in the mantissa's low bits).
+// columns; words of eight codes lie in the cache as the operand's registers want them, and one AND makes a pair of codes a pair of
+// f16: nibbles 0 and 1 of a half-word are the subnormal numbers c 2^-24 and c 2^-20, which the tensor cores multiply exactly.
 //
 // The reference r of a row's weights is not its largest score but the largest of score + log2 of the key's larger V scale, so that the weights
 // that meet codes, p s, are at most 2^12 and near 2^8 where they count, whatever the scales are; sums and totals carry the same factor.
@@ -17,9 +17,12 @@ namespace b200 {
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps, kCtas = 296;
+constexpr int kWarps = 16, kThreads = 32 * kWarps, kCtas = 148;
 constexpr int kRows = 8;            // query rows of an item: a position's heads (several positions', if they are few)
-constexpr int kStages = 3;          // tiles that a warp has in flight or in hand
+constexpr int kSlots = 4;           // tiles that a warp has in flight or in hand
+constexpr int kLeastKeys = 512;     // of a CTA, where there are not more CTAs than that asks for
+constexpr int kSnap = 256;          // keys that a CTA may have more or fewer, so that it begins with an item (few of many: a quarter)
+constexpr int kMany = 4096;
 constexpr float kTop = 8.f;          // powers of two: what the largest weight p s is at when a row's reference is set,
 constexpr float kLag = 4.f;          // and how far above that one may come before it is set again
 constexpr float kSeed = -1.0e30f;
@@ -31,8 +34,9 @@ struct AttentionParams {
   b200_kv4_attention_args a;
   int G, heads, tokens, subs;       // q heads of a kv head, of an item; positions of an item; items that share a kv head's q heads
   float log2_scale;
+  bool wide_q;                      // rows of q are aligned to four elements
   int *counters;                    // [kCtas]
-  float *parts;                     // [kCtas][2][part floats]
+  float *parts;                     // [kCtas][2][part floats], then [kCtas * kWarps][part floats]
 };
 
 __host__ __device__ constexpr int part_floats(int D) { return kRows * (D + 4) + 2 * kRows; }   // sums in rows of D + 4, maxima, totals
@@ -70,18 +74,25 @@ __device__ __forceinline__ void copy16(void *to, const void *from) {
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// Codes of nibbles p and p + 4 of w >> 8 * (p / 2), p = 0 and 1, as pairs of f16: 1024 + c and 1024 + 16 c as they come, or (CENTRED) c - 8.  All exact.
-// Centred operands keep a sum of n weighted codes as small as the values' own spread: the tensor cores' sums round towards zero.
-constexpr float kCentre = 8.f;
-constexpr float kOffset = 1024.f;   // not centred: of the products with q (lo), and with q / 16 (hi)
-template <bool CENTRED> __device__ __forceinline__ void codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
-  lo = (w & 0x000f000fu) | 0x64006400u;
-  hi = (w & 0x00f000f0u) | 0x64006400u;
-  if constexpr (CENTRED) {
-    asm("add.rn.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(0xe408e408u));                                   // - 1032
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(hi) : "r"(0x2c002c00u), "r"(0xd480d480u));             // / 16 - 72
-  }
+// Codes of the low nibble of each byte-pair of w (bits 0 .. 3 and 16 .. 19) and of the high one, as pairs of f16: c 2^-24 and c 2^-20.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00f000f0u; }
+// f32 needs normal operands (the tensor cores line products up by their exponents, and a subnormal number's says little): c - 8 by way of 1024 + c and
+// 1024 + 16 c, one operation more.
+__device__ __forceinline__ uint32_t low_exact(uint32_t w) {
+  uint32_t x = (w & 0x000f000fu) | 0x64006400u;
+  asm("add.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0xe408e408u));                            // - 1032
+  return x;
 }
+__device__ __forceinline__ uint32_t high_exact(uint32_t w) {
+  uint32_t x = (w & 0x00f000f0u) | 0x64006400u;
+  asm("add.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0xe480e480u));                            // - 1152: 16 (c - 8)
+  return x;
+}
+// -8 in both: what centres V's codes.  A sum of n weighted codes then stays as small as the values' own spread, which matters because the tensor
+// cores' sums round towards zero.
+constexpr uint32_t kMinus8Low = 0x80088008u, kMinus8High = 0x80808080u;
+constexpr float kCentre = 8.f;
 
 // x and y as TERMS f16 each
 template <int TERMS> __device__ __forceinline__ void split(float x, float y, uint32_t (&t)[TERMS]) {
@@ -102,27 +113,30 @@ struct Sequence {
   int r0, n;            // rows
   int base;             // position of the first row (negative: rows before it see nothing), at most the table's room
   int past, tiles;      // max(base, 0); row tiles
-  __device__ __forceinline__ Sequence(const AttentionParams &p, int s, int room) {
-    r0 = clamp(p.a.row_start[s], 0, p.a.rows);
-    n = clamp(p.a.row_start[s + 1], r0, p.a.rows) - r0;
-    base = clamp((long long)p.a.lens[s] - n, -n, room);
+  __device__ __forceinline__ Sequence(int first, int end, int position, int tokens) : r0(first), n(max(end - first, 0)), base(position) {
     past = max(base, 0);
-    tiles = (n + p.tokens - 1) / p.tokens;
+    tiles = n <= tokens ? min(n, 1) : (n + tokens - 1) / tokens;
   }
   __device__ __forceinline__ long long before(int rt, int tokens) const {
-    return rt < tiles ? (long long)rt * past + (long long)tokens * rt * (rt + 1) / 2
-                      : tiles == 0 ? 0 : (long long)(tiles - 1) * past + (long long)tokens * tiles * (tiles - 1) / 2 + past + n;
+    return rt == 0 ? 0
+           : rt < tiles ? (long long)rt * past + (long long)tokens * rt * (rt + 1) / 2
+                        : (long long)(tiles - 1) * past + (long long)tokens * tiles * (tiles - 1) / 2 + past + n;
   }
 };
+// x * a / b, rounded down
+__device__ __forceinline__ long long share(long long x, int a, int b) {
+  return x < (1 << 24) && a <= 255 ? (long long)((uint32_t)x * a / (uint32_t)b) : x * a / b;
+}
 
 template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
-  static constexpr int GROUPS = D / kKv4Group, STEPS = D / 16, TERMS = TYPE == B200_F32 ? 2 : 1;
-  // K's codes: a score of bf16 queries does not notice that 1024 + c costs it 2^-13 of the sum of |q s|; f16 would
-  static constexpr bool K_CENTRED = TYPE != B200_BF16;
+  static constexpr int GROUPS = D / kKv4Group, STEPS = D / 16, BYTES = kv4_tile_bytes(D);
+  static constexpr bool EXACT = TYPE == B200_F32;
+  static constexpr int TERMS = EXACT ? 2 : 1;
+  static constexpr int KT = EXACT ? 1 : 2;  // tiles at a time
+  static constexpr float LOW = EXACT ? 1.f : 5.9604645e-8f, HIGH = EXACT ? 16.f : 9.5367432e-7f;   // units of the codes' operands
   uint32_t q[TERMS][STEPS][2];
   float qs[GROUPS][2];                      // sums of q over a group, times the scores' scale, of rows 2 t and 2 t + 1 (t: lane % 4)
-  float minus[K_CENTRED ? 1 : GROUPS][2];   // what the offsets of codes add up to, negative
-  float unit[2];                            // the scores' scale over the row's power of two
+  float unit[2];                            // the scores' scale over the row's power of two and the codes' unit
   float o[STEPS][4];                        // dims 16 i + g (+ 8), rows 2 t (+ 1) (g: lane / 4)
   float bias[GROUPS][2], r[2], l[2];        // sums over this lane's keys: p (lo + 8 s), p
 
@@ -142,6 +156,20 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
     }
   }
 
+  __device__ __forceinline__ static void load_wide(const void *q, int64_t at, float (&x)[4]) {
+    if constexpr (TYPE == B200_F32) {
+      *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>((const float *)q + at);
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2 *>((const uint16_t *)q + at);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t w = e ? v.y : v.x;
+        const float2 f = TYPE == B200_F16 ? halves(w) : make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+      }
+    }
+  }
   // q of this lane's row (lane / 4), or none
   __device__ __forceinline__ void load_q(const AttentionParams &p, bool live, int64_t at) {
     const int lane = threadIdx.x & 31, t = lane & 3;
@@ -150,33 +178,32 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
     for (int k = 0; k < STEPS; ++k) {
       const int d = 32 * (k / 2) + 8 * t + 4 * (k & 1);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[k][e] = live ? load_as_float(p.a.q, TYPE, at + d + e) : 0.f;
+      for (int e = 0; e < 4; ++e)
+        x[k][e] = live && !p.wide_q ? load_as_float(p.a.q, TYPE, at + d + e) : 0.f;
+      if (live && p.wide_q)
+        load_wide(p.a.q, at + d, x[k]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
         most = fmaxf(most, fabsf(x[k][e]));
-      }
     }
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
     // 2^up: the row's largest comes to 2^14 .. 2^15 (a row below 2^-86 not as far)
     const int up = min(max(14 + 127 - (int)(__float_as_uint(most) >> 23), -113), 100);
-    const float factor = __uint_as_float((uint32_t)(127 + up) << 23), over = p.log2_scale * __uint_as_float((uint32_t)(127 - up) << 23);
+    const float factor = __uint_as_float((uint32_t)(127 + up) << 23), over = p.log2_scale * __uint_as_float((uint32_t)(127 - up) << 23) * (1.f / LOW);
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       unit[e] = __shfl_sync(0xffffffffu, over, 8 * t + 4 * e);
 #pragma unroll
     for (int gr = 0; gr < GROUPS; ++gr) {
-      float sum = 0.f, off = 0.f;
+      float sum = 0.f;
 #pragma unroll
       for (int k = 4 * gr; k < 4 * gr + 4; ++k) {
         float y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           sum += x[k][e];
-          y[e] = x[k][e] * factor;
-          if constexpr (!K_CENTRED) {
-            y[e] = __half2float(__float2half_rn(e / 2 == 0 ? y[e] : y[e] * 0.0625f));
-            off = fmaf(kOffset, y[e], off);
-          }
+          y[e] = x[k][e] * (e / 2 == 0 ? factor : factor * (LOW / HIGH));
         }
         uint32_t lo[TERMS], hi[TERMS];
         split<TERMS>(y[0], y[1], lo);
@@ -193,98 +220,87 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         qs[gr][e] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
-      if constexpr (!K_CENTRED) {
-        off += __shfl_xor_sync(0xffffffffu, off, 1);
-        off += __shfl_xor_sync(0xffffffffu, off, 2);
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          minus[gr][e] = -__shfl_sync(0xffffffffu, off, 8 * t + 4 * e);
-      }
     }
   }
 
-  // sixteen keys from j0 on; limit: keys that rows 2 t and 2 t + 1 see (only where MASKED)
-  template <bool MASKED> __device__ __forceinline__ void keys(const uint8_t *tile, int j0, const int (&limit)[2]) {
+  // KT tiles of sixteen keys, from j0[i] on; limit: keys that rows 2 t and 2 t + 1 see (only where MASKED)
+  template <bool MASKED> __device__ __forceinline__ void keys(const uint8_t *tiles, const int (&j0)[KT], const int (&limit)[2]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    uint32_t kw[2][D / 32], kp[2][GROUPS], vp[2][GROUPS];   // of keys g and g + 8
+    float s[KT][4], top[2] = {-INFINITY, -INFINITY};
+    bool out[KT][4];   // not seen
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j = g + 8 * h;
-      if constexpr (D == 128) {
-        *reinterpret_cast<uint4 *>(kw[h]) = *reinterpret_cast<const uint4 *>(tile + j * 64 + t * 16);
-        *reinterpret_cast<uint2 *>(kp[h]) = *reinterpret_cast<const uint2 *>(tile + kv4_k_pairs(D) + j * 8);
-        *reinterpret_cast<uint2 *>(vp[h]) = *reinterpret_cast<const uint2 *>(tile + kv4_v_pairs(D) + j * 8);
-      } else {
-        *reinterpret_cast<uint2 *>(kw[h]) = *reinterpret_cast<const uint2 *>(tile + j * 32 + t * 8);
-        kp[h][0] = *reinterpret_cast<const uint32_t *>(tile + kv4_k_pairs(D) + j * 4);
-        vp[h][0] = *reinterpret_cast<const uint32_t *>(tile + kv4_v_pairs(D) + j * 4);
-      }
-    }
-    float dot[4] = {}, low[4] = {};
-#pragma unroll
-    for (int gr = 0; gr < GROUPS; ++gr) {
-      float c[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        c[e] = K_CENTRED ? 0.f : minus[K_CENTRED ? 0 : gr][e & 1];
-#pragma unroll
-      for (int i = 2 * gr; i < 2 * gr + 2; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t a[4];
-          codes<K_CENTRED>(kw[0][i] >> (8 * u), a[0], a[2]);
-          codes<K_CENTRED>(kw[1][i] >> (8 * u), a[1], a[3]);
-#pragma unroll
-          for (int e = TERMS - 1; e >= 0; --e)
-            mma(c, a, q[e][2 * i + u][0], q[e][2 * i + u][1]);
-        }
+    for (int n = 0; n < KT; ++n) {
+      const uint8_t *tile = tiles + n * BYTES;
+      uint32_t kw[2][D / 32], kp[2][GROUPS], vp[2][GROUPS];   // of keys g and g + 8
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float2 pair = halves(kp[h][gr]);
-        const float lo = K_CENTRED ? fmaf(kCentre, pair.x, pair.y) : pair.y;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          dot[2 * h + e] = fmaf(c[2 * h + e], pair.x, dot[2 * h + e]);
-          low[2 * h + e] = fmaf(lo, qs[gr][e], low[2 * h + e]);
+        const int j = g + 8 * h;
+        if constexpr (D == 128) {
+          *reinterpret_cast<uint4 *>(kw[h]) = *reinterpret_cast<const uint4 *>(tile + j * 64 + t * 16);
+          *reinterpret_cast<uint2 *>(kp[h]) = *reinterpret_cast<const uint2 *>(tile + kv4_k_pairs(D) + j * 8);
+          *reinterpret_cast<uint2 *>(vp[h]) = *reinterpret_cast<const uint2 *>(tile + kv4_v_pairs(D) + j * 8);
+        } else {
+          *reinterpret_cast<uint2 *>(kw[h]) = *reinterpret_cast<const uint2 *>(tile + j * 32 + t * 8);
+          kp[h][0] = *reinterpret_cast<const uint32_t *>(tile + kv4_k_pairs(D) + j * 4);
+          vp[h][0] = *reinterpret_cast<const uint32_t *>(tile + kv4_v_pairs(D) + j * 4);
         }
       }
-    }
-    float s[4], at[4], vs[GROUPS][2], vb[GROUPS][2];
-    bool out[4];   // not seen
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float largest = kLeastScale;
+      float dot[4] = {}, low[4] = {};
 #pragma unroll
       for (int gr = 0; gr < GROUPS; ++gr) {
-        const float2 pair = halves(vp[h][gr]);
-        vs[gr][h] = pair.x;
-        vb[gr][h] = fmaf(kCentre, pair.x, pair.y);
-        largest = fmaxf(largest, pair.x);
-      }
-      const float height = lg2(largest);
+        float c[4] = {};
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int k = 2 * h + e;
-        s[k] = fmaf(dot[k], unit[e], low[k]);
-        if constexpr (MASKED) {
-          out[k] = j0 + g + 8 * h >= limit[e];
-          s[k] = out[k] ? -INFINITY : s[k];
+        for (int i = 2 * gr; i < 2 * gr + 2; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t x = kw[0][i] >> (8 * u), y = kw[1][i] >> (8 * u);
+            const uint32_t a[4] = {EXACT ? low_exact(x) : low_codes(x), EXACT ? low_exact(y) : low_codes(y), EXACT ? high_exact(x) : high_codes(x),
+                                   EXACT ? high_exact(y) : high_codes(y)};
+#pragma unroll
+            for (int e = TERMS - 1; e >= 0; --e)
+              mma(c, a, q[e][2 * i + u][0], q[e][2 * i + u][1]);
+          }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 pair = halves(kp[h][gr]);
+          const float lo = EXACT ? fmaf(kCentre, pair.x, pair.y) : pair.y;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            dot[2 * h + e] = fmaf(c[2 * h + e], pair.x, dot[2 * h + e]);
+            low[2 * h + e] = fmaf(lo, qs[gr][e], low[2 * h + e]);
+          }
         }
-        at[k] = s[k] + height;
-        if constexpr (MASKED)
-          at[k] = out[k] ? -INFINITY : at[k];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float largest = kLeastScale;
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr)
+          largest = fmaxf(largest, halves(vp[h][gr]).x);
+        const float height = lg2(largest);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int k = 2 * h + e;
+          s[n][k] = fmaf(dot[k], unit[e], low[k]);
+          float at = s[n][k] + height;
+          if constexpr (MASKED) {
+            out[n][k] = j0[n] + g + 8 * h >= limit[e];
+            s[n][k] = out[n][k] ? -INFINITY : s[n][k];
+            at = out[n][k] ? -INFINITY : at;
+          }
+          top[e] = fmaxf(top[e], at);
+        }
       }
     }
-    if (__any_sync(0xffffffffu, fmaxf(at[0], at[2]) > r[0] + (kTop + kLag) || fmaxf(at[1], at[3]) > r[1] + (kTop + kLag))) {
+    if (__any_sync(0xffffffffu, top[0] > r[0] + (kTop + kLag) || top[1] > r[1] + (kTop + kLag))) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float top = fmaxf(at[e], at[2 + e]);
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1)
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        top = fmaxf(top - kTop, r[e]);
-        const float keep = ex2(r[e] - top);
-        r[e] = top;
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
+        top[e] = top[e] > r[e] + (kTop + kLag) ? top[e] - kTop : r[e];   // (each row for itself)
+        const float keep = ex2(r[e] - top[e]);
+        r[e] = top[e];
         l[e] *= keep;
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr)
@@ -297,48 +313,66 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
       }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s[e] = ex2(s[e] - r[e & 1]);
-      l[e & 1] += s[e];
-    }
+    for (int n = 0; n < KT; ++n) {
+      const uint8_t *tile = tiles + n * BYTES;
+      uint32_t vp[2][GROUPS];
 #pragma unroll
-    for (int gr = 0; gr < GROUPS; ++gr) {
-      float w[4];
+      for (int h = 0; h < 2; ++h)
+        if constexpr (D == 128)
+          *reinterpret_cast<uint2 *>(vp[h]) = *reinterpret_cast<const uint2 *>(tile + kv4_v_pairs(D) + (g + 8 * h) * 8);
+        else
+          vp[h][0] = *reinterpret_cast<const uint32_t *>(tile + kv4_v_pairs(D) + (g + 8 * h) * 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        w[e] = s[e] * vs[gr][e >> 1];
-        float b = fmaf(s[e], vb[gr][e >> 1], bias[gr][e & 1]);
-        if constexpr (MASKED) {   // (what is not seen may be NaN)
-          w[e] = out[e] ? 0.f : w[e];
-          b = out[e] ? bias[gr][e & 1] : b;
+        s[n][e] = ex2(s[n][e] - r[e & 1]);
+        l[e & 1] += s[n][e];
+      }
+#pragma unroll
+      for (int gr = 0; gr < GROUPS; ++gr) {
+        float w[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 pair = halves(vp[h][gr]);
+          const float centre = fmaf(kCentre, pair.x, pair.y);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int k = 2 * h + e;
+            w[k] = s[n][k] * pair.x;
+            float b = fmaf(s[n][k], centre, bias[gr][e]);
+            if constexpr (MASKED) {   // (what is not seen may be NaN)
+              w[k] = out[n][k] ? 0.f : w[k];
+              b = out[n][k] ? bias[gr][e] : b;
+            }
+            bias[gr][e] = b;
+          }
         }
-        bias[gr][e & 1] = b;
-      }
-      uint32_t b0[TERMS], b1[TERMS];
-      split<TERMS>(w[0], w[1], b0);
-      split<TERMS>(w[2], w[3], b1);
+        uint32_t b0[TERMS], b1[TERMS];
+        split<TERMS>(w[0], w[1], b0);
+        split<TERMS>(w[2], w[3], b1);
 #pragma unroll
-      for (int e = 0; e < TERMS; ++e) {
-        b0[e] = transpose8(b0[e]);
-        b1[e] = transpose8(b1[e]);
-      }
-      uint32_t vw[4];
-      *reinterpret_cast<uint4 *>(vw) = *reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + gr * 512 + lane * 16);
+        for (int e = 0; e < TERMS; ++e) {
+          b0[e] = transpose8(b0[e]);
+          b1[e] = transpose8(b1[e]);
+        }
+        uint32_t vw[4];
+        *reinterpret_cast<uint4 *>(vw) = *reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + gr * 512 + lane * 16);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t a[4];
-        codes<true>(vw[i], a[0], a[1]);
-        codes<true>(vw[i] >> 8, a[2], a[3]);
-        if constexpr (TERMS == 1) {
-          mma(o[4 * gr + i], a, b0[0], b1[0]);
-        } else {   // f32: a sum of its own, added with rounding to nearest
-          float c[4] = {};
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (!EXACT) {
+            const uint32_t minus8[4] = {kMinus8Low, kMinus8High, kMinus8Low, kMinus8High};
+            const uint32_t a[4] = {low_codes(vw[i]), high_codes(vw[i]), low_codes(vw[i] >> 8), high_codes(vw[i] >> 8)};
+            mma(o[4 * gr + i], minus8, b0[0], b1[0]);
+            mma(o[4 * gr + i], a, b0[0], b1[0]);
+          } else {   // a sum of its own, added with rounding to nearest
+            const uint32_t a[4] = {low_exact(vw[i]), high_exact(vw[i]), low_exact(vw[i] >> 8), high_exact(vw[i] >> 8)};
+            float c[4] = {};
 #pragma unroll
-          for (int e = TERMS - 1; e >= 0; --e)
-            mma(c, a, b0[e], b1[e]);
+            for (int e = TERMS - 1; e >= 0; --e)
+              mma(c, a, b0[e], b1[e]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            o[4 * gr + i][e] += c[e];
+            for (int e = 0; e < 4; ++e)
+              o[4 * gr + i][e] += c[e];
+          }
         }
       }
     }
@@ -357,8 +391,8 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
       }
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
-        o[i][e] += bias[i * 16 / kKv4Group][e];
-        o[i][2 + e] += bias[i * 16 / kKv4Group][e];
+        o[i][e] = fmaf(o[i][e], 1.f / LOW, bias[i * 16 / kKv4Group][e]);
+        o[i][2 + e] = fmaf(o[i][2 + e], 1.f / HIGH, bias[i * 16 / kKv4Group][e]);
       }
     }
   }
@@ -379,10 +413,10 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
   }
 };
 
-__device__ __forceinline__ void put(const AttentionParams &p, int64_t at, float x) {
-  if (p.a.dtype == B200_F32)
+template <int TYPE> __device__ __forceinline__ void put(const AttentionParams &p, int64_t at, float x) {
+  if constexpr (TYPE == B200_F32)
     ((float *)p.a.out)[at] = x;
-  else if (p.a.dtype == B200_F16)
+  else if constexpr (TYPE == B200_F16)
     ((__half *)p.a.out)[at] = __float2half_rn(x);
   else
     ((__nv_bfloat16 *)p.a.out)[at] = __float2bfloat16_rn(x);
@@ -400,27 +434,25 @@ struct Place {
   int s, slot, rt, tile;
 };
 
-// A chain of parts of an item that ends in this CTA, or leaves it (by its last warp).
-struct Chain {
-  Place at;          // the item
-  int first, last;   // warps with its parts
-  bool opened;       // here: the first part is that warp's second one
-  bool ends;
+// What a warp leaves behind: parts of its first item (that began before it) and of its last (that goes on behind it).
+struct Left {
+  Place a, b;
+  int a_tiles, b_tiles;
+  const float *a_part;
+  bool has_a, a_ends, has_b;
 };
 
-template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 2) kv4_attention_kernel(const __grid_constant__ AttentionParams p) {
-  constexpr int BYTES = kv4_tile_bytes(D), PART = part_floats(D), RING = kStages * BYTES;
-  static_assert(RING >= PART * 4, "the second part of a warp lies in its ring");
+template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_attention_kernel(const __grid_constant__ AttentionParams p) {
+  using T = Tile<D, TYPE>;
+  constexpr int BYTES = T::BYTES, PART = part_floats(D), RING = kSlots * BYTES, KT = T::KT, STAGES = kSlots / KT;
+  static_assert(RING >= PART * 4, "a part of a warp lies in its ring");
   extern __shared__ __align__(128) uint8_t s_all[];
-  uint8_t *s_ring = s_all;
-  float *s_part = reinterpret_cast<float *>(s_all + kWarps * RING);                                // first parts
-  long long *s_cost = reinterpret_cast<long long *>(s_all + kWarps * (RING + PART * 4));          // [n_seqs + 1]
-  __shared__ long long s_sum[kWarps];
-  __shared__ Chain s_chain[kWarps + 1];
-  __shared__ bool s_has_a[kWarps], s_a_ends[kWarps], s_has_b[kWarps];
-  __shared__ Place s_a[kWarps], s_b[kWarps];
-  __shared__ int s_n_chains, s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.a.n_seqs, room = p.a.table_stride * p.page, slots = p.kv_heads * p.subs;
+  long long *s_cost = reinterpret_cast<long long *>(s_all + kWarps * RING);          // [n + 1]
+  int *s_r0 = reinterpret_cast<int *>(s_cost + n + 1), *s_base = s_r0 + n + 1;      // [n + 1], [n]
+  __shared__ long long s_sum[kWarps];
+  __shared__ Left s_left[kWarps];
+  __shared__ int s_ctas[2][3];     // of a shared item that this CTA adds up: whether it does, the CTAs with its first and last part
   kernel_go();
   kernel_wait();
 
@@ -429,7 +461,13 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 2) kv4_at
     const int per = (n + kThreads - 1) / kThreads, first = min(n, tid * per), last = min(n, first + per);
     long long sum = 0;
     for (int s = first; s < last; ++s) {
-      const Sequence q(p, s, room);
+      const int r0 = clamp(p.a.row_start[s], 0, p.a.rows), r1 = clamp(p.a.row_start[s + 1], 0, p.a.rows);
+      const int rows = max(r1 - r0, 0), base = clamp((long long)p.a.lens[s] - rows, -rows, room);
+      s_r0[s] = r0;
+      s_base[s] = base;
+      if (s == n - 1)
+        s_r0[n] = r1;
+      const Sequence q(r0, r1, base, p.tokens);
       s_cost[s] = sum;
       sum += slots * q.before(q.tiles, p.tokens);
     }
@@ -442,34 +480,41 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 2) kv4_at
     }
     if (lane == 31)
       s_sum[warp] = upto;
+    if (lane == 0)
+      s_left[warp].has_a = s_left[warp].has_b = false;
+    if (tid < 2)
+      s_ctas[tid][0] = 0;
     __syncthreads();
     long long before = upto - sum;
-    for (int w = 0; w < warp; ++w)
-      before += s_sum[w];
-    for (int s = first; s < last; ++s)
-      s_cost[s] += before;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      before += w < warp ? s_sum[w] : 0;
+    if (before != 0)
+      for (int s = first; s < last; ++s)
+        s_cost[s] += before;
     if (tid == kThreads - 1)
       s_cost[n] = before + sum;
     __syncthreads();
   }
+  auto sequence = [&](int s) { return Sequence(s_r0[s], s_r0[s + 1], s_base[s], p.tokens); };
   // rows of no sequence
   {
-    const int lo = clamp(p.a.row_start[0], 0, p.a.rows), hi = clamp(p.a.row_start[n], lo, p.a.rows), none = lo + p.a.rows - hi, cols = p.a.q_heads * D;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < (int64_t)none * cols; i += (int64_t)gridDim.x * kThreads) {
-      const int r = (int)(i / cols);
-      put(p, (int64_t)(r < lo ? r : hi + r - lo) * p.a.out_ld + i % cols, 0.f);
-    }
+    const int lo = s_r0[0], hi = max(lo, s_r0[n]), none = lo + p.a.rows - hi, cols = p.a.q_heads * D;
+    if (none > 0)
+      for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < (int64_t)none * cols; i += (int64_t)gridDim.x * kThreads) {
+        const int r = (int)(i / cols);
+        put<TYPE>(p, (int64_t)(r < lo ? r : hi + r - lo) * p.a.out_ld + i % cols, 0.f);
+      }
   }
+
+  // ---- this CTA's keys, this warp's keys ----------------------------------------------------------------------------------------
   const long long total = s_cost[n];
-  if (total == 0)
+  const int ctas = total >= (long long)gridDim.x * kLeastKeys ? gridDim.x : max(1, (int)total / kLeastKeys);
+  if (total == 0 || (int)blockIdx.x >= ctas)
     return;
-  // the warps that work: sixteen keys each at least (then each begins a tile)
-  const long long workers = max(1ll, min((long long)gridDim.x * kWarps, total / 16));
-  const long long me = (long long)blockIdx.x * kWarps + warp;
-  if ((long long)blockIdx.x * kWarps >= workers)
-    return;
-  auto place = [&](long long x) {   // the first tile that begins at x or behind it
-    Place at;
+  const long long chunk = share(total, 1, ctas);
+  const int window = chunk > kMany ? kSnap / 4 : (int)min((long long)kSnap, chunk / 2 - 1);
+  auto locate = [&](long long x, Place &at, long long &begin, long long &end) {   // the item with key x, from begin to end; at.tile: the first tile from x on
     int lo = 0, hi = n;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -479,64 +524,84 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 2) kv4_at
         hi = mid;
     }
     at.s = lo;
-    const Sequence q(p, lo, room);
-    x -= s_cost[lo];
+    const Sequence q = sequence(lo);
+    begin = s_cost[lo];
     const long long head = q.before(q.tiles, p.tokens);
-    at.slot = (int)(x / head);
-    x -= at.slot * head;
+    at.slot = (x - begin) >> 32 ? (int)((x - begin) / head) : (int)((uint32_t)(x - begin) / (uint32_t)min(head, 0xffffffffll));
+    begin += at.slot * head;
     int a = 0, b = q.tiles;
     while (b - a > 1) {
       const int mid = (a + b) >> 1;
-      if (q.before(mid, p.tokens) <= x)
+      if (q.before(mid, p.tokens) <= x - begin)
         a = mid;
       else
         b = mid;
     }
     at.rt = a;
-    at.tile = (int)((x - q.before(a, p.tokens) + 15) >> 4);
-    return at;
+    end = begin + q.before(a + 1, p.tokens);
+    begin += q.before(a, p.tokens);
+    at.tile = (int)((x - begin + 15) >> 4);
   };
+  auto border = [&](int c) {   // where CTA c begins: at its share of all keys, or at the item border next to that
+    if (c <= 0 || c >= ctas)
+      return c <= 0 ? 0 : total;
+    const long long x = share(total, c, ctas);
+    Place at;
+    long long begin, end;
+    locate(x, at, begin, end);
+    return x - begin <= end - x ? (x - begin <= window ? begin : x) : end - x <= window ? end : x;
+  };
+  auto nominal = [&](long long x) { return (int)(((x + 1) * ctas - 1) / total); };   // the CTA that x would lie in without that
   auto item_tiles = [&](const Sequence &q, int rt) { return (q.past + min((rt + 1) * p.tokens, q.n) + 15) >> 4; };
-  auto next_item = [&](Place &at, const Sequence &q) {   // (leaves the sequence: true)
+  auto next_item = [&](Place &at, const Sequence &q) {
     at.tile = 0;
     if (++at.rt < q.tiles)
-      return false;
+      return;
     at.rt = 0;
     if (++at.slot < slots)
-      return false;
+      return;
     at.slot = 0;
     do
       ++at.s;
     while (at.s < n && s_cost[at.s + 1] == s_cost[at.s]);
-    return true;
   };
-  if (lane == 0)
-    s_has_a[warp] = s_has_b[warp] = false;
+  long long x = border(blockIdx.x + min(lane, 1));   // (a lane each)
+  const long long cta_begin = __shfl_sync(0xffffffffu, x, 0), mine = __shfl_sync(0xffffffffu, x, 1) - cta_begin;
+  const int act = (int)max(1ll, min((long long)kWarps, mine >> 4));   // the warps that work: sixteen keys each at least (then each begins a tile)
+  Place at{n, 0, 0, 0}, stop;
+  x = cta_begin + share(mine, warp + min(lane, 1), act);
+  if (x < total) {
+    long long begin, end;
+    locate(x, at, begin, end);
+  }
+  stop.s = __shfl_sync(0xffffffffu, at.s, 1);
+  stop.slot = __shfl_sync(0xffffffffu, at.slot, 1);
+  stop.rt = __shfl_sync(0xffffffffu, at.rt, 1);
+  stop.tile = __shfl_sync(0xffffffffu, at.tile, 1);
+  at.s = __shfl_sync(0xffffffffu, at.s, 0);
+  at.slot = __shfl_sync(0xffffffffu, at.slot, 0);
+  at.rt = __shfl_sync(0xffffffffu, at.rt, 0);
+  at.tile = __shfl_sync(0xffffffffu, at.tile, 0);
 
-  if (me < workers) {
-    Place at = place(total * me / workers);
-    const long long end = total * (me + 1) / workers;
-    Place stop{n, 0, 0, 0};
-    if (end < total)
-      stop = place(end);
-    Tile<D, TYPE> tile;
-    uint8_t *ring = s_ring + warp * RING;
+  if (warp < act && mine > 0) {
+    uint8_t *ring = s_all + warp * RING;
+    T tile;
     while (at.s < n) {
-      const Sequence q(p, at.s, room);
-      const int T = item_tiles(q, at.rt);
-      if (at.tile >= T) {   // (a boundary behind an item's last tile)
+      const Sequence q = sequence(at.s);
+      const int all = item_tiles(q, at.rt);
+      if (at.tile >= all) {   // (a border behind an item's last tile)
         next_item(at, q);
         continue;
       }
       const bool here = stop.s == at.s && stop.slot == at.slot && stop.rt == at.rt;
-      const int t0 = at.tile, t1 = here ? min(stop.tile, T) : T;
+      const int t0 = at.tile, t1 = here ? min(stop.tile, all) : all;
       if (t0 >= t1)
         break;
       // ---- this warp's tiles of the item ----------------------------------------------------------------------------------------
       const int live = rows_of(p, q, at.rt, at.slot), first_token = at.rt * p.tokens, tokens = min(p.tokens, q.n - first_token);
       const int least = clamp((long long)q.base + first_token + 1, 0, room), most = clamp((long long)q.base + first_token + tokens, 0, room);
       const int kv = at.slot / p.subs, per_page = p.page / kKv4Tile;
-      auto source = [&](int t) {   // of lane's tile: its number in the pool, or -1
+      auto source = [&](int t) {   // of a tile: its number in the pool, or -1
         if (t >= t1 || t * kKv4Tile >= most)
           return -1;
         const int id = p.a.block_table[(int64_t)at.s * p.a.table_stride + t / per_page];
@@ -544,46 +609,51 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 2) kv4_at
       };
       int now = source(t0 + lane), next = source(t0 + 32 + lane);
       tile.clear();
-      uint32_t none = 0;   // bit of a stage: nothing to see in its tile
-      int ahead = 0, hand = 0;      // stages: of the next tile to ask for, of the tile in hand
-      auto request = [&](int i) {   // tile t0 + i
+      uint32_t none = 0;            // bit of a slot: nothing to see in its tile
+      int ahead = 0, hand = 0;      // slots: of the next tiles to ask for, of the tiles in hand
+      auto request = [&](int i) {   // tiles t0 + i ..
         if (i > 0 && (i & 31) == 0) {
           now = next;
           next = source(t0 + i + 32 + lane);
         }
-        const int from = __shfl_sync(0xffffffffu, now, i & 31);
-        none = from < 0 ? none | 1u << ahead : none & ~(1u << ahead);
-        if (from >= 0) {
-          const uint8_t *src = p.pool + (int64_t)from * BYTES + lane * 16;
-          uint8_t *to = ring + ahead * BYTES + lane * 16;
 #pragma unroll
-          for (int c = 0; c < BYTES / 512; ++c)
-            copy16(to + c * 512, src + c * 512);
-          if (BYTES % 512 != 0 && lane < BYTES % 512 / 16)
-            copy16(to + BYTES / 512 * 512, src + BYTES / 512 * 512);
+        for (int k = 0; k < KT; ++k) {
+          const int from = __shfl_sync(0xffffffffu, now, (i + k) & 31);
+          none = from < 0 ? none | 1u << (ahead + k) : none & ~(1u << (ahead + k));
+          if (from >= 0) {
+            const uint8_t *src = p.pool + (int64_t)from * BYTES + lane * 16;
+            uint8_t *to = ring + (ahead + k) * BYTES + lane * 16;
+#pragma unroll
+            for (int c = 0; c < BYTES / 512; ++c)
+              copy16(to + c * 512, src + c * 512);
+            if (BYTES % 512 != 0 && lane < BYTES % 512 / 16)
+              copy16(to + BYTES / 512 * 512, src + BYTES / 512 * 512);
+          }
         }
         copies_commit();
-        ahead = ahead == kStages - 1 ? 0 : ahead + 1;
+        ahead = (ahead + KT) % kSlots;
       };
       const int count = t1 - t0;
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < kStages - 1; ++i)
-        request(i);
+      for (int i = 0; i < STAGES - 1; ++i)
+        request(i * KT);
       tile.load_q(p, lane / 4 < live, lane / 4 < live ? row_at(p, q.r0, at.rt, at.slot, lane / 4, p.a.q_ld, D) : 0);
 #pragma unroll 1
-      for (int i = 0; i < count; ++i) {
-        copies_wait<kStages - 2>();
+      for (int i = 0; i < count; i += KT) {
+        copies_wait<STAGES - 2>();
         __syncwarp();
-        const bool skip = none >> hand & 1;
+        const uint32_t skip = none >> hand & ((1u << KT) - 1);
         const uint8_t *bytes = ring + hand * BYTES;
-        hand = hand == kStages - 1 ? 0 : hand + 1;
-        request(i + kStages - 1);
-        if (skip)
+        hand = (hand + KT) % kSlots;
+        request(i + kSlots - KT);
+        if (skip == (1u << KT) - 1)
           continue;
-        const int j0 = (t0 + i) * kKv4Tile;
-        int limit[2] = {0, 0};
-        if (j0 + kKv4Tile <= least) {
+        int j0[KT], limit[2] = {0, 0};
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+          j0[k] = skip >> k & 1 ? room : (t0 + i + k) * kKv4Tile;   // (no row sees a key from `room` on)
+        if (j0[KT - 1] + kKv4Tile <= least && skip == 0) {
           tile.template keys<false>(bytes, j0, limit);
         } else {
 #pragma unroll
@@ -598,7 +668,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 2) kv4_at
       __syncwarp();
       tile.finish();
       // ---- whole, or a part -------------------------------------------------------------------------------------------------------
-      if (t0 == 0 && t1 == T) {
+      if (t0 == 0 && t1 == all) {
         float over[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -610,23 +680,27 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 2) kv4_at
             const int64_t to = row_at(p, q.r0, at.rt, at.slot, row, p.a.out_ld, D) + lane / 4;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-              put(p, to + 16 * i, tile.l[e] == 0.f ? 0.f : tile.o[i][e] * over[e]);
-              put(p, to + 16 * i + 8, tile.l[e] == 0.f ? 0.f : tile.o[i][2 + e] * over[e]);
+              put<TYPE>(p, to + 16 * i, tile.l[e] == 0.f ? 0.f : tile.o[i][e] * over[e]);
+              put<TYPE>(p, to + 16 * i + 8, tile.l[e] == 0.f ? 0.f : tile.o[i][2 + e] * over[e]);
             }
           }
         }
-      } else if (t0 > 0) {   // (only a warp's first item)
-        tile.store(s_part + warp * PART);
+      } else {   // a part of the first item, or of the last; that of the first has to lie elsewhere where others follow
+        float *part = t0 > 0 && !here ? p.parts + ((int64_t)2 * kCtas + blockIdx.x * kWarps + warp) * PART : reinterpret_cast<float *>(ring);
+        tile.store(part);
         if (lane == 0) {
-          s_has_a[warp] = true;
-          s_a_ends[warp] = t1 == T;
-          s_a[warp] = at;
-        }
-      } else {               // (only its last)
-        tile.store(reinterpret_cast<float *>(ring));
-        if (lane == 0) {
-          s_has_b[warp] = true;
-          s_b[warp] = at;
+          Left &left = s_left[warp];
+          if (t0 > 0) {
+            left.has_a = true;
+            left.a_ends = t1 == all;
+            left.a_tiles = count;
+            left.a_part = part;
+            left.a = at;
+          } else {
+            left.has_b = true;
+            left.b_tiles = count;
+            left.b = at;
+          }
         }
       }
       if (here)
@@ -637,113 +711,127 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 2) kv4_at
   __syncthreads();
 
   // ---- parts of items: over the warps of this CTA, then over CTAs ----------------------------------------------------------------
-  if (tid == 0) {
-    int k = 0;
-    const int act = (int)min((long long)kWarps, workers - (long long)blockIdx.x * kWarps);
-    for (int w = -1; w < act; ++w) {
-      if (w < 0 ? !s_has_a[0] : !s_has_b[w])
-        continue;
-      Chain c;
-      c.opened = w >= 0;
-      c.at = w < 0 ? s_a[0] : s_b[w];
-      c.first = max(w, 0);
-      c.last = c.first;
-      c.ends = w < 0 && s_a_ends[0];
-      while (!c.ends && c.last + 1 < act) {
-        ++c.last;
-        c.ends = s_a_ends[c.last];
-      }
-      s_chain[k++] = c;
+  const uint32_t has_a = __ballot_sync(0xffffffffu, lane < act && s_left[lane % kWarps].has_a), has_b = __ballot_sync(0xffffffffu, lane < act && s_left[lane % kWarps].has_b);
+  const uint32_t ends = __ballot_sync(0xffffffffu, lane < act && s_left[lane % kWarps].has_a && s_left[lane % kWarps].a_ends);
+  // A chain: the parts of an item, of neighbouring warps.  One may have begun in another CTA (chain 0, then), the others are opened by the warps of
+  // has_b; the last of them may go on in the next CTA.
+  const int incoming = has_a & 1, chains = incoming + __popc(has_b);
+  if (chains == 0)
+    return;
+  struct Chain {
+    int first, last;
+    bool opened, whole;
+  };
+  auto chain = [&](int k) {
+    Chain c;
+    c.opened = k >= incoming;
+    uint32_t b = has_b;
+    for (int i = incoming; i < k; ++i)
+      b &= b - 1;
+    c.first = c.opened ? __ffs(b) - 1 : 0;
+    const uint32_t end = ends >> (c.first + c.opened) << (c.first + c.opened);
+    c.last = end != 0 ? __ffs(end) - 1 : act - 1;
+    c.whole = c.opened && end != 0;
+    return c;
+  };
+  auto add = [](float4 &o, float &l, float4 v, float pl, float f) {
+    l = fmaf(pl, f, l);
+    o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
+  };
+  auto write_out = [&](const Place &at, int row, int d, float4 o, float l) {
+    const Sequence q = sequence(at.s);
+    if (row >= rows_of(p, q, at.rt, at.slot))
+      return;
+    const int64_t to = row_at(p, q.r0, at.rt, at.slot, row, p.a.out_ld, D) + d;
+    const float over = l == 0.f ? 0.f : 1.f / l;
+    put<TYPE>(p, to, l == 0.f ? 0.f : o.x * over);
+    put<TYPE>(p, to + 1, l == 0.f ? 0.f : o.y * over);
+    put<TYPE>(p, to + 2, l == 0.f ? 0.f : o.z * over);
+    put<TYPE>(p, to + 3, l == 0.f ? 0.f : o.w * over);
+  };
+  constexpr int FOURS = kRows * D / 4;
+  const int row = tid % FOURS / (D / 4), d = tid % (D / 4) * 4;
+  for (int k = tid / FOURS; k < chains; k += kThreads / FOURS) {
+    const Chain c = chain(k);
+    auto part = [&](int w) { return c.opened && w == c.first ? reinterpret_cast<const float *>(s_all + w * RING) : s_left[w].a_part; };
+    float top = kSeed, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = c.first; w <= c.last; ++w)
+      top = fmaxf(top, part(w)[kRows * (D + 4) + row]);
+    for (int w = c.first; w <= c.last; ++w) {
+      const float *x = part(w);
+      add(o, l, *reinterpret_cast<const float4 *>(x + row * (D + 4) + d), x[kRows * (D + 4) + kRows + row], ex2(x[kRows * (D + 4) + row] - top));
     }
-    s_n_chains = k;
+    if (c.whole) {
+      write_out(s_left[c.first].b, row, d, o, l);
+    } else {
+      float *to = p.parts + ((int64_t)blockIdx.x * 2 + c.opened) * PART;
+      *reinterpret_cast<float4 *>(to + row * (D + 4) + d) = o;
+      if (d == 0) {
+        to[kRows * (D + 4) + row] = top;
+        to[kRows * (D + 4) + kRows + row] = l;
+      }
+    }
+  }
+  const bool outgoing = !chain(chains - 1).whole && chain(chains - 1).opened;
+  if (!incoming && !outgoing)
+    return;
+  __threadfence();
+  __syncthreads();
+  // An item's tiles are counted as its parts arrive, in the counter of the CTA that would begin it were there no borders moved (no two items that are
+  // shared have the same); who completes them adds its parts up, in their order.
+  if (warp < 2 && (warp == 0 ? incoming : outgoing)) {
+    const Chain c = chain(warp == 0 ? 0 : chains - 1);
+    const Place item = c.opened ? s_left[c.first].b : s_left[0].a;
+    const Sequence q = sequence(item.s);
+    const int all = item_tiles(q, item.rt);
+    const long long first = s_cost[item.s] + item.slot * q.before(q.tiles, p.tokens) + q.before(item.rt, p.tokens), last = first + 16ll * (all - 1);
+    const int from = nominal(first), to = nominal(last);
+    int tiles = 0, before = 0;
+    for (int w = c.first; w <= c.last; ++w)
+      tiles += c.opened && w == c.first ? s_left[w].b_tiles : s_left[w].a_tiles;
+    if (lane == 0)
+      before = atomicAdd(p.counters + from, tiles);
+    if (__shfl_sync(0xffffffffu, before, 0) + tiles == all) {
+      const long long x = border(lane == 0 ? from + 1 : lane == 1 ? to : to + 1);   // (a lane each)
+      const bool later = __shfl_sync(0xffffffffu, (int)(x <= first), 0), sooner = __shfl_sync(0xffffffffu, (int)(x > last), 1),
+                 beyond = __shfl_sync(0xffffffffu, (int)(x <= last), 2);
+      if (lane == 0) {
+        p.counters[from] = 0;
+        s_ctas[warp][0] = 1;
+        s_ctas[warp][1] = from + later;
+        s_ctas[warp][2] = to - sooner + beyond;
+      }
+    }
   }
   __syncthreads();
-  auto part_of = [&](const Chain &c, int w) { return c.opened && w == c.first ? reinterpret_cast<const float *>(s_ring + w * RING) : s_part + w * PART; };
-  for (int k = 0; k < s_n_chains; ++k) {
-    const Chain c = s_chain[k];
-    const Sequence q(p, c.at.s, room);
-    const int live = rows_of(p, q, c.at.rt, c.at.slot);
-    const bool whole = c.opened && c.ends;
-    float *mine = p.parts + ((int64_t)blockIdx.x * 2 + c.opened) * PART;
-    for (int i = tid; i < kRows * D / 4; i += kThreads) {
-      const int row = i / (D / 4), d = i % (D / 4) * 4;
-      float top = kSeed, l = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int w = c.first; w <= c.last; ++w)
-        top = fmaxf(top, part_of(c, w)[kRows * (D + 4) + row]);
-      for (int w = c.first; w <= c.last; ++w) {
-        const float *part = part_of(c, w), pl = part[kRows * (D + 4) + kRows + row], f = ex2(part[kRows * (D + 4) + row] - top);
-        const float4 v = *reinterpret_cast<const float4 *>(part + row * (D + 4) + d);
-        l = fmaf(pl, f, l);
-        o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
-      }
-      if (whole) {
-        if (row < live) {
-          const int64_t to = row_at(p, q.r0, c.at.rt, c.at.slot, row, p.a.out_ld, D) + d;
-          const float over = l == 0.f ? 0.f : 1.f / l;
-          put(p, to, l == 0.f ? 0.f : o.x * over);
-          put(p, to + 1, l == 0.f ? 0.f : o.y * over);
-          put(p, to + 2, l == 0.f ? 0.f : o.z * over);
-          put(p, to + 3, l == 0.f ? 0.f : o.w * over);
-        }
-      } else {
-        *reinterpret_cast<float4 *>(mine + row * (D + 4) + d) = o;
-        if (d == 0) {
-          mine[kRows * (D + 4) + row] = top;
-          mine[kRows * (D + 4) + kRows + row] = l;
-        }
-      }
-    }
-    if (whole)
-      continue;
-    // the CTAs with parts of this item: those of its first and last tile's workers
-    const long long begin = s_cost[c.at.s] + c.at.slot * q.before(q.tiles, p.tokens) + q.before(c.at.rt, p.tokens);
-    const long long final = begin + 16ll * (item_tiles(q, c.at.rt) - 1);
-    const int from = (int)((((begin + 1) * workers - 1) / total) / kWarps), to = (int)((((final + 1) * workers - 1) / total) / kWarps);
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-      const int before = atomicAdd(p.counters + from, 1);
-      s_last = before == to - from;
-      if (s_last)
-        p.counters[from] = 0;
-    }
-    __syncthreads();
-    if (!s_last)
+  for (int k = tid / FOURS; k < 2; k += kThreads / FOURS) {
+    if (s_ctas[k][0] == 0)
       continue;
     __threadfence();
-    for (int i = tid; i < kRows * D / 4; i += kThreads) {
-      const int row = i / (D / 4), d = i % (D / 4) * 4;
-      if (row >= live)
-        continue;
-      auto part = [&](int b) { return p.parts + ((int64_t)b * 2 + (b == from)) * PART; };
-      float top = kSeed, l = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int b = from; b <= to; ++b)
-        top = fmaxf(top, __ldcg(part(b) + kRows * (D + 4) + row));
-      for (int b = from; b <= to; ++b) {
-        const float pl = __ldcg(part(b) + kRows * (D + 4) + kRows + row), f = ex2(__ldcg(part(b) + kRows * (D + 4) + row) - top);
-        const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(b) + row * (D + 4) + d));
-        l = fmaf(pl, f, l);
-        o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
-      }
-      const int64_t at = row_at(p, q.r0, c.at.rt, c.at.slot, row, p.a.out_ld, D) + d;
-      const float over = l == 0.f ? 0.f : 1.f / l;
-      put(p, at, l == 0.f ? 0.f : o.x * over);
-      put(p, at + 1, l == 0.f ? 0.f : o.y * over);
-      put(p, at + 2, l == 0.f ? 0.f : o.z * over);
-      put(p, at + 3, l == 0.f ? 0.f : o.w * over);
-    }
+    const Chain c = chain(k == 0 ? 0 : chains - 1);
+    const int from = s_ctas[k][1], to = s_ctas[k][2];
+    auto part = [&](int b) { return p.parts + ((int64_t)b * 2 + (b == from)) * PART; };
+    float top = kSeed, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int b = from; b <= to; ++b)
+      top = fmaxf(top, __ldcg(part(b) + kRows * (D + 4) + row));
+#pragma unroll 4
+    for (int b = from; b <= to; ++b)
+      add(o, l, __ldcg(reinterpret_cast<const float4 *>(part(b) + row * (D + 4) + d)), __ldcg(part(b) + kRows * (D + 4) + kRows + row),
+          ex2(__ldcg(part(b) + kRows * (D + 4) + row) - top));
+    write_out(c.opened ? s_left[c.first].b : s_left[0].a, row, d, o, l);
   }
 }
 
 RaisedOn g_raised[6];
 
 template <int D, int TYPE> int attention_launch(RaisedOn &raised, const AttentionParams &p, cudaStream_t st) {
-  const int fixed = kWarps * (kStages * kv4_tile_bytes(D) + part_floats(D) * 4);
-  if (int rc = raise_shared_limit(raised, (const void *)kv4_attention_kernel<D, TYPE>, fixed + 8 * (B200_KV4_ATTENTION_MAX_SEQS + 1)))
+  const int fixed = kWarps * kSlots * kv4_tile_bytes(D);
+  if (int rc = raise_shared_limit(raised, (const void *)kv4_attention_kernel<D, TYPE>, fixed + 16 * (B200_KV4_ATTENTION_MAX_SEQS + 1)))
     return rc;
-  return launch_after(kv4_attention_kernel<D, TYPE>, dim3(kCtas), kThreads, fixed + 8 * (p.a.n_seqs + 1), st, p);
+  return launch_after(kv4_attention_kernel<D, TYPE>, dim3(kCtas), kThreads, fixed + 16 * (p.a.n_seqs + 1), st, p);
 }
 
 } // namespace
@@ -757,7 +845,7 @@ extern "C" {
 int64_t b200_kv4_attention_workspace_bytes(int q_heads, int kv_heads, int head_dim) {
   if (kv_heads < 1 || kv_heads > 1024 || q_heads < 1 || q_heads % kv_heads != 0 || (head_dim != 64 && head_dim != 128))
     return B200_EINVAL;
-  return 2048 + (int64_t)kCtas * 2 * part_floats(head_dim) * 4;
+  return 2048 + (int64_t)kCtas * (2 + kWarps) * part_floats(head_dim) * 4;
 }
 
 int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a, void *workspace, int64_t workspace_bytes, void *stream) {
@@ -767,7 +855,7 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
     return fail(B200_EINVAL, "kv4_attention: null pointer");
   if (a->dtype != B200_F32 && a->dtype != B200_F16 && a->dtype != B200_BF16)
     return fail(B200_EINVAL, "kv4_attention: element type %d", a->dtype);
-  if (a->rows < 0 || a->n_seqs < 1 || a->table_stride < 1 || a->q_heads < 1 || a->q_heads % c->kv_heads != 0 || (int64_t)a->table_stride * c->page > INT32_MAX)
+  if (a->rows < 0 || a->n_seqs < 1 || a->table_stride < 1 || a->q_heads < 1 || a->q_heads % c->kv_heads != 0 || (int64_t)a->table_stride * c->page > INT32_MAX - 64)
     return fail(B200_EINVAL, "kv4_attention: %d rows of %d sequences, tables of %d pages, %d heads on %d", a->rows, a->n_seqs, a->table_stride, a->q_heads,
                 c->kv_heads);
   if (a->n_seqs > B200_KV4_ATTENTION_MAX_SEQS)
@@ -793,6 +881,8 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
   p.heads = std::min(p.G, kRows);
   p.tokens = p.subs == 1 ? kRows / p.G : 1;
   p.log2_scale = a->scale * 1.4426950408889634f;
+  const int size = a->dtype == B200_F32 ? 4 : 2;
+  p.wide_q = (((uintptr_t)a->q | (uintptr_t)(a->q_ld * size)) & (4 * size - 1)) == 0;
   p.counters = (int *)workspace;
   p.parts = (float *)((char *)workspace + 2048);
   cudaStream_t st = (cudaStream_t)stream;

@@ -213,11 +213,10 @@ def test_row_maps_may_be_left_out():
 def bound(kind, S, V, n):
     """Of an output's error.  S: the largest sum of |q||k| of a score; V: the largest |v|; n: keys.
     A score: at most 2^-20 S (f32 sums of sixteen terms at a time that round towards zero, 2^-23 each, eight in a row for a group, one of two terms of q;
-    parameters' products); bf16: 2^-13 S more, since its codes come with an offset of 1024, some 2^7 times a value's own size, and lose as much; so weights
-    twice that, in the sum and the total.  A sum of n weighted values: 2^-23 for every
+    parameters' products), so weights twice that, in the sum and the total.  A sum of n weighted values: 2^-23 for every
     sixteen keys, and some for the sums of warps and CTAs.  Weights as operands: half a step of f16 (f32:
     of two f16), exponentials 2^-21.  The output's own rounding.  All relative to V, which bounds each sum of weighted values over the sum of weights."""
-    weight = {"f32": 2.0 ** -21, "f16": 2.0 ** -11, "bf16": 2.0 ** -11 + 2.0 ** -11 * S}[kind]
+    weight = {"f32": 2.0 ** -21, "f16": 2.0 ** -11, "bf16": 2.0 ** -11}[kind]
     sums = (n / 16 + 16) * 2.0 ** -23
     return V * (2.0 ** -18 * S + 2 * sums + 2.0 ** -20 + weight) + V * HALF[kind] + 2.0 ** -25
 
