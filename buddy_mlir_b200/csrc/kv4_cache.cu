@@ -1,8 +1,13 @@
 // The 4-bit KV cache's writer and reader (b200_kv4_write, b200_kv4_read).
 //
-// A half-warp has a group of 64 dims of one row and head, four dims a lane: its extremes by four shuffles, lo and the scale rounded to
-// f16, the codes by one division each.
+// A lane has eight dims of a row's K or V, eight lanes a group of 64: a warp takes both groups of K and V of a head of 128 dims at once, or two heads
+// of 64.  A group's extremes take three shuffles; eight dims of K are one word of codes, those of V, with a neighbour's, a byte for each of
+// eight pairs of dims sixteen apart.  A code's quotient is a product and one correction (quotient.cuh), the same bits as a division.
+// What bounds them is instructions (some 190 and 130 of a warp per 256 values), then bytes.
 #include "kv4.cuh"
+#include "quotient.cuh"
+
+#include <algorithm>
 
 namespace b200 {
 
@@ -13,151 +18,182 @@ constexpr int kThreads = 256;
 struct CacheParams {
   uint8_t *pool;
   int64_t positions;     // of the pool
-  int kv_heads, D, page;
+  int kv_heads, page;
   void *k, *v;
   int64_t k_ld, v_ld;
   const int64_t *slots;
-  int64_t groups;        // rows * kv heads * D / 64
+  int rows, heads;       // heads: pairs of them for D = 64
 };
 
-template <typename T> struct Four {   // four elements of a row, with one load where they are aligned
-  T e[4];
-};
-template <typename T, bool WIDE> __device__ __forceinline__ void load4(const T *p, float (&x)[4]) {
-  Four<T> v;
-  if constexpr (WIDE && sizeof(T) == 4)
-    *reinterpret_cast<uint4 *>(&v) = *reinterpret_cast<const uint4 *>(p);
-  else if constexpr (WIDE)
-    *reinterpret_cast<uint2 *>(&v) = *reinterpret_cast<const uint2 *>(p);
-  else
-    for (int i = 0; i < 4; ++i)
-      v.e[i] = p[i];
+// eight elements of a row, with 16-byte loads where they are aligned
+template <typename T, bool WIDE> __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
+  if constexpr (WIDE && sizeof(T) == 4) {
+    *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>(p);
+    *reinterpret_cast<float4 *>(x + 4) = *reinterpret_cast<const float4 *>(p + 4);
+  } else if constexpr (WIDE) {
+    __align__(16) T e[8];
+    *reinterpret_cast<uint4 *>(e) = *reinterpret_cast<const uint4 *>(p);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    x[i] = (float)v.e[i];
+    for (int i = 0; i < 8; ++i)
+      x[i] = (float)e[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x[i] = (float)p[i];
+  }
 }
-template <typename T, bool WIDE> __device__ __forceinline__ void store4(T *p, const float (&x)[4]) {
-  Four<T> v;
+template <typename T, bool WIDE> __device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
+  if constexpr (WIDE && sizeof(T) == 4) {
+    *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4 *>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+  } else if constexpr (WIDE) {
+    __align__(16) T e[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    v.e[i] = (T)x[i];
-  if constexpr (WIDE && sizeof(T) == 4)
-    *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<uint4 *>(&v);
-  else if constexpr (WIDE)
-    *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<uint2 *>(&v);
-  else
-    for (int i = 0; i < 4; ++i)
-      p[i] = v.e[i];
+    for (int i = 0; i < 8; ++i)
+      e[i] = (T)x[i];
+    *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<uint4 *>(e);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      p[i] = (T)x[i];
+  }
 }
 
-// Codes of a lane's four dims, and the group's pair (scale in the low half); all 16 lanes of the group call it.
-__device__ __forceinline__ uint32_t quantise(const float (&in)[4], uint32_t lanes, int (&code)[4]) {
-  float x[4], mn = INFINITY, mx = -INFINITY;
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    nan = nan || in[i] != in[i];
-    x[i] = fminf(fmaxf(in[i], -kKv4Most), kKv4Most);
-    mn = fminf(mn, x[i]);
-    mx = fmaxf(mx, x[i]);
-  }
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    mn = fminf(mn, __shfl_xor_sync(lanes, mn, o));
-    mx = fmaxf(mx, __shfl_xor_sync(lanes, mx, o));
-  }
-  nan = __any_sync(lanes, nan);
-  const __half lo = __float2half_rn(mn), scale = __float2half_rn(__fdiv_rn(__fsub_rn(mx, __half2float(lo)), 15.f));
-  const float l = __half2float(lo), s = __half2float(scale);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    code[i] = nan || !(s > 0.f) ? 0 : (int)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], l), s)), 0.f), 15.f);
-  return nan ? 0x7e000000u : (uint32_t)__half_as_ushort(scale) | (uint32_t)__half_as_ushort(lo) << 16;
-}
-
-struct Place {   // of a half-warp's group
-  int64_t row;
-  int head, group, j;      // j: the position in its tile
+// Where a lane's eight dims lie: lanes 0 .. 15 have K's, the others V's; of a head of 128, or of two of 64.
+template <int D> struct Place {
+  int head, group, m;      // m: which eight dims of the group
+  int j;                   // the position in its tile
   uint8_t *tile;           // null: no position of the pool
+  __device__ __forceinline__ Place(const CacheParams &p, int row, int head_of) {
+    const int lane = threadIdx.x & 31;
+    m = lane & 7;
+    group = D == 128 ? lane >> 3 & 1 : 0;
+    head = D == 128 ? head_of : 2 * head_of + (lane >> 3 & 1);
+    const int64_t slot = p.slots[row];
+    if (slot < 0 || slot >= p.positions || head >= p.kv_heads) {
+      tile = nullptr;
+      j = 0;
+      return;
+    }
+    const int64_t id = slot >> 31 ? slot / p.page : (int64_t)((uint32_t)slot / (uint32_t)p.page);
+    const int off = (int)(slot - id * p.page);
+    j = off % kKv4Tile;
+    tile = p.pool + ((id * p.kv_heads + head) * (p.page / kKv4Tile) + off / kKv4Tile) * kv4_tile_bytes(D);
+  }
+  __device__ __forceinline__ int column() const { return head * D + group * kKv4Group + 8 * m; }
+  __device__ __forceinline__ uint32_t *k_word() const { return reinterpret_cast<uint32_t *>(tile + j * (D / 2) + m % 4 * (D / 8) + (2 * group + m / 4) * 4); }
+  // of V: of the first of the four pairs of dims that this lane stores or loads (64 bytes from one to the next)
+  __device__ __forceinline__ uint8_t *v_bytes() const {
+    return tile + kv4_v_codes(D) + group * 512 + (m & 1) * 256 + j % 8 / 2 * 16 + m / 2 * 4 + j % 2 * 2 + j / 8;
+  }
+  __device__ __forceinline__ uint32_t *pair(bool is_k) const {
+    return reinterpret_cast<uint32_t *>(tile + (is_k ? kv4_k_pairs(D) : kv4_v_pairs(D)) + (j * (D / kKv4Group) + group) * 4);
+  }
 };
-__device__ __forceinline__ Place place_of(const CacheParams &p, int64_t at) {
-  const int per_head = p.D / kKv4Group, per_row = p.kv_heads * per_head;
-  Place g;
-  g.row = at / per_row;
-  const int in_row = (int)(at % per_row);
-  g.head = in_row / per_head;
-  g.group = in_row % per_head;
-  const int64_t slot = p.slots[g.row];
-  const int64_t page = slot / p.page;
-  const int off = (int)(slot % p.page);
-  g.j = off % kKv4Tile;
-  g.tile = slot < 0 || slot >= p.positions
-               ? nullptr
-               : p.pool + ((page * p.kv_heads + g.head) * (p.page / kKv4Tile) + off / kKv4Tile) * kv4_tile_bytes(p.D);
-  return g;
-}
 
-template <typename T, bool WIDE> __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const __grid_constant__ CacheParams p) {
+template <int D, typename T, bool WIDE> __global__ void __launch_bounds__(kThreads) kv4_write_kernel(const __grid_constant__ CacheParams p) {
   kernel_go();
   kernel_wait();
-  const int r = threadIdx.x & 15;
-  const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
-  for (int64_t at = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4; at < p.groups; at += (int64_t)gridDim.x * (kThreads / 16)) {
-    const Place g = place_of(p, at);
-    if (g.tile == nullptr)
-      continue;   // (all 16 lanes)
-    const int64_t col = (int64_t)g.head * p.D + g.group * kKv4Group + 4 * r;
-    float x[4];
-    int c[4];
-    load4<T, WIDE>((const T *)p.k + g.row * p.k_ld + col, x);
-    uint32_t pair = quantise(x, lanes, c);
-    // bytes (c0, c2) and (c1, c3) of lanes r (even) and r + 1: one word
-    const uint32_t mine = c[0] | c[2] << 4 | (c[1] | c[3] << 4) << 16, other = __shfl_down_sync(lanes, mine, 1, 16);
-    if ((r & 1) == 0)
-      *reinterpret_cast<uint32_t *>(g.tile + g.j * (p.D / 2) + (r / 2) % 4 * (p.D / 8) + (2 * g.group + r / 8) * 4) = mine | other << 8;
-    if (r == 0)
-      *reinterpret_cast<uint32_t *>(g.tile + kv4_k_pairs(p.D) + (g.j * (p.D / kKv4Group) + g.group) * 4) = pair;
-    load4<T, WIDE>((const T *)p.v + g.row * p.v_ld + col, x);
-    pair = quantise(x, lanes, c);
-    // dims 16 i + g (low nibble) and 16 i + 8 + g are four lanes' halves apart: lanes r and r ^ 2 store two bytes each
-    const uint32_t all = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, apart = __shfl_xor_sync(lanes, all, 2);
-    const bool high = r & 2;
-    const uint32_t both = high ? apart | all << 4 : all | apart << 4;
-    uint8_t *v = g.tile + kv4_v_codes(p.D) + g.group * 512 + (r & 1) * 256 + g.j % 8 / 2 * 16 + r / 4 * 4 + g.j % 2 * 2 + g.j / 8;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int e = high ? 2 + i : i;
-      v[e * 64] = (uint8_t)(both >> (8 * e));
+  const int lane = threadIdx.x & 31;
+  const bool is_k = lane < 16;
+  int row = blockIdx.x;
+  for (int h = threadIdx.x >> 5; row < p.rows; h += kThreads / 32) {
+    while (h >= p.heads) {
+      h -= p.heads;
+      row += gridDim.x;
     }
-    if (r == 0)
-      *reinterpret_cast<uint32_t *>(g.tile + kv4_v_pairs(p.D) + (g.j * (p.D / kKv4Group) + g.group) * 4) = pair;
+    if (row >= p.rows)
+      break;
+    const Place<D> g(p, row, h);
+    float x[8], mn = kKv4Most, mx = -kKv4Most;
+    bool nan = false;
+    if (g.head < p.kv_heads) {
+      load8<T, WIDE>((const T *)(is_k ? p.k : p.v) + row * (is_k ? p.k_ld : p.v_ld) + g.column(), x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      nan = nan || x[i] != x[i];
+      x[i] = fminf(fmaxf(x[i], -kKv4Most), kKv4Most);
+      mn = fminf(mn, x[i]);
+      mx = fmaxf(mx, x[i]);
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    nan = __ballot_sync(0xffffffffu, nan) >> (lane & 24) & 0xff;
+    const __half lo = __float2half_rn(mn), scale = __float2half_rn(__fdiv_rn(__fsub_rn(mx, __half2float(lo)), 15.f));
+    const float l = __half2float(lo), s = __half2float(scale), b = s * 16777216.f, r = __frcp_rn(b);   // (b >= 1: the smallest scale is 2^-24)
+    const bool some = s > 0.f && !nan;
+    // dim 2 a + h of the eight: nibble a + 4 h
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float a = __fsub_rn(x[i], l) * 16777216.f, q = a * r, code = fmaf(fmaf(-b, q, a), r, q);
+      // rounded as rint does: added to 1.5 * 2^23
+      word |= (__float_as_uint(__fadd_rn(fminf(fmaxf(code, 0.f), 15.f), 12582912.f)) & 15u) << (is_k ? 4 * (i / 2 + 4 * (i & 1)) : 4 * i);
+    }
+    word = some ? word : 0;
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 1);
+    if (g.tile == nullptr)
+      continue;
+    if (is_k) {
+      *g.k_word() = word;
+    } else {   // dims 16 i + g (low nibbles: the even lane's) and 16 i + 8 + g: four pairs each
+      const uint32_t low = g.m & 1 ? other >> 16 : word, high = g.m & 1 ? word >> 16 : other;
+      uint8_t *v = g.v_bytes();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i * 64] = (uint8_t)((low >> (4 * i) & 15) | (high >> (4 * i) & 15) << 4);
+    }
+    if (g.m == 0)
+      *g.pair(is_k) = nan ? 0x7e000000u : (uint32_t)__half_as_ushort(scale) | (uint32_t)__half_as_ushort(lo) << 16;
   }
 }
 
-template <typename T, bool WIDE> __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const __grid_constant__ CacheParams p) {
+template <int D, typename T, bool WIDE> __global__ void __launch_bounds__(kThreads) kv4_read_kernel(const __grid_constant__ CacheParams p) {
   kernel_go();
   kernel_wait();
-  const int r = threadIdx.x & 15;
-  for (int64_t at = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 4; at < p.groups; at += (int64_t)gridDim.x * (kThreads / 16)) {
-    const Place g = place_of(p, at);
-    const int64_t col = (int64_t)g.head * p.D + g.group * kKv4Group + 4 * r;
-    float k[4] = {}, v[4] = {};
-    if (g.tile != nullptr) {
-      const int pair_at = (g.j * (p.D / kKv4Group) + g.group) * 4;
-      __half2 pair = *reinterpret_cast<const __half2 *>(g.tile + kv4_k_pairs(p.D) + pair_at);
-      const uint32_t word =
-          *reinterpret_cast<const uint32_t *>(g.tile + g.j * (p.D / 2) + (r / 2) % 4 * (p.D / 8) + (2 * g.group + r / 8) * 4) >> (8 * (r & 1));
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        k[i] = fmaf(__low2float(pair), (float)(word >> (16 * (i & 1) + 4 * (i >> 1)) & 15), __high2float(pair));
-      pair = *reinterpret_cast<const __half2 *>(g.tile + kv4_v_pairs(p.D) + pair_at);
-      const uint8_t *c = g.tile + kv4_v_codes(p.D) + g.group * 512 + (r & 1) * 256 + g.j % 8 / 2 * 16 + r / 4 * 4 + g.j % 2 * 2 + g.j / 8;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = fmaf(__low2float(pair), (float)(c[i * 64] >> (r & 2 ? 4 : 0) & 15), __high2float(pair));
+  const int lane = threadIdx.x & 31;
+  const bool is_k = lane < 16;
+  int row = blockIdx.x;
+  for (int h = threadIdx.x >> 5; row < p.rows; h += kThreads / 32) {
+    while (h >= p.heads) {
+      h -= p.heads;
+      row += gridDim.x;
     }
-    store4<T, WIDE>((T *)p.k + g.row * p.k_ld + col, k);
-    store4<T, WIDE>((T *)p.v + g.row * p.v_ld + col, v);
+    if (row >= p.rows)
+      break;
+    const Place<D> g(p, row, h);
+    uint32_t word = 0, pair = 0;   // word of V: low nibbles (dims g) and high ones of this lane's four pairs
+    if (g.tile != nullptr) {
+      pair = *g.pair(is_k);
+      if (is_k) {
+        word = *g.k_word();
+      } else {
+        const uint8_t *v = g.v_bytes();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          word |= (uint32_t)(v[i * 64] & 15) << (4 * i) | (uint32_t)(v[i * 64] >> 4) << (16 + 4 * i);
+      }
+    }
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 1);
+    if (g.head >= p.kv_heads)
+      continue;
+    if (!is_k)   // the even lane's dims are the low nibbles of both, the odd one's the high
+      word = g.m & 1 ? other >> 16 | (word & 0xffff0000u) : (word & 0xffffu) | other << 16;
+    const __half2 both = *reinterpret_cast<const __half2 *>(&pair);
+    const float s = __low2float(both), l = __high2float(both);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x[i] = fmaf(s, (float)(word >> (is_k ? 4 * (i / 2 + 4 * (i & 1)) : 4 * i) & 15), l);
+    store8<T, WIDE>((T *)(is_k ? p.k : p.v) + row * (is_k ? p.k_ld : p.v_ld) + g.column(), x);
   }
 }
 
@@ -165,17 +201,20 @@ template <bool WRITE> int cache_launch(const b200_kv4_cache &c, const void *k, i
                                        int rows, cudaStream_t st) {
   if (rows == 0)
     return B200_OK;
-  const int64_t groups = (int64_t)rows * c.kv_heads * (c.head_dim / kKv4Group);
-  const CacheParams p{(uint8_t *)c.pool, (int64_t)c.n_pages * c.page, c.kv_heads, c.head_dim, c.page, (void *)k, (void *)v, k_ld, v_ld, slots, groups};
-  const int64_t blocks = (groups + kThreads / 16 - 1) / (kThreads / 16);
-  const dim3 grid((unsigned)(blocks < 148 * 64 ? blocks : 148 * 64));
+  const int heads = c.head_dim == 128 ? c.kv_heads : (c.kv_heads + 1) / 2, warps = kThreads / 32;
+  const CacheParams p{(uint8_t *)c.pool, (int64_t)c.n_pages * c.page, c.kv_heads, c.page, (void *)k, (void *)v, k_ld, v_ld, slots, rows, heads};
+  // a CTA takes rows that are the grid apart, its warps one head after the other
+  const int64_t ctas = ((int64_t)rows * heads + warps - 1) / warps;
+  const dim3 grid((unsigned)std::min<int64_t>(std::min<int64_t>(ctas, rows), 148 * 8));
   const int size = dtype == B200_F32 ? 4 : 2;
-  const bool wide = (((uintptr_t)k | (uintptr_t)v | (uintptr_t)(k_ld * size) | (uintptr_t)(v_ld * size)) & (4 * size - 1)) == 0;
-#define B200_TYPE(T)                                                                                                                       \
-  (WRITE ? launch_after(wide ? kv4_write_kernel<T, true> : kv4_write_kernel<T, false>, grid, kThreads, 0, st, p)                          \
-         : launch_after(wide ? kv4_read_kernel<T, true> : kv4_read_kernel<T, false>, grid, kThreads, 0, st, p))
+  const bool wide = (((uintptr_t)k | (uintptr_t)v | (uintptr_t)(k_ld * size) | (uintptr_t)(v_ld * size)) & 15) == 0;
+#define B200_KERNEL(D, T, W) (WRITE ? kv4_write_kernel<D, T, W> : kv4_read_kernel<D, T, W>)
+#define B200_TYPE(T)                                                                                                                            \
+  launch_after(c.head_dim == 128 ? (wide ? B200_KERNEL(128, T, true) : B200_KERNEL(128, T, false)) : (wide ? B200_KERNEL(64, T, true) : B200_KERNEL(64, T, false)), \
+               grid, kThreads, 0, st, p)
   return dtype == B200_F32 ? B200_TYPE(float) : dtype == B200_F16 ? B200_TYPE(__half) : B200_TYPE(__nv_bfloat16);
 #undef B200_TYPE
+#undef B200_KERNEL
 }
 
 int check_rows(const char *call, const b200_kv4_cache *c, const void *k, int64_t k_ld, const void *v, int64_t v_ld, int dtype, const int64_t *slots,

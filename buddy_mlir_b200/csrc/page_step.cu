@@ -1,15 +1,18 @@
 // One step of the page allocator on the device (b200_page_step): lengths in, block tables, slots and row maps out.
 //
 // Every CTA adds up all sequences (new rows, pages taken, pages given back: three prefix sums in shared memory) and then writes its share of
-// the outputs; a row, a page or a place of the stack finds its sequence by binary search.  Old values are read before the barrier, or are
-// never written (entries below a sequence's old end, places below the old top of the stack), so a step may be in place.
+// the outputs; a row, a page or a place of the stack finds its sequence by binary search.  Table entries and places of the stack that are read
+// (below a sequence's old end, below the old top) are not those that are written; lengths and the top may be written where they were read, by
+// one CTA, after the others where there are any: a second launch of its own.
 #include "kv4.cuh"
+
+#include <algorithm>
 
 namespace b200 {
 
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32;
+constexpr int kThreads = 1024, kWarps = kThreads / 32, kMostCtas = 148;
 
 struct Sums {
   long long rows, taken, given;
@@ -32,7 +35,8 @@ __device__ __forceinline__ int owner(const int32_t *first, int n, int x) {
   return lo;
 }
 
-__global__ void __launch_bounds__(kThreads) page_step_kernel(const __grid_constant__ b200_page_step_args p) {
+// what: 1 rows, tables, stack and status; 2 lengths and the stack's top
+__global__ void __launch_bounds__(kThreads) page_step_kernel(const __grid_constant__ b200_page_step_args p, const int what) {
   extern __shared__ int32_t s_all[];
   __shared__ Sums s_warp[kWarps];
   __shared__ int s_over, s_state;
@@ -111,37 +115,40 @@ __global__ void __launch_bounds__(kThreads) page_step_kernel(const __grid_consta
     const int at = top - 1 - i;
     return at < n_free ? p.free_pages[at] : returned(at - n_free);
   };
-  for (int r = tid; r < p.max_rows; r += kThreads) {
-    int64_t slot = -1;
-    int seq = -1, pos = -1;
-    if (r < rows) {
-      seq = owner(s_row, n, r);
-      pos = s_held[seq] + r - s_row[seq];
-      const int have = (s_held[seq] + p.page - 1) / p.page, at = pos / p.page;
-      const int page = at < have ? p.block_table[(int64_t)seq * p.table_stride + at] : new_page(s_take[seq] + at - have);
-      slot = (int64_t)page * p.page + pos % p.page;
+  const int at0 = blockIdx.x * kThreads + tid, step = gridDim.x * kThreads;
+  if (what & 1) {
+    for (int r = at0; r < p.max_rows; r += step) {
+      int64_t slot = -1;
+      int seq = -1, pos = -1;
+      if (r < rows) {
+        seq = owner(s_row, n, r);
+        pos = s_held[seq] + r - s_row[seq];
+        const int have = (s_held[seq] + p.page - 1) / p.page, at = pos / p.page;
+        const int page = at < have ? p.block_table[(int64_t)seq * p.table_stride + at] : new_page(s_take[seq] + at - have);
+        slot = (int64_t)page * p.page + pos % p.page;
+      }
+      p.slots[r] = slot;
+      if (p.row_seq != nullptr)
+        p.row_seq[r] = seq;
+      if (p.row_pos != nullptr)
+        p.row_pos[r] = pos;
     }
-    p.slots[r] = slot;
-    if (p.row_seq != nullptr)
-      p.row_seq[r] = seq;
-    if (p.row_pos != nullptr)
-      p.row_pos[r] = pos;
+    for (int i = at0; i < taken; i += step) {
+      const int s = owner(s_take, n, i), have = (s_held[s] + p.page - 1) / p.page;
+      p.block_table[(int64_t)s * p.table_stride + have + i - s_take[s]] = new_page(i);
+    }
+    for (int i = at0; i < given - taken; i += step)   // what stays on the stack of them
+      p.free_pages[n_free + i] = returned(i);
+    for (int s = at0; s <= n; s += step)
+      p.row_start[s] = ok ? s_row[s] : 0;
+    if (at0 == 0)
+      *p.status = status;
   }
-  for (int i = tid; i < taken; i += kThreads) {
-    const int s = owner(s_take, n, i), have = (s_held[s] + p.page - 1) / p.page;
-    p.block_table[(int64_t)s * p.table_stride + have + i - s_take[s]] = new_page(i);
-  }
-  for (int i = tid; i < given - taken; i += kThreads)   // what stays on the stack of them
-    p.free_pages[n_free + i] = returned(i);
-  for (int s = tid; s < n; s += kThreads) {
-    const int add = p.add[s];
-    p.held_out[s] = !ok ? s_held[s] : add < 0 ? 0 : s_held[s] + add;
-  }
-  for (int s = tid; s <= n; s += kThreads)
-    p.row_start[s] = ok ? s_row[s] : 0;
-  if (tid == 0) {
-    *p.n_free_out = ok ? top - taken : n_free;
-    *p.status = status;
+  if (what & 2) {
+    for (int s = at0; s < n; s += step)
+      p.held_out[s] = !ok ? s_held[s] : s_row[s + 1] > s_row[s] ? s_held[s] + s_row[s + 1] - s_row[s] : p.add[s] < 0 ? 0 : s_held[s];
+    if (at0 == 0)
+      *p.n_free_out = ok ? top - taken : n_free;
   }
 }
 
@@ -153,7 +160,12 @@ int page_step_launch(const b200_page_step_args &a, cudaStream_t st) {
   const int bytes = 4 * (4 * a.n_seqs + 3);
   if (int rc = raise_shared_limit(g_raised, (const void *)page_step_kernel, 4 * (4 * B200_PAGE_STEP_MAX_SEQS + 3)))
     return rc;
-  return launch_after(page_step_kernel, dim3(1), kThreads, bytes, st, a);
+  // one CTA up to 2048 rows (4.9 us; more CTAs gain nothing there), then one for every 1024
+  const int ctas = a.max_rows <= 2048 ? 1 : std::min(kMostCtas, (a.max_rows + kThreads - 1) / kThreads);
+  const bool apart = ctas > 1 && (a.held_out == a.held || a.n_free_out == a.n_free);
+  if (int rc = launch_after(page_step_kernel, dim3(ctas), kThreads, bytes, st, a, apart ? 1 : 3))
+    return rc;
+  return apart ? launch_after(page_step_kernel, dim3(1), kThreads, bytes, st, a, 2) : B200_OK;
 }
 
 } // namespace b200
