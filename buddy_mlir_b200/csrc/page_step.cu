@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(kThreads) page_step_kernel(const __grid_consta
   extern __shared__ int32_t s_all[];
   __shared__ Sums s_warp[kWarps];
   __shared__ int s_over, s_state;
-  const int n = p.n_seqs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n = p.n_seqs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads / 32;
   int32_t *s_row = s_all, *s_take = s_row + n + 1, *s_give = s_take + n + 1, *s_held = s_give + n + 1;
   kernel_go();
   if (tid == 0)
@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kThreads) page_step_kernel(const __grid_consta
   __syncthreads();
 
   // ---- this thread's sequences, then all before them ------------------------------------------------------------------------
-  const int per = (n + kThreads - 1) / kThreads, first = min(n, tid * per), last = min(n, first + per);
+  const int per = (n + threads - 1) / threads, first = min(n, tid * per), last = min(n, first + per);
   const long long room = (long long)p.table_stride * p.page;
   Sums mine{0, 0, 0};
   bool over = false, bad = false;
@@ -76,12 +76,18 @@ __global__ void __launch_bounds__(kThreads) page_step_kernel(const __grid_consta
   if (lane == 31)
     s_warp[warp] = sum;
   __syncthreads();
-  Sums before{0, 0, 0}, total{0, 0, 0};
-  for (int w = 0; w < kWarps; ++w) {
-    if (w == warp)
-      before = total;
-    total = total + s_warp[w];
+  Sums upto = lane < warps ? s_warp[lane] : Sums{0, 0, 0};   // (every warp adds up the warps' sums)
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const Sums v = up(upto, o);
+    if (lane >= o)
+      upto = upto + v;
   }
+  const Sums total{__shfl_sync(0xffffffffu, upto.rows, 31), __shfl_sync(0xffffffffu, upto.taken, 31), __shfl_sync(0xffffffffu, upto.given, 31)};
+  const int one = max(warp - 1, 0);
+  Sums before{__shfl_sync(0xffffffffu, upto.rows, one), __shfl_sync(0xffffffffu, upto.taken, one), __shfl_sync(0xffffffffu, upto.given, one)};
+  if (warp == 0)
+    before = Sums{0, 0, 0};
   const int status = s_state || n_free < 0 || n_free > p.n_pages || n_free + total.given > p.n_pages ? B200_PAGES_STATE
                      : s_over                                                                        ? B200_PAGES_TABLE
                      : total.rows > p.max_rows                                                       ? B200_PAGES_ROWS
@@ -115,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) page_step_kernel(const __grid_consta
     const int at = top - 1 - i;
     return at < n_free ? p.free_pages[at] : returned(at - n_free);
   };
-  const int at0 = blockIdx.x * kThreads + tid, step = gridDim.x * kThreads;
+  const int at0 = blockIdx.x * threads + tid, step = gridDim.x * threads;
   if (what & 1) {
     for (int r = at0; r < p.max_rows; r += step) {
       int64_t slot = -1;
@@ -160,10 +166,11 @@ int page_step_launch(const b200_page_step_args &a, cudaStream_t st) {
   const int bytes = 4 * (4 * a.n_seqs + 3);
   if (int rc = raise_shared_limit(g_raised, (const void *)page_step_kernel, 4 * (4 * B200_PAGE_STEP_MAX_SEQS + 3)))
     return rc;
-  // one CTA up to 2048 rows (4.9 us; more CTAs gain nothing there), then one for every 1024
+  // one CTA up to 2048 rows, a small one for a few sequences, then one for every 1024
   const int ctas = a.max_rows <= 2048 ? 1 : std::min(kMostCtas, (a.max_rows + kThreads - 1) / kThreads);
+  const int threads = ctas == 1 && a.n_seqs <= 256 && a.max_rows <= 512 ? 256 : kThreads;
   const bool apart = ctas > 1 && (a.held_out == a.held || a.n_free_out == a.n_free);
-  if (int rc = launch_after(page_step_kernel, dim3(ctas), kThreads, bytes, st, a, apart ? 1 : 3))
+  if (int rc = launch_after(page_step_kernel, dim3(ctas), threads, bytes, st, a, apart ? 1 : 3))
     return rc;
   return apart ? launch_after(page_step_kernel, dim3(1), kThreads, bytes, st, a, 2) : B200_OK;
 }
