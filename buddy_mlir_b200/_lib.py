@@ -114,6 +114,7 @@ def load():
         "b200_kv4_read": (i32, [C.POINTER(Kv4Cache), vp, i64, vp, i64, i32, vp, i32, vp]),
         "b200_page_step": (i32, [C.POINTER(PageStep), vp]),
         "b200_kv4_attention_workspace_bytes": (i64, [i32, i32, i32]),
+        "b200_kv4_attention_status": (i32, [vp, vp]),
         "b200_kv4_attention": (i32, [C.POINTER(Kv4Cache), C.POINTER(Kv4Attention), vp, i64, vp]),
         "b200_model_create": (i32, [C.POINTER(ModelConfigC), C.POINTER(vp)]),
         "b200_model_destroy": (None, [vp]),

@@ -9,7 +9,7 @@
 //
 // The reference r of a row's weights is not its largest score but the largest of score + log2 of the key's larger V scale, so that the weights
 // that meet codes, p s, are at most 2^12 and near 2^8 where they count, whatever the scales are; sums and totals carry the same factor.
-#include "kv4.cuh"
+#include "kv4_plan.cuh"
 
 #include <algorithm>
 
@@ -17,47 +17,20 @@ namespace b200 {
 
 namespace {
 
-constexpr int kWarps = 16, kThreads = 32 * kWarps, kCtas = 148;
+constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr int kRows = 8;            // query rows of an item: a position's heads (several positions', if they are few)
 constexpr int kSlots = 4;           // tiles that a warp has in flight or in hand
+constexpr int kChunkRows = 64;     // query vectors of a sequence and kv head from which on tcgen05 has them
 constexpr int kLeastKeys = 512;     // of a CTA, where there are not more CTAs than that asks for
-constexpr int kSnap = 256;          // keys that a CTA may have more or fewer, so that it begins with an item (few of many: a quarter)
-constexpr int kMany = 4096;
-constexpr float kTop = 8.f;          // powers of two: what the largest weight p s is at when a row's reference is set,
-constexpr float kLag = 4.f;          // and how far above that one may come before it is set again
-constexpr float kSeed = -1.0e30f;
 constexpr float kLeastScale = 5.9604645e-8f;   // (f16's smallest: a group of equal values has the scale 0)
-
-struct AttentionParams {
-  const uint8_t *pool;
-  int n_pages, kv_heads, page;
-  b200_kv4_attention_args a;
-  int G, heads, tokens, subs;       // q heads of a kv head, of an item; positions of an item; items that share a kv head's q heads
-  float log2_scale;
-  bool wide_q;                      // rows of q are aligned to four elements
-  int *counters;                    // [kCtas]
-  float *parts;                     // [kCtas][2][part floats], then [kCtas * kWarps][part floats]
-};
 
 __host__ __device__ constexpr int part_floats(int D) { return kRows * (D + 4) + 2 * kRows; }   // sums in rows of D + 4, maxima, totals
 
-__device__ __forceinline__ int clamp(long long x, int lo, int hi) { return (int)(x < lo ? lo : x > hi ? hi : x); }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float2 halves(uint32_t pair) { return __half22float2(*reinterpret_cast<const __half2 *>(&pair)); }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -107,27 +80,6 @@ template <int TERMS> __device__ __forceinline__ void split(float x, float y, uin
   }
 }
 
-// A sequence as its items: its rows `tokens` at a time and, for each kv head (or part of its q heads), a range of keys that ends at the last
-// row's own position.  Cost of an item: its keys; of all items before it in a head: before().
-struct Sequence {
-  int r0, n;            // rows
-  int base;             // position of the first row (negative: rows before it see nothing), at most the table's room
-  int past, tiles;      // max(base, 0); row tiles
-  __device__ __forceinline__ Sequence(int first, int end, int position, int tokens) : r0(first), n(max(end - first, 0)), base(position) {
-    past = max(base, 0);
-    tiles = n <= tokens ? min(n, 1) : (n + tokens - 1) / tokens;
-  }
-  __device__ __forceinline__ long long before(int rt, int tokens) const {
-    return rt == 0 ? 0
-           : rt < tiles ? (long long)rt * past + (long long)tokens * rt * (rt + 1) / 2
-                        : (long long)(tiles - 1) * past + (long long)tokens * tiles * (tiles - 1) / 2 + past + n;
-  }
-};
-// x * a / b, rounded down
-__device__ __forceinline__ long long share(long long x, int a, int b) {
-  return x < (1 << 24) && a <= 255 ? (long long)((uint32_t)x * a / (uint32_t)b) : x * a / b;
-}
-
 template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
   static constexpr int GROUPS = D / kKv4Group, STEPS = D / 16, BYTES = kv4_tile_bytes(D);
   static constexpr bool EXACT = TYPE == B200_F32;
@@ -148,7 +100,7 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
         o[i][e] = 0.f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      r[e] = kSeed;
+      r[e] = kKv4Seed;
       l[e] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < GROUPS; ++gr)
@@ -156,22 +108,8 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
     }
   }
 
-  __device__ __forceinline__ static void load_wide(const void *q, int64_t at, float (&x)[4]) {
-    if constexpr (TYPE == B200_F32) {
-      *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>((const float *)q + at);
-    } else {
-      const uint2 v = *reinterpret_cast<const uint2 *>((const uint16_t *)q + at);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t w = e ? v.y : v.x;
-        const float2 f = TYPE == B200_F16 ? halves(w) : make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-        x[2 * e] = f.x;
-        x[2 * e + 1] = f.y;
-      }
-    }
-  }
   // q of this lane's row (lane / 4), or none
-  __device__ __forceinline__ void load_q(const AttentionParams &p, bool live, int64_t at) {
+  __device__ __forceinline__ void load_q(const Kv4Params &p, bool live, int64_t at) {
     const int lane = threadIdx.x & 31, t = lane & 3;
     float x[STEPS][4], most = 0.f;
 #pragma unroll
@@ -181,7 +119,7 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
       for (int e = 0; e < 4; ++e)
         x[k][e] = live && !p.wide_q ? load_as_float(p.a.q, TYPE, at + d + e) : 0.f;
       if (live && p.wide_q)
-        load_wide(p.a.q, at + d, x[k]);
+        load_wide<TYPE>(p.a.q, at + d, x[k]);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         most = fmaxf(most, fabsf(x[k][e]));
@@ -292,13 +230,13 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
         }
       }
     }
-    if (__any_sync(0xffffffffu, top[0] > r[0] + (kTop + kLag) || top[1] > r[1] + (kTop + kLag))) {
+    if (__any_sync(0xffffffffu, top[0] > r[0] + (kKv4Top + kKv4Lag) || top[1] > r[1] + (kKv4Top + kKv4Lag))) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1)
           top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
-        top[e] = top[e] > r[e] + (kTop + kLag) ? top[e] - kTop : r[e];   // (each row for itself)
+        top[e] = top[e] > r[e] + (kKv4Top + kKv4Lag) ? top[e] - kKv4Top : r[e];   // (each row for itself)
         const float keep = ex2(r[e] - top[e]);
         r[e] = top[e];
         l[e] *= keep;
@@ -413,26 +351,10 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
   }
 };
 
-template <int TYPE> __device__ __forceinline__ void put(const AttentionParams &p, int64_t at, float x) {
-  if constexpr (TYPE == B200_F32)
-    ((float *)p.a.out)[at] = x;
-  else if constexpr (TYPE == B200_F16)
-    ((__half *)p.a.out)[at] = __float2half_rn(x);
-  else
-    ((__nv_bfloat16 *)p.a.out)[at] = __float2bfloat16_rn(x);
-}
-// element of an item's row in q (ld: q's) or out, before its dims
-__device__ __forceinline__ int64_t row_at(const AttentionParams &p, int r0, int rt, int slot, int row, int64_t ld, int D) {
-  return (r0 + (int64_t)rt * p.tokens + row / p.heads) * ld + (int64_t)((slot / p.subs) * p.G + slot % p.subs * p.heads + row % p.heads) * D;
-}
-__device__ __forceinline__ int rows_of(const AttentionParams &p, const Sequence &q, int rt, int slot) {   // of an item
+__device__ __forceinline__ int rows_of(const Kv4Params &p, const Sequence &q, int rt, int slot) {   // of an item
   const int tokens = min(p.tokens, q.n - rt * p.tokens);
   return p.subs == 1 ? tokens * p.heads : min(p.heads, p.G - slot % p.subs * p.heads);
 }
-// Where a warp stands: an item and the next of its tiles.
-struct Place {
-  int s, slot, rt, tile;
-};
 
 // What a warp leaves behind: parts of its first item (that began before it) and of its last (that goes on behind it).
 struct Left {
@@ -442,137 +364,45 @@ struct Left {
   bool has_a, a_ends, has_b;
 };
 
-template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_attention_kernel(const __grid_constant__ AttentionParams p) {
+template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_attention_kernel(const __grid_constant__ Kv4Params p) {
   using T = Tile<D, TYPE>;
   constexpr int BYTES = T::BYTES, PART = part_floats(D), RING = kSlots * BYTES, KT = T::KT, STAGES = kSlots / KT;
   static_assert(RING >= PART * 4, "a part of a warp lies in its ring");
   extern __shared__ __align__(128) uint8_t s_all[];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.a.n_seqs, room = p.a.table_stride * p.page, slots = p.kv_heads * p.subs;
-  long long *s_cost = reinterpret_cast<long long *>(s_all + kWarps * RING);          // [n + 1]
-  int *s_r0 = reinterpret_cast<int *>(s_cost + n + 1), *s_base = s_r0 + n + 1;      // [n + 1], [n]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.a.n_seqs, room = p.a.table_stride * p.page;
   __shared__ long long s_sum[kWarps];
   __shared__ Left s_left[kWarps];
   __shared__ int s_ctas[2][3];     // of a shared item that this CTA adds up: whether it does, the CTAs with its first and last part
   kernel_go();
   kernel_wait();
 
-  // ---- costs of all sequences, added up --------------------------------------------------------------------------------------
-  {
-    const int per = (n + kThreads - 1) / kThreads, first = min(n, tid * per), last = min(n, first + per);
-    long long sum = 0;
-    for (int s = first; s < last; ++s) {
-      const int r0 = clamp(p.a.row_start[s], 0, p.a.rows), r1 = clamp(p.a.row_start[s + 1], 0, p.a.rows);
-      const int rows = max(r1 - r0, 0), base = clamp((long long)p.a.lens[s] - rows, -rows, room);
-      s_r0[s] = r0;
-      s_base[s] = base;
-      if (s == n - 1)
-        s_r0[n] = r1;
-      const Sequence q(r0, r1, base, p.tokens);
-      s_cost[s] = sum;
-      sum += slots * q.before(q.tiles, p.tokens);
-    }
-    long long upto = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o)
-        upto += v;
-    }
-    if (lane == 31)
-      s_sum[warp] = upto;
-    if (lane == 0)
-      s_left[warp].has_a = s_left[warp].has_b = false;
-    if (tid < 2)
-      s_ctas[tid][0] = 0;
-    __syncthreads();
-    long long before = upto - sum;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w)
-      before += w < warp ? s_sum[w] : 0;
-    if (before != 0)
-      for (int s = first; s < last; ++s)
-        s_cost[s] += before;
-    if (tid == kThreads - 1)
-      s_cost[n] = before + sum;
-    __syncthreads();
-  }
-  auto sequence = [&](int s) { return Sequence(s_r0[s], s_r0[s + 1], s_base[s], p.tokens); };
+  if (lane == 0)
+    s_left[warp].has_a = s_left[warp].has_b = false;
+  if (tid < 2)
+    s_ctas[tid][0] = 0;
+  KeyPlan<4> plan;
+  plan.build<kThreads>(p, s_all + kWarps * RING, s_sum, kLeastKeys);
   // rows of no sequence
-  {
-    const int lo = s_r0[0], hi = max(lo, s_r0[n]), none = lo + p.a.rows - hi, cols = p.a.q_heads * D;
-    if (none > 0)
-      for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < (int64_t)none * cols; i += (int64_t)gridDim.x * kThreads) {
-        const int r = (int)(i / cols);
-        put<TYPE>(p, (int64_t)(r < lo ? r : hi + r - lo) * p.a.out_ld + i % cols, 0.f);
-      }
+  if (p.fill) {
+    const int lo = plan.r0[0], hi = max(lo, plan.r0[n]), none = lo + p.a.rows - hi, cols = p.a.q_heads * D;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < (int64_t)none * cols; i += (int64_t)gridDim.x * kThreads) {
+      const int r = (int)(i / cols);
+      put<TYPE>(p, (int64_t)(r < lo ? r : hi + r - lo) * p.a.out_ld + i % cols, 0.f);
+    }
   }
 
   // ---- this CTA's keys, this warp's keys ----------------------------------------------------------------------------------------
-  const long long total = s_cost[n];
-  const int ctas = total >= (long long)gridDim.x * kLeastKeys ? gridDim.x : max(1, (int)total / kLeastKeys);
-  if (total == 0 || (int)blockIdx.x >= ctas)
+  const long long total = plan.total;
+  if (total == 0 || (int)blockIdx.x >= plan.ctas)
     return;
-  const long long chunk = share(total, 1, ctas);
-  const int window = chunk > kMany ? kSnap / 4 : (int)min((long long)kSnap, chunk / 2 - 1);
-  auto locate = [&](long long x, Place &at, long long &begin, long long &end) {   // the item with key x, from begin to end; at.tile: the first tile from x on
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_cost[mid] <= x)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    at.s = lo;
-    const Sequence q = sequence(lo);
-    begin = s_cost[lo];
-    const long long head = q.before(q.tiles, p.tokens);
-    at.slot = (x - begin) >> 32 ? (int)((x - begin) / head) : (int)((uint32_t)(x - begin) / (uint32_t)min(head, 0xffffffffll));
-    begin += at.slot * head;
-    int a = 0, b = q.tiles;
-    while (b - a > 1) {
-      const int mid = (a + b) >> 1;
-      if (q.before(mid, p.tokens) <= x - begin)
-        a = mid;
-      else
-        b = mid;
-    }
-    at.rt = a;
-    end = begin + q.before(a + 1, p.tokens);
-    begin += q.before(a, p.tokens);
-    at.tile = (int)((x - begin + 15) >> 4);
-  };
-  auto border = [&](int c) {   // where CTA c begins: at its share of all keys, or at the item border next to that
-    if (c <= 0 || c >= ctas)
-      return c <= 0 ? 0 : total;
-    const long long x = share(total, c, ctas);
-    Place at;
-    long long begin, end;
-    locate(x, at, begin, end);
-    return x - begin <= end - x ? (x - begin <= window ? begin : x) : end - x <= window ? end : x;
-  };
-  auto nominal = [&](long long x) { return (int)(((x + 1) * ctas - 1) / total); };   // the CTA that x would lie in without that
-  auto item_tiles = [&](const Sequence &q, int rt) { return (q.past + min((rt + 1) * p.tokens, q.n) + 15) >> 4; };
-  auto next_item = [&](Place &at, const Sequence &q) {
-    at.tile = 0;
-    if (++at.rt < q.tiles)
-      return;
-    at.rt = 0;
-    if (++at.slot < slots)
-      return;
-    at.slot = 0;
-    do
-      ++at.s;
-    while (at.s < n && s_cost[at.s + 1] == s_cost[at.s]);
-  };
-  long long x = border(blockIdx.x + min(lane, 1));   // (a lane each)
+  long long x = plan.border(blockIdx.x + min(lane, 1));   // (a lane each)
   const long long cta_begin = __shfl_sync(0xffffffffu, x, 0), mine = __shfl_sync(0xffffffffu, x, 1) - cta_begin;
   const int act = (int)max(1ll, min((long long)kWarps, mine >> 4));   // the warps that work: sixteen keys each at least (then each begins a tile)
   Place at{n, 0, 0, 0}, stop;
   x = cta_begin + share(mine, warp + min(lane, 1), act);
   if (x < total) {
     long long begin, end;
-    locate(x, at, begin, end);
+    plan.locate(x, at, begin, end);
   }
   stop.s = __shfl_sync(0xffffffffu, at.s, 1);
   stop.slot = __shfl_sync(0xffffffffu, at.slot, 1);
@@ -587,10 +417,10 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
     uint8_t *ring = s_all + warp * RING;
     T tile;
     while (at.s < n) {
-      const Sequence q = sequence(at.s);
-      const int all = item_tiles(q, at.rt);
+      const Sequence q = plan.sequence(at.s);
+      const int all = plan.item_tiles(q, at.rt);
       if (at.tile >= all) {   // (a border behind an item's last tile)
-        next_item(at, q);
+        plan.next_item(at, q);
         continue;
       }
       const bool here = stop.s == at.s && stop.slot == at.slot && stop.rt == at.rt;
@@ -600,13 +430,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
       // ---- this warp's tiles of the item ----------------------------------------------------------------------------------------
       const int live = rows_of(p, q, at.rt, at.slot), first_token = at.rt * p.tokens, tokens = min(p.tokens, q.n - first_token);
       const int least = clamp((long long)q.base + first_token + 1, 0, room), most = clamp((long long)q.base + first_token + tokens, 0, room);
-      const int kv = at.slot / p.subs, per_page = p.page / kKv4Tile;
-      auto source = [&](int t) {   // of a tile: its number in the pool, or -1
-        if (t >= t1 || t * kKv4Tile >= most)
-          return -1;
-        const int id = p.a.block_table[(int64_t)at.s * p.a.table_stride + t / per_page];
-        return id < 0 || id >= p.n_pages ? -1 : (id * p.kv_heads + kv) * per_page + t % per_page;
-      };
+      auto source = [&](int t) { return t >= t1 || t * kKv4Tile >= most ? -1 : tile_source(p, at.s, at.slot / p.subs, t); };
       int now = source(t0 + lane), next = source(t0 + 32 + lane);
       tile.clear();
       uint32_t none = 0;            // bit of a slot: nothing to see in its tile
@@ -638,7 +462,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
 #pragma unroll
       for (int i = 0; i < STAGES - 1; ++i)
         request(i * KT);
-      tile.load_q(p, lane / 4 < live, lane / 4 < live ? row_at(p, q.r0, at.rt, at.slot, lane / 4, p.a.q_ld, D) : 0);
+      tile.load_q(p, lane / 4 < live, lane / 4 < live ? row_at(p, q.r0 + first_token, at.slot, lane / 4, p.a.q_ld, D) : 0);
 #pragma unroll 1
       for (int i = 0; i < count; i += KT) {
         copies_wait<STAGES - 2>();
@@ -677,7 +501,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
         for (int e = 0; e < 2; ++e) {
           const int row = 2 * (lane & 3) + e;
           if (row < live) {
-            const int64_t to = row_at(p, q.r0, at.rt, at.slot, row, p.a.out_ld, D) + lane / 4;
+            const int64_t to = row_at(p, q.r0 + first_token, at.slot, row, p.a.out_ld, D) + lane / 4;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
               put<TYPE>(p, to + 16 * i, tile.l[e] == 0.f ? 0.f : tile.o[i][e] * over[e]);
@@ -686,7 +510,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
           }
         }
       } else {   // a part of the first item, or of the last; that of the first has to lie elsewhere where others follow
-        float *part = t0 > 0 && !here ? p.parts + ((int64_t)2 * kCtas + blockIdx.x * kWarps + warp) * PART : reinterpret_cast<float *>(ring);
+        float *part = t0 > 0 && !here ? p.parts + ((int64_t)2 * kKv4Ctas + blockIdx.x * kWarps + warp) * PART : reinterpret_cast<float *>(ring);
         tile.store(part);
         if (lane == 0) {
           Left &left = s_left[warp];
@@ -705,7 +529,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
       }
       if (here)
         break;
-      next_item(at, q);
+      plan.next_item(at, q);
     }
   }
   __syncthreads();
@@ -739,10 +563,10 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
     o = make_float4(fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w));
   };
   auto write_out = [&](const Place &at, int row, int d, float4 o, float l) {
-    const Sequence q = sequence(at.s);
+    const Sequence q = plan.sequence(at.s);
     if (row >= rows_of(p, q, at.rt, at.slot))
       return;
-    const int64_t to = row_at(p, q.r0, at.rt, at.slot, row, p.a.out_ld, D) + d;
+    const int64_t to = row_at(p, q.r0 + at.rt * p.tokens, at.slot, row, p.a.out_ld, D) + d;
     const float over = l == 0.f ? 0.f : 1.f / l;
     put<TYPE>(p, to, l == 0.f ? 0.f : o.x * over);
     put<TYPE>(p, to + 1, l == 0.f ? 0.f : o.y * over);
@@ -754,7 +578,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
   for (int k = tid / FOURS; k < chains; k += kThreads / FOURS) {
     const Chain c = chain(k);
     auto part = [&](int w) { return c.opened && w == c.first ? reinterpret_cast<const float *>(s_all + w * RING) : s_left[w].a_part; };
-    float top = kSeed, l = 0.f;
+    float top = kKv4Seed, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int w = c.first; w <= c.last; ++w)
       top = fmaxf(top, part(w)[kRows * (D + 4) + row]);
@@ -778,30 +602,15 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
     return;
   __threadfence();
   __syncthreads();
-  // An item's tiles are counted as its parts arrive, in the counter of the CTA that would begin it were there no borders moved (no two items that are
-  // shared have the same); who completes them adds its parts up, in their order.
   if (warp < 2 && (warp == 0 ? incoming : outgoing)) {
     const Chain c = chain(warp == 0 ? 0 : chains - 1);
-    const Place item = c.opened ? s_left[c.first].b : s_left[0].a;
-    const Sequence q = sequence(item.s);
-    const int all = item_tiles(q, item.rt);
-    const long long first = s_cost[item.s] + item.slot * q.before(q.tiles, p.tokens) + q.before(item.rt, p.tokens), last = first + 16ll * (all - 1);
-    const int from = nominal(first), to = nominal(last);
-    int tiles = 0, before = 0;
+    int tiles = 0, from, to;
     for (int w = c.first; w <= c.last; ++w)
       tiles += c.opened && w == c.first ? s_left[w].b_tiles : s_left[w].a_tiles;
-    if (lane == 0)
-      before = atomicAdd(p.counters + from, tiles);
-    if (__shfl_sync(0xffffffffu, before, 0) + tiles == all) {
-      const long long x = border(lane == 0 ? from + 1 : lane == 1 ? to : to + 1);   // (a lane each)
-      const bool later = __shfl_sync(0xffffffffu, (int)(x <= first), 0), sooner = __shfl_sync(0xffffffffu, (int)(x > last), 1),
-                 beyond = __shfl_sync(0xffffffffu, (int)(x <= last), 2);
-      if (lane == 0) {
-        p.counters[from] = 0;
-        s_ctas[warp][0] = 1;
-        s_ctas[warp][1] = from + later;
-        s_ctas[warp][2] = to - sooner + beyond;
-      }
+    if (plan.arrive(p.counters, c.opened ? s_left[c.first].b : s_left[0].a, tiles, from, to) && lane == 0) {
+      s_ctas[warp][0] = 1;
+      s_ctas[warp][1] = from;
+      s_ctas[warp][2] = to;
     }
   }
   __syncthreads();
@@ -812,7 +621,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
     const Chain c = chain(k == 0 ? 0 : chains - 1);
     const int from = s_ctas[k][1], to = s_ctas[k][2];
     auto part = [&](int b) { return p.parts + ((int64_t)b * 2 + (b == from)) * PART; };
-    float top = kSeed, l = 0.f;
+    float top = kKv4Seed, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int b = from; b <= to; ++b)
@@ -827,11 +636,11 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
 
 RaisedOn g_raised[6];
 
-template <int D, int TYPE> int attention_launch(RaisedOn &raised, const AttentionParams &p, cudaStream_t st) {
+template <int D, int TYPE> int attention_launch(RaisedOn &raised, const Kv4Params &p, cudaStream_t st) {
   const int fixed = kWarps * kSlots * kv4_tile_bytes(D);
-  if (int rc = raise_shared_limit(raised, (const void *)kv4_attention_kernel<D, TYPE>, fixed + 16 * (B200_KV4_ATTENTION_MAX_SEQS + 1)))
+  if (int rc = raise_shared_limit(raised, (const void *)kv4_attention_kernel<D, TYPE>, fixed + KeyPlan<4>::bytes(B200_KV4_ATTENTION_MAX_SEQS)))
     return rc;
-  return launch_after(kv4_attention_kernel<D, TYPE>, dim3(kCtas), kThreads, fixed + 16 * (p.a.n_seqs + 1), st, p);
+  return launch_after(kv4_attention_kernel<D, TYPE>, dim3(kKv4Ctas), kThreads, fixed + KeyPlan<4>::bytes(p.a.n_seqs), st, p);
 }
 
 } // namespace
@@ -845,7 +654,18 @@ extern "C" {
 int64_t b200_kv4_attention_workspace_bytes(int q_heads, int kv_heads, int head_dim) {
   if (kv_heads < 1 || kv_heads > 1024 || q_heads < 1 || q_heads % kv_heads != 0 || (head_dim != 64 && head_dim != 128))
     return B200_EINVAL;
-  return 2048 + (int64_t)kCtas * (2 + kWarps) * part_floats(head_dim) * 4;
+  return 2048 + (int64_t)kKv4Ctas * std::max<int64_t>((2 + kWarps) * part_floats(head_dim), kv4_chunk_part_floats(head_dim)) * 4;
+}
+
+int b200_kv4_attention_status(void *workspace, void *stream) {
+  if (!workspace)
+    return fail(B200_EINVAL, "kv4_attention_status: null workspace");
+  if (int rc = ensure_device())
+    return rc;
+  int code = 0, *at = (int *)workspace + kKv4Ctas;
+  B200_CUDA(cudaMemcpyAsync(&code, at, 4, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
+  B200_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+  return code == 0 ? B200_OK : fail(B200_ECUDA, "kv4_attention: a bounded wait gave up (code %d)", code);
 }
 
 int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a, void *workspace, int64_t workspace_bytes, void *stream) {
@@ -875,17 +695,41 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
                 (long long)b200_kv4_attention_workspace_bytes(a->q_heads, c->kv_heads, c->head_dim));
   if (int rc = ensure_device())
     return rc;
-  AttentionParams p{(const uint8_t *)c->pool, c->n_pages, c->kv_heads, c->page, *a};
+  Kv4Params p{};
+  p.pool = (const uint8_t *)c->pool;
+  p.n_pages = c->n_pages;
+  p.kv_heads = c->kv_heads;
+  p.page = c->page;
+  p.a = *a;
   p.G = a->q_heads / c->kv_heads;
-  p.subs = (p.G + kRows - 1) / kRows;
-  p.heads = std::min(p.G, kRows);
-  p.tokens = p.subs == 1 ? kRows / p.G : 1;
   p.log2_scale = a->scale * 1.4426950408889634f;
   const int size = a->dtype == B200_F32 ? 4 : 2;
   p.wide_q = (((uintptr_t)a->q | (uintptr_t)(a->q_ld * size)) & (4 * size - 1)) == 0;
+  p.wide_out = (((uintptr_t)a->out | (uintptr_t)(a->out_ld * size)) & (4 * size - 1)) == 0;
   p.counters = (int *)workspace;
   p.parts = (float *)((char *)workspace + 2048);
+  p.fill = 1;
+  p.least_rows = 1;
+  p.most_rows = INT32_MAX;
+  p.subs = (p.G + kRows - 1) / kRows;
+  p.heads = std::min(p.G, kRows);
+  p.tokens = p.subs == 1 ? kRows / p.G : 1;
   cudaStream_t st = (cudaStream_t)stream;
+  // Sequences of many rows go to tcgen05, in a launch of their own; who has how many rows is known on the device only, so both launches are made where
+  // the mean does not say that there are none of one kind.
+  if (kv4_chunk_takes(a->dtype, p.G, a->n_seqs) && (int64_t)a->rows * p.G >= kChunkRows && a->rows >= 2 * (int64_t)a->n_seqs) {
+    const int from = (kChunkRows + p.G - 1) / p.G;
+    Kv4Params chunk = p;
+    if (a->n_seqs > 1) {
+      p.most_rows = from - 1;
+      chunk.least_rows = from;
+      chunk.fill = 0;
+    }
+    if (int rc = kv4_chunk_launch(chunk, c->head_dim, st))
+      return rc;
+    if (a->n_seqs == 1)
+      return B200_OK;
+  }
 #define B200_D(D_)                                                                                                                    \
   (a->dtype == B200_F32   ? attention_launch<D_, B200_F32>(g_raised[D_ / 64 - 1], p, st)                                              \
    : a->dtype == B200_F16 ? attention_launch<D_, B200_F16>(g_raised[D_ / 64 + 1], p, st)                                              \

@@ -1,0 +1,246 @@
+// How the attention kernels over the 4-bit cache share out their work: sequences cut into items, the items' keys dealt evenly to CTAs, whatever the
+// sequences' lengths (known on the device only).
+#pragma once
+#include "kv4.cuh"
+
+namespace b200 {
+
+constexpr int kKv4Ctas = 148;          // of a launch at most
+constexpr int kKv4Snap = 256;          // keys that a CTA may have more or fewer, so that it begins with an item (few of many: a quarter)
+constexpr int kKv4Many = 4096;
+constexpr float kKv4Top = 8.f;         // powers of two: what the largest weight that meets codes is at when a row's reference is set,
+constexpr float kKv4Lag = 4.f;         // and how far above that one may come before it is set again
+constexpr float kKv4Seed = -1.0e30f;   // a row's reference before its first key
+
+struct Kv4Params {
+  const uint8_t *pool;
+  int n_pages, kv_heads, page;
+  b200_kv4_attention_args a;
+  int G;                            // q heads of a kv head
+  int heads, tokens, subs;          // of an item: q heads, positions; items that share a position's kv head
+  int least_rows, most_rows;        // sequences of this launch: by their rows
+  int fill;                         // 1: rows of no sequence are zeroed here
+  float log2_scale;
+  bool wide_q, wide_out;            // rows are aligned to four elements
+  int *counters;                    // [kKv4Ctas], then an error word
+  float *parts;
+};
+
+__device__ __forceinline__ int clamp(long long x, int lo, int hi) { return (int)(x < lo ? lo : x > hi ? hi : x); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint32_t pair) { return __half22float2(*reinterpret_cast<const __half2 *>(&pair)); }
+template <int TYPE> __device__ __forceinline__ void put(const Kv4Params &p, int64_t at, float x) {
+  if constexpr (TYPE == B200_F32)
+    ((float *)p.a.out)[at] = x;
+  else if constexpr (TYPE == B200_F16)
+    ((__half *)p.a.out)[at] = __float2half_rn(x);
+  else
+    ((__nv_bfloat16 *)p.a.out)[at] = __float2bfloat16_rn(x);
+}
+// four elements of q, aligned
+template <int TYPE> __device__ __forceinline__ void load_wide(const void *q, int64_t at, float (&x)[4]) {
+  if constexpr (TYPE == B200_F32) {
+    *reinterpret_cast<float4 *>(x) = *reinterpret_cast<const float4 *>((const float *)q + at);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2 *>((const uint16_t *)q + at);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t w = e ? v.y : v.x;
+      const float2 f = TYPE == B200_F16 ? halves(w) : make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+      x[2 * e] = f.x;
+      x[2 * e + 1] = f.y;
+    }
+  }
+}
+
+// A sequence as its items: its rows `tokens` at a time and, for each kv head (or part of its q heads), a range of keys that ends at the last
+// row's own position.  Cost of an item: its keys; of all items before it in a head: before().
+struct Sequence {
+  int r0, n;            // rows
+  int base;             // position of the first row (negative: rows before it see nothing), at most the table's room
+  int past, tiles;      // max(base, 0); row tiles
+  __device__ __forceinline__ Sequence(int first, int end, int position, int tokens) : r0(first), n(max(end - first, 0)), base(position) {
+    past = max(base, 0);
+    tiles = n <= tokens ? min(n, 1) : (n + tokens - 1) / tokens;
+  }
+  __device__ __forceinline__ long long before(int rt, int tokens) const {
+    return rt == 0 ? 0
+           : rt < tiles ? (long long)rt * past + (long long)tokens * rt * (rt + 1) / 2
+                        : (long long)(tiles - 1) * past + (long long)tokens * tiles * (tiles - 1) / 2 + past + n;
+  }
+};
+// x * a / b, rounded down
+__device__ __forceinline__ long long share(long long x, int a, int b) {
+  return x < (1 << 24) && a <= 255 ? (long long)((uint32_t)x * a / (uint32_t)b) : x * a / b;
+}
+
+// An item and the first of its tiles that is meant.
+struct Place {
+  int s, slot, rt, tile;
+};
+
+// SHIFT: log2 of a tile's keys
+template <int SHIFT> struct KeyPlan {
+  const long long *cost;   // [n + 1], in shared memory as the others
+  const int *r0, *base;    // [n + 1], [n]: a sequence's rows, and the position of the first
+  int n, tokens, slots, ctas, window;
+  long long total;
+
+  static __host__ __device__ constexpr int bytes(int n) { return 16 * (n + 1); }
+
+  // By all THREADS of the CTA; sums: THREADS / 32 words of shared memory.
+  template <int THREADS> __device__ __forceinline__ void build(const Kv4Params &p, void *memory, long long *sums, int least_keys) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, room = p.a.table_stride * p.page;
+    n = p.a.n_seqs;
+    tokens = p.tokens;
+    slots = p.kv_heads * p.subs;
+    long long *s_cost = reinterpret_cast<long long *>(memory);
+    int *s_r0 = reinterpret_cast<int *>(s_cost + n + 1), *s_base = s_r0 + n + 1;
+    const int per = (n + THREADS - 1) / THREADS, first = min(n, tid * per), last = min(n, first + per);
+    long long sum = 0;
+    for (int s = first; s < last; ++s) {
+      const int a = clamp(p.a.row_start[s], 0, p.a.rows), b = clamp(p.a.row_start[s + 1], 0, p.a.rows), rows = max(b - a, 0);
+      const int at = clamp((long long)p.a.lens[s] - rows, -rows, room);
+      s_r0[s] = a;
+      s_base[s] = at;
+      if (s == n - 1)
+        s_r0[n] = b;
+      const Sequence q(a, b, at, tokens);
+      s_cost[s] = sum;
+      if (rows >= p.least_rows && rows <= p.most_rows)
+        sum += slots * q.before(q.tiles, tokens);
+    }
+    long long upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o)
+        upto += v;
+    }
+    if (lane == 31)
+      sums[warp] = upto;
+    __syncthreads();
+    long long before = upto - sum;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w)
+      before += w < warp ? sums[w] : 0;
+    if (before != 0)
+      for (int s = first; s < last; ++s)
+        s_cost[s] += before;
+    if (tid == THREADS - 1)
+      s_cost[n] = before + sum;
+    __syncthreads();
+    cost = s_cost;
+    r0 = s_r0;
+    base = s_base;
+    total = s_cost[n];
+    ctas = total >= (long long)gridDim.x * least_keys ? gridDim.x : max(1, (int)total / least_keys);
+    const long long chunk = share(total, 1, ctas);
+    window = chunk > kKv4Many ? kKv4Snap / 4 : (int)min((long long)kKv4Snap, chunk / 2 - 1);
+  }
+  __device__ __forceinline__ Sequence sequence(int s) const { return Sequence(r0[s], r0[s + 1], base[s], tokens); }
+  __device__ __forceinline__ int item_keys(const Sequence &q, int rt) const { return q.past + min((rt + 1) * tokens, q.n); }
+  __device__ __forceinline__ int item_tiles(const Sequence &q, int rt) const { return (item_keys(q, rt) + (1 << SHIFT) - 1) >> SHIFT; }
+  // the item with key x of all, from begin to end; at.tile: the first tile from x on (none of the item's, if x lies in its last)
+  __device__ __forceinline__ void locate(long long x, Place &at, long long &begin, long long &end) const {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (cost[mid] <= x)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    at.s = lo;
+    const Sequence q = sequence(lo);
+    begin = cost[lo];
+    const long long head = q.before(q.tiles, tokens);
+    at.slot = (x - begin) >> 32 ? (int)((x - begin) / head) : (int)((uint32_t)(x - begin) / (uint32_t)min(head, 0xffffffffll));
+    begin += at.slot * head;
+    int a = 0, b = q.tiles;
+    while (b - a > 1) {
+      const int mid = (a + b) >> 1;
+      if (q.before(mid, tokens) <= x - begin)
+        a = mid;
+      else
+        b = mid;
+    }
+    at.rt = a;
+    end = begin + q.before(a + 1, tokens);
+    begin += q.before(a, tokens);
+    at.tile = (int)((x - begin + (1 << SHIFT) - 1) >> SHIFT);
+  }
+  // where CTA c begins: at its share of all keys, or at the item border next to that
+  __device__ __forceinline__ long long border(int c) const {
+    if (c <= 0 || c >= ctas)
+      return c <= 0 ? 0 : total;
+    const long long x = share(total, c, ctas);
+    Place at;
+    long long begin, end;
+    locate(x, at, begin, end);
+    return x - begin <= end - x ? (x - begin <= window ? begin : x) : end - x <= window ? end : x;
+  }
+  __device__ __forceinline__ int nominal(long long x) const { return (int)(((x + 1) * ctas - 1) / total); }   // the CTA that x would lie in without that
+  __device__ __forceinline__ void next_item(Place &at, const Sequence &q) const {
+    at.tile = 0;
+    if (++at.rt < q.tiles)
+      return;
+    at.rt = 0;
+    if (++at.slot < slots)
+      return;
+    at.slot = 0;
+    do
+      ++at.s;
+    while (at.s < n && cost[at.s + 1] == cost[at.s]);
+  }
+  // The tiles of an item are counted as its parts arrive, in the counter of the CTA that would begin it were there no borders moved (no two items
+  // that are shared have the same).  By a whole warp, `tiles` of them having arrived and being visible: true for who completes the item, with the
+  // CTAs of its first and last part.
+  __device__ __forceinline__ bool arrive(int *counters, const Place &item, int tiles, int &from, int &to) const {
+    const int lane = threadIdx.x & 31;
+    const Sequence q = sequence(item.s);
+    const int all = item_tiles(q, item.rt);
+    const long long first = cost[item.s] + item.slot * q.before(q.tiles, tokens) + q.before(item.rt, tokens), last = first + ((long long)(all - 1) << SHIFT);
+    from = nominal(first);
+    to = nominal(last);
+    int before = 0;
+    if (lane == 0)
+      before = atomicAdd(counters + from, tiles);
+    if (__shfl_sync(0xffffffffu, before, 0) + tiles != all)
+      return false;
+    if (lane == 0)
+      counters[from] = 0;
+    const long long x = border(lane == 0 ? from + 1 : lane == 1 ? to : to + 1);   // (a lane each)
+    const bool later = __shfl_sync(0xffffffffu, (int)(x <= first), 0), sooner = __shfl_sync(0xffffffffu, (int)(x > last), 1),
+               beyond = __shfl_sync(0xffffffffu, (int)(x <= last), 2);
+    from += later;
+    to += beyond - sooner;
+    return true;
+  }
+};
+
+// element of a row in q (ld: q's) or out, before its dims: row i of the position `token` and on, of an item's heads
+__device__ __forceinline__ int64_t row_at(const Kv4Params &p, int token, int slot, int i, int64_t ld, int D) {
+  return (token + (int64_t)(i / p.heads)) * ld + (int64_t)((slot / p.subs) * p.G + slot % p.subs * p.heads + i % p.heads) * D;
+}
+// number of a tile of sixteen keys of a sequence in the pool, or -1
+__device__ __forceinline__ int tile_source(const Kv4Params &p, int s, int kv, int t) {
+  const int per_page = p.page / kKv4Tile, id = p.a.block_table[(int64_t)s * p.a.table_stride + t / per_page];
+  return id < 0 || id >= p.n_pages ? -1 : (id * p.kv_heads + kv) * per_page + t % per_page;
+}
+
+// kv4_chunk.cu: sequences of many rows, on tcgen05
+int64_t kv4_chunk_part_floats(int D);   // of a CTA's two parts
+bool kv4_chunk_takes(int dtype, int G, int n_seqs);
+int kv4_chunk_launch(Kv4Params p, int D, cudaStream_t st);
+
+} // namespace b200

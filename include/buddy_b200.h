@@ -382,6 +382,9 @@ int64_t b200_kv4_attention_workspace_bytes(int q_heads, int kv_heads,
 int b200_kv4_attention(const b200_kv4_cache *c,
                        const b200_kv4_attention_args *a, void *workspace,
                        int64_t workspace_bytes, void *stream);
+/* Waits for `stream`: B200_ECUDA when a bounded wait of a call with this workspace gave up
+ * since it was zeroed (its results are not to be used then). */
+int b200_kv4_attention_status(void *workspace, void *stream);
 
 /* ------------------------------------------------------------------------
  * Device-resident decode session.
