@@ -705,6 +705,7 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
   p.log2_scale = a->scale * 1.4426950408889634f;
   const int size = a->dtype == B200_F32 ? 4 : 2;
   p.wide_q = (((uintptr_t)a->q | (uintptr_t)(a->q_ld * size)) & (4 * size - 1)) == 0;
+  p.wide_q16 = (((uintptr_t)a->q | (uintptr_t)(a->q_ld * size)) & 15) == 0;
   p.wide_out = (((uintptr_t)a->out | (uintptr_t)(a->out_ld * size)) & (4 * size - 1)) == 0;
   p.counters = (int *)workspace;
   p.parts = (float *)((char *)workspace + 2048);
@@ -717,7 +718,7 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
   cudaStream_t st = (cudaStream_t)stream;
   // Sequences of many rows go to tcgen05, in a launch of their own; who has how many rows is known on the device only, so both launches are made where
   // the mean does not say that there are none of one kind.
-  if (kv4_chunk_takes(a->dtype, p.G, a->n_seqs) && (int64_t)a->rows * p.G >= kChunkRows && a->rows >= 2 * (int64_t)a->n_seqs) {
+  if (kv4_chunk_takes(a->dtype, p.G, a->n_seqs) && (int64_t)a->rows * p.G >= kChunkRows && (int64_t)a->rows * p.G >= 24 * (int64_t)a->n_seqs) {
     const int from = (kChunkRows + p.G - 1) / p.G;
     Kv4Params chunk = p;
     if (a->n_seqs > 1) {

@@ -1,19 +1,21 @@
 // Attention over the 4-bit KV cache for sequences of many rows (a chunk of a prompt, or all of it) on the 5th-generation tensor cores.
 //
-// Where many rows meet a key its 128 codes are better made values once: four warps turn 128 keys into f16 operands (K [128][D], V
+// Where many rows meet a key its 128 codes are better made values once: seven warps turn 128 keys into f16 operands (K [128][D], V
 // transposed [D][128], swizzled), two times 128 query rows are multiplied with them.  A tile of sixteen keys has a power of two of its own, so
 // that its largest value comes to 2^-8 .. 2^-7: code, scale and minimum then meet in one fma with one rounding (codes as the subnormal
 // numbers c 2^-24 and c 2^-20, the scale times 2^24 and 2^20).  K's power goes into the scores' factor, V's into the weights' exponent, whose reference
 // counts it too: weights fit f16 whatever the values are, and need no other normalisation.
 //
-// One thread per row does the softmax: scores come from tensor memory twice (their maximum, then the weights), the weights go back in their
-// place as the A operand of O += P V, which stays in tensor memory; it is multiplied only when a row's reference moves by more than 2^4.
+// One thread per row does the softmax in one pass: 32 scores at a time come from tensor memory, their weights go back in their place as the A operand of
+// O += P V, which stays in tensor memory.  Where a score is more than 2^4 above the row's reference, that moves (by whole powers of two), and
+// what has been summed and the block's weights so far are multiplied: rare after a row's first keys.
 // Two sets of 128 rows take turns: one's products run under the other's softmax.  (S 2 x 128 columns, O 2 x D.)
 // A key's values that are not finite are zero in the operands, and what sees them becomes NaN afterwards: nothing reaches rows that do not.
 #include "kv4_plan.cuh"
 #include "tensor_core.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace b200 {
 
@@ -21,7 +23,8 @@ namespace {
 
 constexpr int kRows = 128, kSets = 2;               // query rows of a set
 constexpr int kKeys = 128, kShift = 7;              // of a block
-constexpr int kSoftmaxWarps = 4 * kSets, kMakers = 4, kThreads = 32 * (kSoftmaxWarps + kMakers + 1);
+constexpr int kTiles = kKeys / kKv4Tile;            // of a block
+constexpr int kSoftmaxWarps = 4 * kSets, kMakers = 7, kThreads = 32 * (kSoftmaxWarps + kMakers + 1);
 constexpr int kStages = 2, kNotes = 4;
 constexpr uint32_t kCols = 512;
 constexpr int kLeastKeys = 256;
@@ -37,8 +40,10 @@ template <int D> struct Shape {
 // What the softmax has to know of a block's keys.
 struct Notes {
   float factor[8], height[8], unit[8];   // of a tile: of its scores; log2 of V's power of two, and that itself (inverted)
-  uint32_t special[4];                   // any of the words below
-  uint32_t k_bad[4], hole[4], v_bad[2][4];   // keys: K not finite; no page; V not finite, by group
+  // bits of sixteen keys, by tile: any of the next; K not finite; no page; V not finite, by group
+  __align__(16) uint16_t special[8];
+  uint16_t k_bad[8], hole[8], v_bad[2][8];
+  __device__ __forceinline__ static uint32_t word(const uint16_t *x, int c) { return reinterpret_cast<const uint32_t *>(x)[c]; }   // of keys 32 c ..
 };
 struct Bars {
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[kSets], p_ready[kSets], o_full[kSets], q_full[kSets];
@@ -75,15 +80,54 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[
                "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
                : "memory");
 }
+// (the values are there after the wait, and the compiler takes them from it)
+__device__ __forceinline__ void tmem_arrived(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
+                 "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]),
+                 "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]),
+                 "+r"(v[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// byte offset of 16-byte chunk c of row r in a tile of 128-byte rows, 128-byte swizzle
-__device__ __forceinline__ uint32_t swz(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+// (Operands in shared memory: rows of 128 bytes, 128-byte swizzle: 16-byte chunk c of row r lies at chunk c ^ (r & 7).)
+__device__ __forceinline__ void put4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {   // (an address in shared memory)
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void put1(uint32_t at, uint32_t a) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(a) : "memory"); }
 __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// two f32 at once
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ bool finite_pair(uint32_t pair) { return (pair & 0x7c00u) != 0x7c00u && (pair & 0x7c000000u) != 0x7c000000u; }
@@ -159,8 +203,8 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&bars.k_full[i], kMakers);
-      mbar_init(&bars.v_full[i], kMakers);
+      mbar_init(&bars.k_full[i], kTiles);
+      mbar_init(&bars.v_full[i], kTiles);
       mbar_init(&bars.k_empty[i], 1);
       mbar_init(&bars.v_empty[i], 1);
     }
@@ -204,7 +248,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
     // ---- softmax: a thread per row --------------------------------------------------------------------------------------------
     const int set = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), col_s = lanes + H::COL_S + set * kKeys, col_o = lanes + H::COL_O + set * D;
-    uint8_t *q_at = qs + set * H::Q_BYTES;
+    const uint32_t q_at = smem_u32(qs) + set * H::Q_BYTES + row * 128;
     bool ok = true;
     uint32_t blocks = 0, segments = 0, made = 0;   // of this set so far; of the CTA
     Walk walk(plan);
@@ -219,38 +263,36 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
       const bool live = any && token < min(mine, half);
       const int64_t q_row = live ? row_at(p, g.r0 + g.first + set * half, g.at.slot, row, p.a.q_ld, D) : 0;
       if (any) {
-        // ---- q: times a power of two, as f16
-        float x[4], most = 0.f, sum = 0.f;
-        auto load = [&](int d) {
-          if (live && p.wide_q)
-            load_wide<TYPE>(p.a.q, q_row + d, x);
-          else
+        // ---- q: times a power of two, as f16; two elements a word
+        uint32_t w[D / 2];
+        if (live && p.wide_q16) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              x[e] = live ? load_as_float(p.a.q, TYPE, q_row + d + e) : 0.f;
-        };
-#pragma unroll 4
-        for (int d = 0; d < D; d += 4) {
-          load(d);
+          for (int c = 0; c < D / 8; ++c)
+            *reinterpret_cast<uint4 *>(w + 4 * c) = __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)p.a.q + q_row) + c);
+        } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            most = fmaxf(most, fabsf(x[e]));
-            sum += x[e] * 0.f;               // (NaN where one is not finite)
-          }
+          for (int c = 0; c < D / 2; ++c)
+            w[c] = live ? ((const uint16_t *)p.a.q)[q_row + 2 * c] | (uint32_t)((const uint16_t *)p.a.q)[q_row + 2 * c + 1] << 16 : 0u;
+        }
+        auto two = [](uint32_t x) { return TYPE == B200_F16 ? halves(x) : make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); };
+        float most = 0.f, sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 2; ++c) {
+          const float2 x = two(w[c]);
+          most = max3(most, fabsf(x.x), fabsf(x.y));
+          sum = fmaf(x.x, 0.f, fmaf(x.y, 0.f, sum));   // (NaN where one is not finite)
         }
         const int up = min(max(14 + 127 - (int)(__float_as_uint(most) >> 23), -113), 100);
         const float by = p.log2_scale < 0.f ? -power(up) : power(up);
         factor = sum == 0.f ? fabsf(p.log2_scale) * power(-up) : NAN;
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          uint32_t w[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            load(8 * c + 4 * h);
-            w[2 * h] = pack_f16(x[0] * by, x[1] * by);
-            w[2 * h + 1] = pack_f16(x[2] * by, x[3] * by);
+        for (int c = 0; c < D / 8; ++c) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 x = two(w[4 * c + e]);
+            w[4 * c + e] = pack_f16(x.x * by, x.y * by);
           }
-          *reinterpret_cast<uint4 *>(q_at + (c >> 3) * (kRows * 128) + swz(row, c & 7)) = make_uint4(w[0], w[1], w[2], w[3]);
+          put4(q_at + (c >> 3) * (kRows * 128) + (((c & 7) ^ (row & 7)) << 4), w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
         }
         fence_proxy();
         fence_before();
@@ -265,84 +307,108 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
         fence_after();
         // (the makers wrote them before the products that have been waited for could begin; another block's come four blocks later)
         const Notes &notes = bars.notes[(made + j) % kNotes];
-        const bool special = (notes.special[0] | notes.special[1] | notes.special[2] | notes.special[3]) != 0;
+        const uint4 any_special = *reinterpret_cast<const uint4 *>(notes.special);
+        const bool special = (any_special.x | any_special.y | any_special.z | any_special.w) != 0;
         const bool masked = special || __any_sync(0xffffffffu, live && seen < kKeys);
         auto sees = [&](int c) {   // of keys 32 c ..: a bit each
           const int k = seen - 32 * c;
-          return (k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1) & ~notes.hole[c];
+          return (k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1) & ~Notes::word(notes.hole, c);
         };
-        float top = -INFINITY;
-        // ---- the largest of score + log2 of V's power
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[32];
-          tmem_load32(col_s + 32 * c, w);
-          tmem_wait_load();
-          if (masked) {
-            const uint32_t m = sees(c);
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              w[e] = m >> e & 1 ? w[e] : 0xff800000u;
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x = __uint_as_float(w[16 * h]);
-#pragma unroll
-            for (int e = 1; e < 16; ++e)
-              x = fmaxf(x, __uint_as_float(w[16 * h + e]));
-            top = fmaxf(top, fmaf(x, factor * notes.factor[2 * c + h], notes.height[2 * c + h]));
-          }
-        }
-        const bool moves = top > r + (kKv4Top + kKv4Lag);
-        if (__any_sync(0xffffffffu, moves)) {
-          const float to = moves ? top - kKv4Top : r, keep = ex2(r - to);   // (each row for itself)
+        // a row's reference moves, at the keys 32 c and on
+        auto move = [&](float top, int c) {
+          const bool moves = top > r + (kKv4Top + kKv4Lag);
+          const float to = moves ? ceilf(top) - kKv4Top : r, keep = ex2(r - to);   // (each row for itself)
           r = to;
           l *= keep;
-          if (j > 0) {   // (the sums so far are complete: their products came before the scores)
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t w[32];
-              tmem_load32(col_o + c, w);
-              tmem_wait_load();
+          auto times = [&](uint32_t at, bool pairs) {
+            uint32_t w[32];
+            tmem_load32(at, w);
+            tmem_arrived(w);
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < 32; ++e)
+              if (pairs) {
+                const float2 x = halves(w[e]);
+                w[e] = pack_f16(x.x * keep, x.y * keep);
+              } else {
                 w[e] = __float_as_uint(__uint_as_float(w[e]) * keep);
-              tmem_store32(col_o + c, w);
-            }
-          }
-        }
-        // ---- weights, in place of the scores
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[32], out[16];
-          tmem_load32(col_s + 32 * c, w);
-          tmem_wait_load();
-          const uint32_t m = masked ? sees(c) : 0xffffffffu, bad = masked ? notes.k_bad[c] & m : 0u;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float f = factor * notes.factor[2 * c + h], b = notes.height[2 * c + h] - r;
-            float sum[2] = {};
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              float x[2];
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const int k = 16 * h + e + u;
-                x[u] = ex2(fmaf(__uint_as_float(w[k]), f, b));
-                if (masked)
-                  x[u] = bad >> k & 1 ? NAN : m >> k & 1 ? x[u] : 0.f;
-                sum[u] += x[u];
               }
-              out[8 * h + e / 2] = pack_f16(x[0], x[1]);
-            }
-            l = fmaf(sum[0] + sum[1], notes.unit[2 * c + h], l);
+            tmem_store32(at, w);
+          };
+          if (j > 0)   // (the sums so far are complete: their products came before the scores)
+#pragma unroll 1
+            for (int i = 0; i < D; i += 32)
+              times(col_o + i, false);
+          if (c > 0) {
+            tmem_wait_store();
+            // weights of this block; where they end in the middle of 32 columns, scores that are used no more
+            times(col_s, true);
+            if (c == 3)
+              times(col_s + 32, true);
+            tmem_wait_store();
           }
-          tmem_store16(col_s + 16 * c, out);
-          if (special)
+        };
+        auto weigh = [&](auto hidden) {
+          constexpr bool HIDDEN = decltype(hidden)::value;
+          uint32_t s[2][32];
+          tmem_load32(col_s, s[0]);
 #pragma unroll
-            for (int gr = 0; gr < GROUPS; ++gr)
-              marks[gr] = marks[gr] || (notes.v_bad[gr][c] & m) != 0;
-        }
+          for (int c = 0; c < 4; ++c) {
+            uint32_t (&w)[32] = s[c & 1];
+            tmem_arrived(w);
+            if (c < 3)
+              tmem_load32(col_s + 32 * (c + 1), s[(c + 1) & 1]);
+            const uint32_t m = HIDDEN ? sees(c) : 0u, bad = HIDDEN ? Notes::word(notes.k_bad, c) & m : 0u;
+            float f[2], b[2], top = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              f[h] = factor * notes.factor[2 * c + h];
+              b[h] = notes.height[2 * c + h];
+              float x[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                const int k = 16 * h + e;
+                if constexpr (HIDDEN) {
+                  w[k] = m >> k & 1 ? w[k] : 0xff800000u;
+                  w[k + 1] = m >> (k + 1) & 1 ? w[k + 1] : 0xff800000u;
+                }
+                x[e / 2 & 1] = max3(x[e / 2 & 1], __uint_as_float(w[k]), __uint_as_float(w[k + 1]));
+              }
+              top = fmaxf(top, fmaf(fmaxf(x[0], x[1]), f[h], b[h]));
+            }
+            if (__any_sync(0xffffffffu, top > r + (kKv4Top + kKv4Lag)))
+              move(top, c);
+            uint32_t out[16];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint64_t ff = pack2(f[h], f[h]), bb = pack2(b[h] - r, b[h] - r);
+              uint64_t sum = 0;
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                const int k = 16 * h + e;
+                float2 x = unpack2(fma_2(pack2(__uint_as_float(w[k]), __uint_as_float(w[k + 1])), ff, bb));
+                x.x = ex2(x.x);
+                x.y = ex2(x.y);
+                if constexpr (HIDDEN) {
+                  x.x = bad >> k & 1 ? NAN : m >> k & 1 ? x.x : 0.f;
+                  x.y = bad >> (k + 1) & 1 ? NAN : m >> (k + 1) & 1 ? x.y : 0.f;
+                }
+                sum = add_2(sum, pack2(x.x, x.y));
+                out[8 * h + e / 2] = pack_f16(x.x, x.y);
+              }
+              const float2 both = unpack2(sum);
+              l = fmaf(both.x + both.y, notes.unit[2 * c + h], l);
+            }
+            tmem_store16(col_s + 16 * c, out);
+            if constexpr (HIDDEN)
+#pragma unroll
+              for (int gr = 0; gr < GROUPS; ++gr)
+                marks[gr] = marks[gr] || (Notes::word(notes.v_bad[gr], c) & m) != 0;
+          }
+        };
+        if (masked)
+          weigh(std::true_type());
+        else
+          weigh(std::false_type());
         tmem_wait_store();
         fence_before();
         __syncwarp();
@@ -384,7 +450,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
         for (int c = 0; c < D; c += 32) {
           uint32_t w[32];
           tmem_load32(col_o + c, w);
-          tmem_wait_load();
+          tmem_arrived(w);
           if (live) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
@@ -428,8 +494,10 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
       auto rest = [&](int b, int i) { return __ldcg(other(b) + kSets * kRows * (D + i) + at); };
       float top = kKv4Seed, total = 0.f;
       bool nan[GROUPS] = {};
+#pragma unroll 4
       for (int b = from; b <= until; ++b)
         top = fmaxf(top, rest(b, 0));
+#pragma unroll 2
       for (int b = from; b <= until; ++b) {
         total = fmaf(rest(b, 1), ex2(rest(b, 0) - top), total);
 #pragma unroll
@@ -437,12 +505,13 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
           nan[gr] = nan[gr] || rest(b, 2 + gr) != 0.f;
       }
 #pragma unroll 1
-      for (int d = 0; d < D; d += 16) {
-        float o[4][4] = {};
+      for (int d = 0; d < D; d += 32) {
+        float o[8][4] = {};
+#pragma unroll 2
         for (int b = from; b <= until; ++b) {
           const float f = ex2(rest(b, 0) - top);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 8; ++i) {
             const float4 v = __ldcg(reinterpret_cast<const float4 *>(other(b)) + (d / 4 + i) * (kSets * kRows) + at);
             o[i][0] = fmaf(v.x, f, o[i][0]);
             o[i][1] = fmaf(v.y, f, o[i][1]);
@@ -451,44 +520,36 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
           }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 8; ++i)
           write_out(d + 4 * i, o[i], total, nan);
       }
     }
   } else if (works && warp < kSoftmaxWarps + kMakers) {
-    // ---- makers: 32 keys of every block, two tiles, each ------------------------------------------------------------------------
+    // ---- makers: every seventh tile each -------------------------------------------------------------------------------------------
     const int mw = warp - kSoftmaxWarps, gq = lane >> 2, t = lane & 3;
+    const uint32_t s_k = smem_u32(ks) + gq * 128, s_v = smem_u32(vs) + gq * 128 + 4 * t;
     struct Raw {
-      uint32_t k[2][D / 32], v[D / 16], kp[2][GROUPS], vp[2][2][GROUPS];   // rows g and g + 8; words of V; pairs of keys 2 t + e + 8 u
+      uint32_t k[2][D / 32], v[D / 16];               // codes of rows g and g + 8; words of V
+      uint32_t kp[2][GROUPS], vp[2][2][GROUPS];       // pairs of rows g and g + 8; of keys 2 t + e + 8 u
     };
-    auto load_k = [&](Raw &x, int from) {
+    auto load = [&](Raw &x, int from) {
       const uint8_t *tile = p.pool + (int64_t)max(from, 0) * H::BYTES;   // (a tile that nobody sees: its pairs become zero)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int j = gq + 8 * h;
         if constexpr (D == 128) {
           *reinterpret_cast<uint4 *>(x.k[h]) = __ldg(reinterpret_cast<const uint4 *>(tile + j * 64 + t * 16));
+          *reinterpret_cast<uint4 *>(x.v + 4 * h) = __ldg(reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + h * 512 + lane * 16));
           *reinterpret_cast<uint2 *>(x.kp[h]) = __ldg(reinterpret_cast<const uint2 *>(tile + kv4_k_pairs(D) + j * 8));
+          *reinterpret_cast<uint4 *>(x.vp[h]) = __ldg(reinterpret_cast<const uint4 *>(tile + kv4_v_pairs(D) + (2 * t + 8 * h) * 8));
         } else {
           *reinterpret_cast<uint2 *>(x.k[h]) = __ldg(reinterpret_cast<const uint2 *>(tile + j * 32 + t * 8));
+          if (h == 0)
+            *reinterpret_cast<uint4 *>(x.v) = __ldg(reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + lane * 16));
           x.kp[h][0] = __ldg(reinterpret_cast<const uint32_t *>(tile + kv4_k_pairs(D) + j * 4));
+          *reinterpret_cast<uint2 *>(x.vp[h]) = __ldg(reinterpret_cast<const uint2 *>(tile + kv4_v_pairs(D) + (2 * t + 8 * h) * 4));
         }
       }
-    };
-    auto load_v = [&](Raw &x, int from) {
-      const uint8_t *tile = p.pool + (int64_t)max(from, 0) * H::BYTES;
-#pragma unroll
-      for (int gr = 0; gr < GROUPS; ++gr)
-        *reinterpret_cast<uint4 *>(x.v + 4 * gr) = __ldg(reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + gr * 512 + lane * 16));
-    };
-    auto load_pairs = [&](Raw &x, int from) {
-      const uint8_t *tile = p.pool + (int64_t)max(from, 0) * H::BYTES;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if constexpr (D == 128)
-          *reinterpret_cast<uint4 *>(x.vp[u]) = __ldg(reinterpret_cast<const uint4 *>(tile + kv4_v_pairs(D) + (2 * t + 8 * u) * 8));
-        else
-          *reinterpret_cast<uint2 *>(x.vp[u]) = __ldg(reinterpret_cast<const uint2 *>(tile + kv4_v_pairs(D) + (2 * t + 8 * u) * 4));
     };
     bool ok = true;
     uint32_t made = 0;
@@ -496,158 +557,141 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
     Segment g;
     while (walk.next(plan, g)) {
       const int most = clamp((long long)g.base + g.first + g.tokens, 0, room);   // keys that any row sees
-      const uint32_t n = g.b1 - g.b0;
-      auto source = [&](uint32_t j, int i) {   // of this warp's tile i of block b0 + j
-        const int tile = 8 * (g.b0 + (int)j) + 2 * mw + i;
-        return j >= n || tile * kKv4Tile >= most ? -1 : tile_source(p, g.at.s, g.at.slot, tile);
+      const int n = g.b1 - g.b0, tiles = kTiles * n;
+      auto source = [&](int i) {   // of this warp's i-th tile: its number in the pool, or -1
+        const int q = mw + kMakers * i, tile = kTiles * g.b0 + q;
+        return q >= tiles || tile * kKv4Tile >= most ? -1 : tile_source(p, g.at.s, g.at.slot, tile);
       };
-      int now = source(lane >> 1, lane & 1), next = source(16 + (lane >> 1), lane & 1);
-      Raw raw[2];
-      int from[2], then[2];   // numbers of the tiles in hand, and of the next block's
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        from[i] = __shfl_sync(0xffffffffu, now, i);
-        load_k(raw[i], from[i]);
-        load_v(raw[i], from[i]);
-        load_pairs(raw[i], from[i]);
-      }
-      for (uint32_t j = 0; j < n; ++j, ++made) {
-        uint32_t hole = 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if ((g.b0 + (int)j) * kKeys + 32 * mw + 16 * i < most && from[i] < 0)
-            hole |= 0xffffu << (16 * i);
-        if (((j + 1) & 15) == 0) {
+      int now = source(lane), next = source(32 + lane);
+      Raw raw, ahead;
+      int from, then = __shfl_sync(0xffffffffu, now, 0);
+      load(ahead, then);
+      for (int i = 0, q = mw; q < tiles; ++i, q += kMakers) {
+        raw = ahead;
+        from = then;
+        if (((i + 1) & 31) == 0) {
           now = next;
-          next = source(j + 17 + (lane >> 1), lane & 1);
+          next = source(i + 33 + lane);
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          then[i] = __shfl_sync(0xffffffffu, now, ((j + 1) & 15) * 2 + i);
-        const uint32_t stage = made % kStages;
-        const int key0 = (g.b0 + (int)j) * kKeys + 32 * mw;
+        then = __shfl_sync(0xffffffffu, now, (i + 1) & 31);
+        load(ahead, then);
+        const uint32_t block = made + q / kTiles, stage = block % kStages;
+        const int tile = q % kTiles, key0 = (g.b0 + q / kTiles) * kKeys + kKv4Tile * tile;
         // ---- pairs: those of keys that nobody sees, and those that are not finite, are zero
-        uint32_t k_bad = 0, v_bad[GROUPS] = {};
-        int k_lift[2], v_lift[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float largest = 0.f;
-          auto look = [&](uint32_t &pair, int key, uint32_t &bad) {   // key: of this warp's 32
-            const bool seen = from[i] >= 0 && key0 + key < most;
-            if (!seen || !finite_pair(pair)) {
-              if (seen)
-                bad |= 1u << key;
-              pair = 0u;
-            }
-            const float2 f = halves(pair);
-            largest = fmaxf(largest, fmaxf(fabsf(f.y), fabsf(fmaf(15.f, f.x, f.y))));
-          };
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int gr = 0; gr < GROUPS; ++gr)
-              look(raw[i].kp[h][gr], 16 * i + gq + 8 * h, k_bad);
-          k_lift[i] = lift(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(largest))));
-          largest = 0.f;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int gr = 0; gr < GROUPS; ++gr)
-                look(raw[i].vp[u][e][gr], 16 * i + 2 * t + e + 8 * u, v_bad[gr]);
-          v_lift[i] = lift(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(largest))));
-        }
-        Notes &notes = bars.notes[made % kNotes];
-        uint32_t bad = k_bad;
-#pragma unroll
-        for (int gr = 0; gr < GROUPS; ++gr)
-          bad |= v_bad[gr];
-        const bool any_bad = __any_sync(0xffffffffu, bad != 0);
-        if (any_bad) {   // (rare)
-          k_bad = __reduce_or_sync(0xffffffffu, k_bad);
+        uint32_t k_bad = 0, v_bad[GROUPS] = {}, strange = 0;
+        auto every = [&](auto f) {   // f(pair, key of the tile, mask of what is bad)
 #pragma unroll
           for (int gr = 0; gr < GROUPS; ++gr)
-            v_bad[gr] = __reduce_or_sync(0xffffffffu, v_bad[gr]);
-        }
-        // ---- K: words of eight dims of a key
-        if (made >= kStages)
-          wait(ok, &bars.k_empty[stage], (made / kStages - 1) & 1, 733);
-        if (lane < 2) {   // (after the wait: the block four before is done with)
-          notes.factor[2 * mw + lane] = power(-(lane ? k_lift[1] : k_lift[0]));
-          notes.height[2 * mw + lane] = (float)-(lane ? v_lift[1] : v_lift[0]);
-          notes.unit[2 * mw + lane] = power(lane ? v_lift[1] : v_lift[0]);
-        }
-        if (lane == 0) {
-          notes.k_bad[mw] = k_bad;
-          notes.hole[mw] = hole;
-#pragma unroll
-          for (int gr = 0; gr < GROUPS; ++gr)
-            notes.v_bad[gr][mw] = v_bad[gr];
-          notes.special[mw] = (any_bad ? 1u : 0u) | hole;
-        }
-        uint8_t *k_at = ks + stage * H::KV_BYTES, *v_at = vs + stage * H::KV_BYTES;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float one = power(k_lift[i]);
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int w = 0; w < D / 32; ++w) {
-              const float2 f = halves(raw[i].kp[h][w / 2]);
-              const float s = f.x * one, l = f.y * one;
-              const uint32_t low = pack_f16(s * 16777216.f, s * 16777216.f), high = pack_f16(s * 1048576.f, s * 1048576.f), lo = pack_f16(l, l);
-              const uint32_t x = raw[i].k[h][w], y = x >> 8;
-              *reinterpret_cast<uint4 *>(k_at + w / 2 * (kKeys * 128) + swz(32 * mw + 16 * i + gq + 8 * h, 4 * (w & 1) + t)) =
-                  make_uint4(fma2(x & 0x000f000fu, low, lo), fma2(x & 0x00f000f0u, high, lo), fma2(y & 0x000f000fu, low, lo), fma2(y & 0x00f000f0u, high, lo));
-            }
-        }
-        fence_proxy();
-        __syncwarp();
-        if (lane == 0)
-          mbar_arrive(&bars.k_full[stage]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          load_k(raw[i], then[i]);
-        // ---- V: words of dims 16 w + g (+ 8) and keys 2 t, 2 t + 1 (+ 8)
-        if (made >= kStages)
-          wait(ok, &bars.v_empty[stage], (made / kStages - 1) & 1, 734);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float unit = power(v_lift[i]);
-#pragma unroll
-          for (int gr = 0; gr < GROUPS; ++gr) {
-            uint32_t low[2], high[2], lo[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              const float2 a = halves(raw[i].vp[u][0][gr]), b = halves(raw[i].vp[u][1][gr]);
-              low[u] = pack_f16(a.x * unit * 16777216.f, b.x * unit * 16777216.f);
-              high[u] = pack_f16(a.x * unit * 1048576.f, b.x * unit * 1048576.f);
-              lo[u] = pack_f16(a.y * unit, b.y * unit);
-            }
+              f(raw.kp[u][gr], gq + 8 * u, k_bad);
 #pragma unroll
-            for (int w = 4 * gr; w < 4 * gr + 4; ++w) {
-              const uint32_t x = raw[i].v[w], y = x >> 8;
-              uint8_t *to = v_at + mw / 2 * (D * 128) + 4 * t;
-              const int c = mw % 2 * 4 + 2 * i, d = 16 * w + gq;
-              *reinterpret_cast<uint32_t *>(to + swz(d, c)) = fma2(x & 0x000f000fu, low[0], lo[0]);
-              *reinterpret_cast<uint32_t *>(to + swz(d + 8, c)) = fma2(x & 0x00f000f0u, high[0], lo[0]);
-              *reinterpret_cast<uint32_t *>(to + swz(d, c + 1)) = fma2(y & 0x000f000fu, low[1], lo[1]);
-              *reinterpret_cast<uint32_t *>(to + swz(d + 8, c + 1)) = fma2(y & 0x00f000f0u, high[1], lo[1]);
+              for (int e = 0; e < 2; ++e)
+                f(raw.vp[u][e][gr], 2 * t + e + 8 * u, v_bad[gr]);
             }
+        };
+        every([&](uint32_t &pair, int, uint32_t &) {   // (x - x is zero, but for infinities and NaN)
+          const __half2 x = *reinterpret_cast<const __half2 *>(&pair), d = __hsub2(x, x);
+          strange |= *reinterpret_cast<const uint32_t *>(&d);
+        });
+        bool any_bad = false;
+        if (from < 0 || key0 + kKv4Tile > most || __any_sync(0xffffffffu, strange != 0)) {
+          every([&](uint32_t &pair, int key, uint32_t &bad) {
+            const bool seen = from >= 0 && key0 + key < most;
+            if (!seen || !finite_pair(pair)) {
+              bad |= seen ? 1u << key : 0u;
+              pair = 0u;
+            }
+          });
+          k_bad = __reduce_or_sync(0xffffffffu, k_bad);
+          uint32_t all = k_bad;
+#pragma unroll
+          for (int gr = 0; gr < GROUPS; ++gr) {
+            v_bad[gr] = __reduce_or_sync(0xffffffffu, v_bad[gr]);
+            all |= v_bad[gr];
+          }
+          any_bad = all != 0;
+        }
+        float k_most = 0.f, v_most = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float2 f = halves(raw.kp[u][gr]);
+            k_most = max3(k_most, fabsf(f.y), fabsf(fmaf(15.f, f.x, f.y)));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 v = halves(raw.vp[u][e][gr]);
+              v_most = max3(v_most, fabsf(v.y), fabsf(fmaf(15.f, v.x, v.y)));
+            }
+          }
+        const int k_lift = lift(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(k_most))));
+        const int v_lift = lift(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v_most))));
+        // ---- K: words of eight dims of a key
+        if (block >= kStages)
+          wait(ok, &bars.k_empty[stage], (block / kStages - 1) & 1, 733);
+        if (lane == 0) {   // (after the wait: the block four before is done with)
+          Notes &notes = bars.notes[block % kNotes];
+          const uint32_t hole = from < 0 && key0 < most ? 0xffffu : 0u;
+          notes.factor[tile] = power(-k_lift);
+          notes.height[tile] = (float)-v_lift;
+          notes.unit[tile] = power(v_lift);
+          notes.k_bad[tile] = (uint16_t)k_bad;
+          notes.hole[tile] = (uint16_t)hole;
+#pragma unroll
+          for (int gr = 0; gr < GROUPS; ++gr)
+            notes.v_bad[gr][tile] = (uint16_t)v_bad[gr];
+          notes.special[tile] = (uint16_t)(any_bad ? 1u : hole);
+        }
+        // (rows of K and of V^T that a lane writes are g, modulo eight)
+        const uint32_t k_at = s_k + stage * H::KV_BYTES + tile * (kKv4Tile * 128), v_at = s_v + stage * H::KV_BYTES + tile / 4 * (D * 128);
+        const float one = power(k_lift), unit = power(v_lift);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int gr = 0; gr < GROUPS; ++gr) {
+            const float2 f = halves(raw.kp[h][gr]);
+            const float s = f.x * one, l = f.y * one;
+            const uint32_t low = pack_f16(s * 16777216.f, s * 16777216.f), high = pack_f16(s * 1048576.f, s * 1048576.f), lo = pack_f16(l, l);
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t x = raw.k[h][2 * gr + w], y = x >> 8;
+              put4(k_at + gr * (kKeys * 128) + h * 1024 + (((4 * w + t) ^ gq) << 4), fma2(x & 0x000f000fu, low, lo), fma2(x & 0x00f000f0u, high, lo),
+                   fma2(y & 0x000f000fu, low, lo), fma2(y & 0x00f000f0u, high, lo));
+            }
+          }
+        // ---- V: words of dims 16 w + g (+ 8) and keys 2 t, 2 t + 1 (+ 8)
+        if (block >= kStages)
+          wait(ok, &bars.v_empty[stage], (block / kStages - 1) & 1, 734);
+        const int c = tile % 4 * 2;
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) {
+          uint32_t low[2], high[2], lo[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float2 a = halves(raw.vp[u][0][gr]), b = halves(raw.vp[u][1][gr]);
+            low[u] = pack_f16(a.x * unit * 16777216.f, b.x * unit * 16777216.f);
+            high[u] = pack_f16(a.x * unit * 1048576.f, b.x * unit * 1048576.f);
+            lo[u] = pack_f16(a.y * unit, b.y * unit);
+          }
+#pragma unroll
+          for (int w = 4 * gr; w < 4 * gr + 4; ++w) {
+            const uint32_t x = raw.v[w], y = x >> 8;
+            const uint32_t to0 = v_at + w * 2048 + ((c ^ gq) << 4), to1 = v_at + w * 2048 + (((c + 1) ^ gq) << 4);
+            put1(to0, fma2(x & 0x000f000fu, low[0], lo[0]));
+            put1(to0 + 1024, fma2(x & 0x00f000f0u, high[0], lo[0]));
+            put1(to1, fma2(y & 0x000f000fu, low[1], lo[1]));
+            put1(to1 + 1024, fma2(y & 0x00f000f0u, high[1], lo[1]));
           }
         }
         fence_proxy();
         __syncwarp();
-        if (lane == 0)
+        if (lane == 0) {
+          mbar_arrive(&bars.k_full[stage]);
           mbar_arrive(&bars.v_full[stage]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          from[i] = then[i];
-          load_v(raw[i], from[i]);
-          load_pairs(raw[i], from[i]);
         }
       }
+      made += n;
     }
   } else if (works) {
     // ---- tensor core issue --------------------------------------------------------------------------------------------------------

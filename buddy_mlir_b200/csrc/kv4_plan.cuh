@@ -21,7 +21,7 @@ struct Kv4Params {
   int least_rows, most_rows;        // sequences of this launch: by their rows
   int fill;                         // 1: rows of no sequence are zeroed here
   float log2_scale;
-  bool wide_q, wide_out;            // rows are aligned to four elements
+  bool wide_q, wide_out, wide_q16;  // rows are aligned to four elements; to 16 bytes
   int *counters;                    // [kKv4Ctas], then an error word
   float *parts;
 };
