@@ -370,7 +370,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
   static_assert(RING >= PART * 4, "a part of a warp lies in its ring");
   extern __shared__ __align__(128) uint8_t s_all[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.a.n_seqs, room = p.a.table_stride * p.page;
-  __shared__ long long s_sum[kWarps];
+  __shared__ long long s_sum[2 * kWarps + 1];
   __shared__ Left s_left[kWarps];
   __shared__ int s_ctas[2][3];     // of a shared item that this CTA adds up: whether it does, the CTAs with its first and last part
   kernel_go();
@@ -380,7 +380,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
     s_left[warp].has_a = s_left[warp].has_b = false;
   if (tid < 2)
     s_ctas[tid][0] = 0;
-  KeyPlan<4> plan;
+  KeyPlan<4, 1000> plan;
   plan.build<kThreads>(p, s_all + kWarps * RING, s_sum, kLeastKeys);
   // rows of no sequence
   if (p.fill) {
@@ -638,9 +638,9 @@ RaisedOn g_raised[6];
 
 template <int D, int TYPE> int attention_launch(RaisedOn &raised, const Kv4Params &p, cudaStream_t st) {
   const int fixed = kWarps * kSlots * kv4_tile_bytes(D);
-  if (int rc = raise_shared_limit(raised, (const void *)kv4_attention_kernel<D, TYPE>, fixed + KeyPlan<4>::bytes(B200_KV4_ATTENTION_MAX_SEQS)))
+  if (int rc = raise_shared_limit(raised, (const void *)kv4_attention_kernel<D, TYPE>, fixed + KeyPlan<4, 1000>::bytes(B200_KV4_ATTENTION_MAX_SEQS)))
     return rc;
-  return launch_after(kv4_attention_kernel<D, TYPE>, dim3(kKv4Ctas), kThreads, fixed + KeyPlan<4>::bytes(p.a.n_seqs), st, p);
+  return launch_after(kv4_attention_kernel<D, TYPE>, dim3(kKv4Ctas), kThreads, fixed + KeyPlan<4, 1000>::bytes(p.a.n_seqs), st, p);
 }
 
 } // namespace

@@ -49,7 +49,7 @@ struct Bars {
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[kSets], p_ready[kSets], o_full[kSets], q_full[kSets];
   uint32_t tmem_base;
   int abort_flag, last, from, to;
-  long long sums[kThreads / 32];
+  long long sums[2 * (kThreads / 32) + 1];
   Notes notes[kNotes];
 };
 
@@ -147,7 +147,7 @@ struct Segment {
 struct Walk {
   Place at, stop;
   bool over;
-  __device__ __forceinline__ Walk(const KeyPlan<kShift> &plan) {
+  __device__ __forceinline__ Walk(const KeyPlan<kShift, 1200> &plan) {
     const int lane = threadIdx.x & 31;
     const long long x = plan.border(blockIdx.x + min(lane, 1));
     over = __shfl_sync(0xffffffffu, x, 0) == __shfl_sync(0xffffffffu, x, 1);
@@ -165,7 +165,7 @@ struct Walk {
     at.rt = __shfl_sync(0xffffffffu, at.rt, 0);
     at.tile = __shfl_sync(0xffffffffu, at.tile, 0);
   }
-  __device__ __forceinline__ bool next(const KeyPlan<kShift> &plan, Segment &g) {
+  __device__ __forceinline__ bool next(const KeyPlan<kShift, 1200> &plan, Segment &g) {
     while (!over && at.s < plan.n) {
       const Sequence q = plan.sequence(at.s);
       g.all = plan.item_tiles(q, at.rt);
@@ -228,7 +228,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
   kernel_go();   // not before the allocation: see tensor_core.cuh
   kernel_wait();
   const int room = p.a.table_stride * p.page;
-  KeyPlan<kShift> plan;
+  KeyPlan<kShift, 1200> plan;
   plan.build<kThreads>(p, s_plan, bars.sums, kLeastKeys);
   if (p.fill) {
     const int lo = plan.r0[0], hi = max(lo, plan.r0[plan.n]), none = lo + p.a.rows - hi, cols = p.a.q_heads * D;
@@ -774,12 +774,12 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
 }
 
 RaisedOn g_raised[4];
-constexpr int kMostSeqs = 1900;   // whose plan fits beside the operands
+constexpr int kMostSeqs = 1500;   // whose plan fits beside the operands
 
 template <int D, int TYPE> int chunk_launch(RaisedOn &raised, const Kv4Params &p, cudaStream_t st) {
-  if (int rc = raise_shared_limit(raised, (const void *)kv4_chunk_kernel<D, TYPE>, Shape<D>::SMEM + KeyPlan<kShift>::bytes(kMostSeqs)))
+  if (int rc = raise_shared_limit(raised, (const void *)kv4_chunk_kernel<D, TYPE>, Shape<D>::SMEM + KeyPlan<kShift, 1200>::bytes(kMostSeqs)))
     return rc;
-  return launch_after(kv4_chunk_kernel<D, TYPE>, dim3(kKv4Ctas), kThreads, Shape<D>::SMEM + KeyPlan<kShift>::bytes(p.a.n_seqs), st, p);
+  return launch_after(kv4_chunk_kernel<D, TYPE>, dim3(kKv4Ctas), kThreads, Shape<D>::SMEM + KeyPlan<kShift, 1200>::bytes(p.a.n_seqs), st, p);
 }
 
 } // namespace

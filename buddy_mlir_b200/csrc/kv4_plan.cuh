@@ -88,25 +88,31 @@ struct Place {
   int s, slot, rt, tile;
 };
 
-// SHIFT: log2 of a tile's keys
-template <int SHIFT> struct KeyPlan {
+// SHIFT: log2 of a tile's keys.  An item that CTAs share costs them what some SPLIT keys do (its parts' way through L2): where whole items leave
+// nobody with that much more than an even share, CTAs have whole items.
+template <int SHIFT, int SPLIT> struct KeyPlan {
   const long long *cost;   // [n + 1], in shared memory as the others
   const int *r0, *base;    // [n + 1], [n]: a sequence's rows, and the position of the first
+  const int *items;        // [n + 1]: items before it
   int n, tokens, slots, ctas, window;
+  bool whole;
   long long total;
 
-  static __host__ __device__ constexpr int bytes(int n) { return 16 * (n + 1); }
+  static __host__ __device__ constexpr int bytes(int n) { return 20 * (n + 1); }
 
-  // By all THREADS of the CTA; sums: THREADS / 32 words of shared memory.
+  // By all THREADS of the CTA; sums: 2 * THREADS / 32 + 1 words of shared memory.
   template <int THREADS> __device__ __forceinline__ void build(const Kv4Params &p, void *memory, long long *sums, int least_keys) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, room = p.a.table_stride * p.page;
     n = p.a.n_seqs;
     tokens = p.tokens;
     slots = p.kv_heads * p.subs;
     long long *s_cost = reinterpret_cast<long long *>(memory);
-    int *s_r0 = reinterpret_cast<int *>(s_cost + n + 1), *s_base = s_r0 + n + 1;
+    int *s_r0 = reinterpret_cast<int *>(s_cost + n + 1), *s_base = s_r0 + n + 1, *s_items = s_base + n, *longest = reinterpret_cast<int *>(sums + 2 * (THREADS / 32));
+    if (tid == 0)
+      *longest = 0;
     const int per = (n + THREADS - 1) / THREADS, first = min(n, tid * per), last = min(n, first + per);
-    long long sum = 0;
+    long long sum = 0, count = 0;
+    int most = 0;
     for (int s = first; s < last; ++s) {
       const int a = clamp(p.a.row_start[s], 0, p.a.rows), b = clamp(p.a.row_start[s + 1], 0, p.a.rows), rows = max(b - a, 0);
       const int at = clamp((long long)p.a.lens[s] - rows, -rows, room);
@@ -116,36 +122,57 @@ template <int SHIFT> struct KeyPlan {
         s_r0[n] = b;
       const Sequence q(a, b, at, tokens);
       s_cost[s] = sum;
-      if (rows >= p.least_rows && rows <= p.most_rows)
+      s_items[s] = (int)count;
+      if (rows >= p.least_rows && rows <= p.most_rows) {
         sum += slots * q.before(q.tiles, tokens);
+        count += (long long)slots * q.tiles;
+        most = max(most, q.past + rows);
+      }
     }
-    long long upto = sum;
+    long long upto = sum, upto_items = count;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o)
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o), i = __shfl_up_sync(0xffffffffu, upto_items, o);
+      if (lane >= o) {
         upto += v;
+        upto_items += i;
+      }
     }
-    if (lane == 31)
+    if (lane == 31) {
       sums[warp] = upto;
+      sums[THREADS / 32 + warp] = upto_items;
+    }
     __syncthreads();
-    long long before = upto - sum;
+    if (most > 0)
+      atomicMax(longest, most);
+    long long before = upto - sum, before_items = upto_items - count;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w)
+    for (int w = 0; w < THREADS / 32; ++w) {
       before += w < warp ? sums[w] : 0;
+      before_items += w < warp ? sums[THREADS / 32 + w] : 0;
+    }
     if (before != 0)
-      for (int s = first; s < last; ++s)
+      for (int s = first; s < last; ++s) {
         s_cost[s] += before;
-    if (tid == THREADS - 1)
+        s_items[s] += (int)before_items;
+      }
+    if (tid == THREADS - 1) {
       s_cost[n] = before + sum;
+      s_items[n] = (int)min(before_items + count, 0x7fffffffll);
+    }
     __syncthreads();
     cost = s_cost;
     r0 = s_r0;
     base = s_base;
+    items = s_items;
     total = s_cost[n];
     ctas = total >= (long long)gridDim.x * least_keys ? gridDim.x : max(1, (int)total / least_keys);
     const long long chunk = share(total, 1, ctas);
     window = chunk > kKv4Many ? kKv4Snap / 4 : (int)min((long long)kKv4Snap, chunk / 2 - 1);
+    const int all = s_items[n], each = (all + (int)gridDim.x - 1) / (int)gridDim.x;
+    whole = all < 0x7fffffff && (long long)each * *longest <= chunk + SPLIT;
+    if (whole)
+      ctas = max(1, min((int)gridDim.x, all));
   }
   __device__ __forceinline__ Sequence sequence(int s) const { return Sequence(r0[s], r0[s + 1], base[s], tokens); }
   __device__ __forceinline__ int item_keys(const Sequence &q, int rt) const { return q.past + min((rt + 1) * tokens, q.n); }
@@ -183,6 +210,20 @@ template <int SHIFT> struct KeyPlan {
   __device__ __forceinline__ long long border(int c) const {
     if (c <= 0 || c >= ctas)
       return c <= 0 ? 0 : total;
+    if (whole) {
+      const int i = (int)share(items[n], c, ctas);
+      int lo = 0, hi = n;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (items[mid] <= i)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      const Sequence q = sequence(lo);
+      const int slot = (i - items[lo]) / q.tiles;
+      return cost[lo] + slot * q.before(q.tiles, tokens) + q.before(i - items[lo] - slot * q.tiles, tokens);
+    }
     const long long x = share(total, c, ctas);
     Place at;
     long long begin, end;
