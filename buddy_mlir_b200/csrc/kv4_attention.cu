@@ -419,14 +419,14 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
     while (at.s < n) {
       const Sequence q = plan.sequence(at.s);
       const int all = plan.item_tiles(q, at.rt);
-      if (at.tile >= all) {   // (a border behind an item's last tile)
+      const bool here = stop.s == at.s && stop.slot == at.slot && stop.rt == at.rt;
+      const int t0 = at.tile, t1 = here ? min(stop.tile, all) : all;
+      if (here && t0 >= t1)
+        break;
+      if (t0 >= all) {   // (a border behind an item's last tile)
         plan.next_item(at, q);
         continue;
       }
-      const bool here = stop.s == at.s && stop.slot == at.slot && stop.rt == at.rt;
-      const int t0 = at.tile, t1 = here ? min(stop.tile, all) : all;
-      if (t0 >= t1)
-        break;
       // ---- this warp's tiles of the item ----------------------------------------------------------------------------------------
       const int live = rows_of(p, q, at.rt, at.slot), first_token = at.rt * p.tokens, tokens = min(p.tokens, q.n - first_token);
       const int least = clamp((long long)q.base + first_token + 1, 0, room), most = clamp((long long)q.base + first_token + tokens, 0, room);
@@ -573,27 +573,33 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
     put<TYPE>(p, to + 2, l == 0.f ? 0.f : o.z * over);
     put<TYPE>(p, to + 3, l == 0.f ? 0.f : o.w * over);
   };
+  // chains side by side, a power of two of them, a warp each at least
   constexpr int FOURS = kRows * D / 4;
-  const int row = tid % FOURS / (D / 4), d = tid % (D / 4) * 4;
-  for (int k = tid / FOURS; k < chains; k += kThreads / FOURS) {
+  const int lanes = max(32, kThreads >> (32 - __clz(chains - 1)));
+  for (int i = tid; i < chains * lanes; i += kThreads) {
+    const int k = i / lanes;
     const Chain c = chain(k);
     auto part = [&](int w) { return c.opened && w == c.first ? reinterpret_cast<const float *>(s_all + w * RING) : s_left[w].a_part; };
-    float top = kKv4Seed, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = c.first; w <= c.last; ++w)
-      top = fmaxf(top, part(w)[kRows * (D + 4) + row]);
-    for (int w = c.first; w <= c.last; ++w) {
-      const float *x = part(w);
-      add(o, l, *reinterpret_cast<const float4 *>(x + row * (D + 4) + d), x[kRows * (D + 4) + kRows + row], ex2(x[kRows * (D + 4) + row] - top));
-    }
-    if (c.whole) {
-      write_out(s_left[c.first].b, row, d, o, l);
-    } else {
-      float *to = p.parts + ((int64_t)blockIdx.x * 2 + c.opened) * PART;
-      *reinterpret_cast<float4 *>(to + row * (D + 4) + d) = o;
-      if (d == 0) {
-        to[kRows * (D + 4) + row] = top;
-        to[kRows * (D + 4) + kRows + row] = l;
+#pragma unroll 2
+    for (int e = i % lanes; e < FOURS; e += lanes) {
+      const int row = e / (D / 4), d = e % (D / 4) * 4;
+      float top = kKv4Seed, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = c.first; w <= c.last; ++w)
+        top = fmaxf(top, part(w)[kRows * (D + 4) + row]);
+      for (int w = c.first; w <= c.last; ++w) {
+        const float *x = part(w);
+        add(o, l, *reinterpret_cast<const float4 *>(x + row * (D + 4) + d), x[kRows * (D + 4) + kRows + row], ex2(x[kRows * (D + 4) + row] - top));
+      }
+      if (c.whole) {
+        write_out(s_left[c.first].b, row, d, o, l);
+      } else {
+        float *to = p.parts + ((int64_t)blockIdx.x * 2 + c.opened) * PART;
+        *reinterpret_cast<float4 *>(to + row * (D + 4) + d) = o;
+        if (d == 0) {
+          to[kRows * (D + 4) + row] = top;
+          to[kRows * (D + 4) + kRows + row] = l;
+        }
       }
     }
   }
@@ -614,6 +620,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
     }
   }
   __syncthreads();
+  const int row = tid % FOURS / (D / 4), d = tid % (D / 4) * 4;
   for (int k = tid / FOURS; k < 2; k += kThreads / FOURS) {
     if (s_ctas[k][0] == 0)
       continue;

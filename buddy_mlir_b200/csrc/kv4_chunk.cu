@@ -169,11 +169,11 @@ struct Walk {
     while (!over && at.s < plan.n) {
       const Sequence q = plan.sequence(at.s);
       g.all = plan.item_tiles(q, at.rt);
-      if (at.tile >= g.all) {
+      const bool here = stop.s == at.s && stop.slot == at.slot && stop.rt == at.rt;
+      if (at.tile >= g.all && !here) {
         plan.next_item(at, q);
         continue;
       }
-      const bool here = stop.s == at.s && stop.slot == at.slot && stop.rt == at.rt;
       g.at = at;
       g.b0 = at.tile;
       g.b1 = here ? min(stop.tile, g.all) : g.all;

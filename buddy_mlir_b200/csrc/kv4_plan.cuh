@@ -8,6 +8,7 @@ namespace b200 {
 constexpr int kKv4Ctas = 148;          // of a launch at most
 constexpr int kKv4Snap = 256;          // keys that a CTA may have more or fewer, so that it begins with an item (few of many: a quarter)
 constexpr int kKv4Many = 4096;
+constexpr int kKv4Item = 48;           // keys that take as long as beginning and ending an item
 constexpr float kKv4Top = 8.f;         // powers of two: what the largest weight that meets codes is at when a row's reference is set,
 constexpr float kKv4Lag = 4.f;         // and how far above that one may come before it is set again
 constexpr float kKv4Seed = -1.0e30f;   // a row's reference before its first key
@@ -63,7 +64,7 @@ template <int TYPE> __device__ __forceinline__ void load_wide(const void *q, int
 }
 
 // A sequence as its items: its rows `tokens` at a time and, for each kv head (or part of its q heads), a range of keys that ends at the last
-// row's own position.  Cost of an item: its keys; of all items before it in a head: before().
+// row's own position.  Cost of an item: its keys, and some more for its beginning and end; of all items before it in a head: before().
 struct Sequence {
   int r0, n;            // rows
   int base;             // position of the first row (negative: rows before it see nothing), at most the table's room
@@ -74,8 +75,8 @@ struct Sequence {
   }
   __device__ __forceinline__ long long before(int rt, int tokens) const {
     return rt == 0 ? 0
-           : rt < tiles ? (long long)rt * past + (long long)tokens * rt * (rt + 1) / 2
-                        : (long long)(tiles - 1) * past + (long long)tokens * tiles * (tiles - 1) / 2 + past + n;
+           : rt < tiles ? (long long)rt * (past + kKv4Item) + (long long)tokens * rt * (rt + 1) / 2
+                        : (long long)tiles * (past + kKv4Item) + (long long)tokens * tiles * (tiles - 1) / 2 + n;
   }
 };
 // x * a / b, rounded down
@@ -126,7 +127,7 @@ template <int SHIFT, int SPLIT> struct KeyPlan {
       if (rows >= p.least_rows && rows <= p.most_rows) {
         sum += slots * q.before(q.tiles, tokens);
         count += (long long)slots * q.tiles;
-        most = max(most, q.past + rows);
+        most = max(most, q.past + rows + kKv4Item);
       }
     }
     long long upto = sum, upto_items = count;
@@ -177,7 +178,7 @@ template <int SHIFT, int SPLIT> struct KeyPlan {
   __device__ __forceinline__ Sequence sequence(int s) const { return Sequence(r0[s], r0[s + 1], base[s], tokens); }
   __device__ __forceinline__ int item_keys(const Sequence &q, int rt) const { return q.past + min((rt + 1) * tokens, q.n); }
   __device__ __forceinline__ int item_tiles(const Sequence &q, int rt) const { return (item_keys(q, rt) + (1 << SHIFT) - 1) >> SHIFT; }
-  // the item with key x of all, from begin to end; at.tile: the first tile from x on (none of the item's, if x lies in its last)
+  // the item with key x of all, from begin to end; at.tile: the first tile from x on (none of the item's, if x lies in its last or behind it)
   __device__ __forceinline__ void locate(long long x, Place &at, long long &begin, long long &end) const {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
