@@ -399,11 +399,9 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
   const long long cta_begin = __shfl_sync(0xffffffffu, x, 0), mine = __shfl_sync(0xffffffffu, x, 1) - cta_begin;
   const int act = (int)max(1ll, min((long long)kWarps, mine >> 4));   // the warps that work: sixteen keys each at least (then each begins a tile)
   Place at{n, 0, 0, 0}, stop;
-  x = cta_begin + share(mine, warp + min(lane, 1), act);
-  if (x < total) {
-    long long begin, end;
-    plan.locate(x, at, begin, end);
-  }
+  x = cta_begin + plan.part_of(mine, warp + min(lane, 1), act);
+  if (x < total && warp < act)
+    at = plan.locate(x);
   stop.s = __shfl_sync(0xffffffffu, at.s, 1);
   stop.slot = __shfl_sync(0xffffffffu, at.slot, 1);
   stop.rt = __shfl_sync(0xffffffffu, at.rt, 1);
@@ -483,7 +481,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int row = 2 * (lane & 3) + e;
-            limit[e] = row < live ? clamp((long long)q.base + first_token + row / p.heads + 1, 0, room) : 0;
+            limit[e] = row < live ? clamp((long long)q.base + first_token + (row * p.over_heads >> 16) + 1, 0, room) : 0;
           }
           tile.template keys<true>(bytes, j0, limit);
         }
@@ -566,12 +564,8 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
     const Sequence q = plan.sequence(at.s);
     if (row >= rows_of(p, q, at.rt, at.slot))
       return;
-    const int64_t to = row_at(p, q.r0 + at.rt * p.tokens, at.slot, row, p.a.out_ld, D) + d;
     const float over = l == 0.f ? 0.f : 1.f / l;
-    put<TYPE>(p, to, l == 0.f ? 0.f : o.x * over);
-    put<TYPE>(p, to + 1, l == 0.f ? 0.f : o.y * over);
-    put<TYPE>(p, to + 2, l == 0.f ? 0.f : o.z * over);
-    put<TYPE>(p, to + 3, l == 0.f ? 0.f : o.w * over);
+    put4<TYPE>(p, row_at(p, q.r0 + at.rt * p.tokens, at.slot, row, p.a.out_ld, D) + d, l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * over, o.y * over, o.z * over, o.w * over));
   };
   // chains side by side, a power of two of them, a warp each at least
   constexpr int FOURS = kRows * D / 4;
@@ -722,6 +716,7 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
   p.subs = (p.G + kRows - 1) / kRows;
   p.heads = std::min(p.G, kRows);
   p.tokens = p.subs == 1 ? kRows / p.G : 1;
+  p.over_heads = (65536 + p.heads - 1) / p.heads;
   cudaStream_t st = (cudaStream_t)stream;
   // Sequences of many rows go to tcgen05, in a launch of their own; who has how many rows is known on the device only, so both launches are made where
   // the mean does not say that there are none of one kind.

@@ -95,10 +95,10 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // (Operands in shared memory: rows of 128 bytes, 128-byte swizzle: 16-byte chunk c of row r lies at chunk c ^ (r & 7).)
-__device__ __forceinline__ void put4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {   // (an address in shared memory)
+__device__ __forceinline__ void store4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {   // (an address in shared memory)
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ void put1(uint32_t at, uint32_t a) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(a) : "memory"); }
+__device__ __forceinline__ void store1(uint32_t at, uint32_t a) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(a) : "memory"); }
 __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
@@ -152,10 +152,8 @@ struct Walk {
     const long long x = plan.border(blockIdx.x + min(lane, 1));
     over = __shfl_sync(0xffffffffu, x, 0) == __shfl_sync(0xffffffffu, x, 1);
     at = Place{plan.n, 0, 0, 0};
-    if (x < plan.total) {
-      long long begin, end;
-      plan.locate(x, at, begin, end);
-    }
+    if (x < plan.total)
+      at = plan.locate(x);
     stop.s = __shfl_sync(0xffffffffu, at.s, 1);
     stop.slot = __shfl_sync(0xffffffffu, at.slot, 1);
     stop.rt = __shfl_sync(0xffffffffu, at.rt, 1);
@@ -292,7 +290,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
             const float2 x = two(w[4 * c + e]);
             w[4 * c + e] = pack_f16(x.x * by, x.y * by);
           }
-          put4(q_at + (c >> 3) * (kRows * 128) + (((c & 7) ^ (row & 7)) << 4), w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+          store4(q_at + (c >> 3) * (kRows * 128) + (((c & 7) ^ (row & 7)) << 4), w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
         }
         fence_proxy();
         fence_before();
@@ -427,20 +425,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           x[e] = nan[d / kKv4Group] ? NAN : total == 0.f ? 0.f : o[e] * over;
-        if (p.wide_out) {
-          if constexpr (TYPE == B200_F16)
-            *reinterpret_cast<uint2 *>((__half *)p.a.out + to + d) = make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]));
-          else {
-            uint32_t lo, hi;
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(x[1]), "f"(x[0]));
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(x[3]), "f"(x[2]));
-            *reinterpret_cast<uint2 *>((__nv_bfloat16 *)p.a.out + to + d) = make_uint2(lo, hi);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            put<TYPE>(p, to + d + e, x[e]);
-        }
+        put4<TYPE>(p, to + d, make_float4(x[0], x[1], x[2], x[3]));
       };
       if (any) {
         wait(ok, &bars.o_full[set], segments & 1, 732);
@@ -656,7 +641,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
               const uint32_t x = raw.k[h][2 * gr + w], y = x >> 8;
-              put4(k_at + gr * (kKeys * 128) + h * 1024 + (((4 * w + t) ^ gq) << 4), fma2(x & 0x000f000fu, low, lo), fma2(x & 0x00f000f0u, high, lo),
+              store4(k_at + gr * (kKeys * 128) + h * 1024 + (((4 * w + t) ^ gq) << 4), fma2(x & 0x000f000fu, low, lo), fma2(x & 0x00f000f0u, high, lo),
                    fma2(y & 0x000f000fu, low, lo), fma2(y & 0x00f000f0u, high, lo));
             }
           }
@@ -678,10 +663,10 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
           for (int w = 4 * gr; w < 4 * gr + 4; ++w) {
             const uint32_t x = raw.v[w], y = x >> 8;
             const uint32_t to0 = v_at + w * 2048 + ((c ^ gq) << 4), to1 = v_at + w * 2048 + (((c + 1) ^ gq) << 4);
-            put1(to0, fma2(x & 0x000f000fu, low[0], lo[0]));
-            put1(to0 + 1024, fma2(x & 0x00f000f0u, high[0], lo[0]));
-            put1(to1, fma2(y & 0x000f000fu, low[1], lo[1]));
-            put1(to1 + 1024, fma2(y & 0x00f000f0u, high[1], lo[1]));
+            store1(to0, fma2(x & 0x000f000fu, low[0], lo[0]));
+            store1(to0 + 1024, fma2(x & 0x00f000f0u, high[0], lo[0]));
+            store1(to1, fma2(y & 0x000f000fu, low[1], lo[1]));
+            store1(to1 + 1024, fma2(y & 0x00f000f0u, high[1], lo[1]));
           }
         }
         fence_proxy();
@@ -792,6 +777,7 @@ int kv4_chunk_launch(Kv4Params p, int D, cudaStream_t st) {
   p.heads = p.G;
   p.subs = 1;
   p.tokens = kSets * (kRows / p.G);
+  p.over_heads = (65536 + p.heads - 1) / p.heads;
   if (p.a.dtype == B200_F16)
     return D == 128 ? chunk_launch<128, B200_F16>(g_raised[0], p, st) : chunk_launch<64, B200_F16>(g_raised[1], p, st);
   return D == 128 ? chunk_launch<128, B200_BF16>(g_raised[2], p, st) : chunk_launch<64, B200_BF16>(g_raised[3], p, st);

@@ -19,6 +19,7 @@ struct Kv4Params {
   b200_kv4_attention_args a;
   int G;                            // q heads of a kv head
   int heads, tokens, subs;          // of an item: q heads, positions; items that share a position's kv head
+  int over_heads;                   // 2^16 / heads, rounded up
   int least_rows, most_rows;        // sequences of this launch: by their rows
   int fill;                         // 1: rows of no sequence are zeroed here
   float log2_scale;
@@ -47,6 +48,23 @@ template <int TYPE> __device__ __forceinline__ void put(const Kv4Params &p, int6
   else
     ((__nv_bfloat16 *)p.a.out)[at] = __float2bfloat16_rn(x);
 }
+template <int TYPE> __device__ __forceinline__ void put4(const Kv4Params &p, int64_t at, float4 x) {
+  if (!p.wide_out) {
+    put<TYPE>(p, at, x.x);
+    put<TYPE>(p, at + 1, x.y);
+    put<TYPE>(p, at + 2, x.z);
+    put<TYPE>(p, at + 3, x.w);
+  } else if constexpr (TYPE == B200_F32) {
+    *reinterpret_cast<float4 *>((float *)p.a.out + at) = x;
+  } else if constexpr (TYPE == B200_F16) {
+    *reinterpret_cast<uint2 *>((__half *)p.a.out + at) = make_uint2(pack_f16(x.x, x.y), pack_f16(x.z, x.w));
+  } else {
+    uint32_t lo, hi;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(x.y), "f"(x.x));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(x.w), "f"(x.z));
+    *reinterpret_cast<uint2 *>((__nv_bfloat16 *)p.a.out + at) = make_uint2(lo, hi);
+  }
+}
 // four elements of q, aligned
 template <int TYPE> __device__ __forceinline__ void load_wide(const void *q, int64_t at, float (&x)[4]) {
   if constexpr (TYPE == B200_F32) {
@@ -73,15 +91,20 @@ struct Sequence {
     past = max(base, 0);
     tiles = n <= tokens ? min(n, 1) : (n + tokens - 1) / tokens;
   }
-  __device__ __forceinline__ long long before(int rt, int tokens) const {
+  template <typename I = long long> __device__ __forceinline__ I before(int rt, int tokens) const {
     return rt == 0 ? 0
-           : rt < tiles ? (long long)rt * (past + kKv4Item) + (long long)tokens * rt * (rt + 1) / 2
-                        : (long long)tiles * (past + kKv4Item) + (long long)tokens * tiles * (tiles - 1) / 2 + n;
+           : rt < tiles ? (I)rt * (past + kKv4Item) + (I)tokens * rt * (rt + 1) / 2
+                        : (I)tiles * (past + kKv4Item) + (I)tokens * tiles * (tiles - 1) / 2 + n;
   }
 };
-// x * a / b, rounded down
-__device__ __forceinline__ long long share(long long x, int a, int b) {
-  return x < (1 << 24) && a <= 255 ? (long long)((uint32_t)x * a / (uint32_t)b) : x * a / b;
+// x * a / b, rounded down, for a <= b up to 2^15
+template <typename I> __device__ __forceinline__ I share(I x, int a, int b) {
+  if constexpr (sizeof(I) == 4) {
+    const uint32_t q = (uint32_t)x / (uint32_t)b, r = (uint32_t)x - q * b;
+    return (I)(q * a + r * a / (uint32_t)b);
+  } else {
+    return x / b * a + x % b * a / b;
+  }
 }
 
 // An item and the first of its tiles that is meant.
@@ -96,8 +119,9 @@ template <int SHIFT, int SPLIT> struct KeyPlan {
   const int *r0, *base;    // [n + 1], [n]: a sequence's rows, and the position of the first
   const int *items;        // [n + 1]: items before it
   int n, tokens, slots, ctas, window;
-  bool whole;
+  bool whole, small;       // small: sums fit 32 bits (with room for one more item)
   long long total;
+  static constexpr int kNone = 1 << 30;   // more items than are counted
 
   static __host__ __device__ constexpr int bytes(int n) { return 20 * (n + 1); }
 
@@ -112,8 +136,8 @@ template <int SHIFT, int SPLIT> struct KeyPlan {
     if (tid == 0)
       *longest = 0;
     const int per = (n + THREADS - 1) / THREADS, first = min(n, tid * per), last = min(n, first + per);
-    long long sum = 0, count = 0;
-    int most = 0;
+    long long sum = 0;
+    int count = 0, most = 0;
     for (int s = first; s < last; ++s) {
       const int a = clamp(p.a.row_start[s], 0, p.a.rows), b = clamp(p.a.row_start[s + 1], 0, p.a.rows), rows = max(b - a, 0);
       const int at = clamp((long long)p.a.lens[s] - rows, -rows, room);
@@ -123,96 +147,134 @@ template <int SHIFT, int SPLIT> struct KeyPlan {
         s_r0[n] = b;
       const Sequence q(a, b, at, tokens);
       s_cost[s] = sum;
-      s_items[s] = (int)count;
+      s_items[s] = count;
       if (rows >= p.least_rows && rows <= p.most_rows) {
         sum += slots * q.before(q.tiles, tokens);
-        count += (long long)slots * q.tiles;
+        count = (int)min((long long)count + (long long)slots * q.tiles, (long long)kNone);
         most = max(most, q.past + rows + kKv4Item);
       }
     }
-    long long upto = sum, upto_items = count;
+    const int busy = (n - 1) / per / 32;   // the last warp with a sequence
+    if (warp <= busy) {
+      long long upto = sum;
+      int upto_items = count;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o), i = __shfl_up_sync(0xffffffffu, upto_items, o);
-      if (lane >= o) {
-        upto += v;
-        upto_items += i;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        const int i = __shfl_up_sync(0xffffffffu, upto_items, o);
+        if (lane >= o) {
+          upto += v;
+          upto_items = min(upto_items, kNone) + min(i, kNone);
+        }
       }
-    }
-    if (lane == 31) {
-      sums[warp] = upto;
-      sums[THREADS / 32 + warp] = upto_items;
+      upto_items = min(upto_items, kNone);
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 31) {
+        sums[warp] = upto;
+        sums[THREADS / 32 + warp] = (long long)upto_items << 32 | (uint32_t)most;
+      }
+      sum = upto - sum;
+      count = upto_items - count;
     }
     __syncthreads();
-    if (most > 0)
-      atomicMax(longest, most);
-    long long before = upto - sum, before_items = upto_items - count;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-      before += w < warp ? sums[w] : 0;
-      before_items += w < warp ? sums[THREADS / 32 + w] : 0;
-    }
-    if (before != 0)
-      for (int s = first; s < last; ++s) {
-        s_cost[s] += before;
-        s_items[s] += (int)before_items;
+    long long before = 0, all = 0;
+    int before_items = 0, all_items = 0;
+    most = 0;
+    for (int w = 0; w <= busy; ++w) {
+      if (w == warp) {
+        before = all;
+        before_items = all_items;
       }
-    if (tid == THREADS - 1) {
-      s_cost[n] = before + sum;
-      s_items[n] = (int)min(before_items + count, 0x7fffffffll);
+      all += sums[w];
+      all_items = min(all_items + (int)(sums[THREADS / 32 + w] >> 32), kNone);
+      most = max(most, (int)(uint32_t)sums[THREADS / 32 + w]);
+    }
+    if (warp <= busy)
+      for (int s = first; s < last; ++s) {
+        s_cost[s] += before + sum;
+        s_items[s] += before_items + count;
+      }
+    if (tid == 0) {
+      s_cost[n] = all;
+      s_items[n] = all_items;
     }
     __syncthreads();
     cost = s_cost;
     r0 = s_r0;
     base = s_base;
     items = s_items;
-    total = s_cost[n];
+    total = all;
+    small = total < (1ll << 30);
     ctas = total >= (long long)gridDim.x * least_keys ? gridDim.x : max(1, (int)total / least_keys);
-    const long long chunk = share(total, 1, ctas);
+    const long long chunk = small ? (int)total / ctas : total / ctas;
     window = chunk > kKv4Many ? kKv4Snap / 4 : (int)min((long long)kKv4Snap, chunk / 2 - 1);
-    const int all = s_items[n], each = (all + (int)gridDim.x - 1) / (int)gridDim.x;
-    whole = all < 0x7fffffff && (long long)each * *longest <= chunk + SPLIT;
+    const int each = (all_items + (int)gridDim.x - 1) / (int)gridDim.x;
+    whole = all_items < kNone && (long long)each * most <= chunk + SPLIT;
     if (whole)
-      ctas = max(1, min((int)gridDim.x, all));
+      ctas = max(1, min((int)gridDim.x, all_items));
   }
   __device__ __forceinline__ Sequence sequence(int s) const { return Sequence(r0[s], r0[s + 1], base[s], tokens); }
   __device__ __forceinline__ int item_keys(const Sequence &q, int rt) const { return q.past + min((rt + 1) * tokens, q.n); }
   __device__ __forceinline__ int item_tiles(const Sequence &q, int rt) const { return (item_keys(q, rt) + (1 << SHIFT) - 1) >> SHIFT; }
   // the item with key x of all, from begin to end; at.tile: the first tile from x on (none of the item's, if x lies in its last or behind it)
-  __device__ __forceinline__ void locate(long long x, Place &at, long long &begin, long long &end) const {
+  template <typename I> __device__ __forceinline__ void locate_in(I x, Place &at, I &begin, I &end) const {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (cost[mid] <= x)
+      if ((I)cost[mid] <= x)
         lo = mid;
       else
         hi = mid;
     }
     at.s = lo;
     const Sequence q = sequence(lo);
-    begin = cost[lo];
-    const long long head = q.before(q.tiles, tokens);
-    at.slot = (x - begin) >> 32 ? (int)((x - begin) / head) : (int)((uint32_t)(x - begin) / (uint32_t)min(head, 0xffffffffll));
-    begin += at.slot * head;
+    begin = (I)cost[lo];
+    if constexpr (sizeof(I) == 4) {
+      const I head = q.template before<I>(q.tiles, tokens);
+      at.slot = (uint32_t)(x - begin) / (uint32_t)head;
+      begin += at.slot * head;
+    } else {
+      const I head = q.template before<I>(q.tiles, tokens);
+      at.slot = (int)((x - begin) / head);
+      begin += at.slot * head;
+    }
     int a = 0, b = q.tiles;
     while (b - a > 1) {
       const int mid = (a + b) >> 1;
-      if (q.before(mid, tokens) <= x - begin)
+      if (q.template before<I>(mid, tokens) <= x - begin)
         a = mid;
       else
         b = mid;
     }
     at.rt = a;
-    end = begin + q.before(a + 1, tokens);
-    begin += q.before(a, tokens);
+    end = begin + q.template before<I>(a + 1, tokens);
+    begin += q.template before<I>(a, tokens);
     at.tile = (int)((x - begin + (1 << SHIFT) - 1) >> SHIFT);
+  }
+  __device__ __forceinline__ Place locate(long long x) const {
+    Place at;
+    if (small) {
+      int begin, end;
+      locate_in<int>((int)x, at, begin, end);
+    } else {
+      long long begin, end;
+      locate_in<long long>(x, at, begin, end);
+    }
+    return at;
+  }
+  template <typename I> __device__ __forceinline__ long long border_in(int c) const {
+    const I x = share<I>((I)total, c, ctas);
+    Place at;
+    I begin, end;
+    locate_in<I>(x, at, begin, end);
+    return x - begin <= end - x ? (x - begin <= window ? begin : x) : end - x <= window ? end : x;
   }
   // where CTA c begins: at its share of all keys, or at the item border next to that
   __device__ __forceinline__ long long border(int c) const {
     if (c <= 0 || c >= ctas)
       return c <= 0 ? 0 : total;
     if (whole) {
-      const int i = (int)share(items[n], c, ctas);
+      const int i = share<int>(items[n], c, ctas);
       int lo = 0, hi = n;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -222,14 +284,14 @@ template <int SHIFT, int SPLIT> struct KeyPlan {
           hi = mid;
       }
       const Sequence q = sequence(lo);
-      const int slot = (i - items[lo]) / q.tiles;
+      const int slot = q.tiles == 1 ? i - items[lo] : (i - items[lo]) / q.tiles;
       return cost[lo] + slot * q.before(q.tiles, tokens) + q.before(i - items[lo] - slot * q.tiles, tokens);
     }
-    const long long x = share(total, c, ctas);
-    Place at;
-    long long begin, end;
-    locate(x, at, begin, end);
-    return x - begin <= end - x ? (x - begin <= window ? begin : x) : end - x <= window ? end : x;
+    return small ? border_in<int>(c) : border_in<long long>(c);
+  }
+  // where part c of n of a range of `mine` keys begins
+  __device__ __forceinline__ long long part_of(long long mine, int c, int of) const {
+    return small ? (long long)share<int>((int)mine, c, of) : share<long long>(mine, c, of);
   }
   __device__ __forceinline__ int nominal(long long x) const { return (int)(((x + 1) * ctas - 1) / total); }   // the CTA that x would lie in without that
   __device__ __forceinline__ void next_item(Place &at, const Sequence &q) const {
@@ -270,9 +332,10 @@ template <int SHIFT, int SPLIT> struct KeyPlan {
   }
 };
 
-// element of a row in q (ld: q's) or out, before its dims: row i of the position `token` and on, of an item's heads
+// element of a row in q (ld: q's) or out, before its dims: row i (0 .. 127) of the position `token` and on, of an item's heads
 __device__ __forceinline__ int64_t row_at(const Kv4Params &p, int token, int slot, int i, int64_t ld, int D) {
-  return (token + (int64_t)(i / p.heads)) * ld + (int64_t)((slot / p.subs) * p.G + slot % p.subs * p.heads + i % p.heads) * D;
+  const int kv = p.subs == 1 ? slot : slot / p.subs, behind = i * p.over_heads >> 16;   // i / heads
+  return (token + behind) * ld + (int64_t)(kv * p.G + (slot - kv * p.subs - behind) * p.heads + i) * D;
 }
 // number of a tile of sixteen keys of a sequence in the pool, or -1
 __device__ __forceinline__ int tile_source(const Kv4Params &p, int s, int kv, int t) {
