@@ -574,25 +574,59 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
     const int k = i / lanes;
     const Chain c = chain(k);
     auto part = [&](int w) { return c.opened && w == c.first ? reinterpret_cast<const float *>(s_all + w * RING) : s_left[w].a_part; };
-#pragma unroll 2
-    for (int e = i % lanes; e < FOURS; e += lanes) {
-      const int row = e / (D / 4), d = e % (D / 4) * 4;
-      float top = kKv4Seed, l = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    // a lane's share of the rows, all of it at once; part by part, to the larger reference
+    constexpr int MOST = FOURS / 32;
+    float top[MOST], l[MOST];
+    float4 o[MOST];
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) {
+      top[u] = kKv4Seed;
+      l[u] = 0.f;
+      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const int e0 = i % lanes;
+    if (lanes >= FOURS) {   // (an element a lane, and many parts: loads side by side)
+      const int row = e0 / (D / 4), d = e0 % (D / 4) * 4;
+      if (e0 >= FOURS)
+        break;
+#pragma unroll 4
       for (int w = c.first; w <= c.last; ++w)
-        top = fmaxf(top, part(w)[kRows * (D + 4) + row]);
+        top[0] = fmaxf(top[0], part(w)[kRows * (D + 4) + row]);
+#pragma unroll 4
       for (int w = c.first; w <= c.last; ++w) {
         const float *x = part(w);
-        add(o, l, *reinterpret_cast<const float4 *>(x + row * (D + 4) + d), x[kRows * (D + 4) + kRows + row], ex2(x[kRows * (D + 4) + row] - top));
+        add(o[0], l[0], *reinterpret_cast<const float4 *>(x + row * (D + 4) + d), x[kRows * (D + 4) + kRows + row], ex2(x[kRows * (D + 4) + row] - top[0]));
       }
+    }
+#pragma unroll 1
+    for (int w = c.first; w <= c.last && lanes < FOURS; ++w) {
+      const float *x = part(w);
+#pragma unroll
+      for (int u = 0; u < MOST; ++u) {
+        const int e = e0 + u * lanes, row = e / (D / 4), d = e % (D / 4) * 4;
+        if (e < FOURS) {
+          const float r = x[kRows * (D + 4) + row], to = fmaxf(top[u], r), keep = ex2(top[u] - to);
+          const float4 v = *reinterpret_cast<const float4 *>(x + row * (D + 4) + d);
+          top[u] = to;
+          l[u] *= keep;
+          o[u] = make_float4(o[u].x * keep, o[u].y * keep, o[u].z * keep, o[u].w * keep);
+          add(o[u], l[u], v, x[kRows * (D + 4) + kRows + row], ex2(r - to));
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) {
+      const int e = e0 + u * lanes, row = e / (D / 4), d = e % (D / 4) * 4;
+      if (e >= FOURS)
+        break;
       if (c.whole) {
-        write_out(s_left[c.first].b, row, d, o, l);
+        write_out(s_left[c.first].b, row, d, o[u], l[u]);
       } else {
         float *to = p.parts + ((int64_t)blockIdx.x * 2 + c.opened) * PART;
-        *reinterpret_cast<float4 *>(to + row * (D + 4) + d) = o;
+        *reinterpret_cast<float4 *>(to + row * (D + 4) + d) = o[u];
         if (d == 0) {
-          to[kRows * (D + 4) + row] = top;
-          to[kRows * (D + 4) + kRows + row] = l;
+          to[kRows * (D + 4) + row] = top[u];
+          to[kRows * (D + 4) + kRows + row] = l[u];
         }
       }
     }
