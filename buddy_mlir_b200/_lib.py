@@ -137,6 +137,7 @@ def load():
         "b200_model_generate": (i32, [vp, i32, i32, i32, vp]),
         "b200_model_prefill": (i32, [vp, vp, i32, i32, vp, i32, C.POINTER(C.c_int)]),
         "b200_batch_create": (i32, [vp, i32, i32, i32, i32, C.POINTER(vp)]),
+        "b200_batch_create_kv4": (i32, [vp, i32, i32, i32, i32, C.POINTER(vp)]),
         "b200_batch_destroy": (None, [vp]),
         "b200_batch_add": (i32, [vp, C.POINTER(C.c_int)]),
         "b200_batch_remove": (i32, [vp, i32]),

@@ -11,6 +11,7 @@
 // q/k/v/gate/up, row-parallel o/down, sum after each, vocab-sharded lm_head;
 // buddy-deepseek-r1-distributed.cpp:521-617) with NCCL in place of MPI.
 #include "common.cuh"
+#include "kv4.cuh"
 #include "decode.cuh"
 
 #include <dlfcn.h>
@@ -1964,12 +1965,52 @@ struct b200_batch {
   int part_rows = 0, max_context = 0;
   int rows_cap = 0;
   float last_ms = 0.f;
+  // A cache in 4 bits: its allocator lives on the device (b200_page_step), from one set of lengths and stack top to the other; a pass that fails
+  // leaves the current one as it was.
+  bool kv4 = false;
+  std::vector<uint8_t *> pool4;         // [layers]
+  int32_t *d_held[2] = {}, *d_n_free[2] = {}, *d_free = nullptr, *d_add = nullptr, *d_row_start = nullptr, *d_status = nullptr;
+  int64_t *d_slots = nullptr;
+  void *work4 = nullptr;
+  int64_t work4_bytes = 0;
+  int cur = 0, free4 = 0;
 };
+
+// Pages of a 4-bit cache for n more positions of a sequence.
+static int batch_pages4(const b200_batch *b, int seq, int n) {
+  return (b->len[seq] + n + b->page - 1) / b->page - (b->len[seq] + b->page - 1) / b->page;
+}
+// Queues the allocator's step: add[s] more positions of every sequence (or its end), up to max_rows of them.
+static int batch_step4(b200_batch *b, const std::vector<int32_t> &add, int max_rows) {
+  b200_model *m = b->m;
+  B200_CUDA(cudaMemcpyAsync(b->d_add, add.data(), add.size() * 4, cudaMemcpyHostToDevice, m->stream));
+  b200_page_step_args a{};
+  a.n_seqs = b->max_seqs;
+  a.page = b->page;
+  a.table_stride = b->table_stride;
+  a.n_pages = b->n_pages;
+  a.max_rows = max_rows;
+  a.held = b->d_held[b->cur];
+  a.add = b->d_add;
+  a.held_out = b->d_held[b->cur ^ 1];
+  a.block_table = b->d_table;
+  a.free_pages = b->d_free;
+  a.n_free = b->d_n_free[b->cur];
+  a.n_free_out = b->d_n_free[b->cur ^ 1];
+  a.row_start = b->d_row_start;
+  a.slots = b->d_slots;
+  a.row_seq = b->d_seq;
+  a.row_pos = b->d_pos;
+  a.status = b->d_status;
+  return b200::page_step_launch(a, m->stream);
+}
 
 // step: a decode step, every row a sequence of its own, with logits of all rows; otherwise a chunk of one sequence's prompt, with
 // those of its last row.
+// A cache in 4 bits: rows stand in the order of their sequences; `order` says which of the caller's a row is (decode steps), `add` how many a
+// sequence has.
 static int batch_rows(b200_batch *b, int M, const int32_t *tokens, const int32_t *row_seq, const int32_t *row_pos, bool step,
-                      float *logits_host, int32_t *next_host) {
+                      float *logits_host, int32_t *next_host, const std::vector<int32_t> *add = nullptr, const int *order = nullptr) {
   b200_model *m = b->m;
   // A w8a8 projection scales its whole activation tensor: rows of unrelated sequences in one
   // batch would share that scale, and each sequence's result would depend on its neighbours.
@@ -1982,32 +2023,60 @@ static int batch_rows(b200_batch *b, int M, const int32_t *tokens, const int32_t
   if (int rc = prefill_reserve(m, M, logit_rows)) return rc;
   cudaStream_t st = m->stream;
   if (M > b->rows_cap) {
-    cudaFree(b->d_seq); cudaFree(b->d_pos); cudaFree(b->d_next);
+    cudaFree(b->d_seq); cudaFree(b->d_pos); cudaFree(b->d_next); cudaFree(b->d_slots);
     b->d_seq = b->d_pos = b->d_next = nullptr;
+    b->d_slots = nullptr;
     b->rows_cap = 0;
     if (int rc = session_alloc(m, (void **)&b->d_seq, (size_t)M * 4)) return rc;
     if (int rc = session_alloc(m, (void **)&b->d_pos, (size_t)M * 4)) return rc;
     if (int rc = session_alloc(m, (void **)&b->d_next, (size_t)M * 4)) return rc;
+    if (b->kv4)
+      if (int rc = session_alloc(m, (void **)&b->d_slots, (size_t)M * 8)) return rc;
     b->rows_cap = M;
   }
   // a prefill chunk: consecutive positions of one sequence
-  bool one_chunk = prefill_attn_takes(m->pf_qkv, QKV, b->pool[0], b->pool[1], m->pf_att, QD, D, M);
+  bool one_chunk = !b->kv4 && prefill_attn_takes(m->pf_qkv, QKV, b->pool[0], b->pool[1], m->pf_att, QD, D, M);
   for (int r = 1; r < M && one_chunk; ++r)
     one_chunk = row_seq[r] == row_seq[0] && row_pos[r] == row_pos[0] + r;
   if (one_chunk)
     if (int rc = prefill_attention_reserve(m, row_pos[0] + M, b->max_context)) return rc;
   const int longest = 1 + *std::max_element(row_pos, row_pos + M);
-  const bool one_kernel = step && paged_decode_takes(m->pf_qkv, QKV, b->pool[0], b->pool[1], m->qh, m->kvh, D, M, longest);
+  const bool one_kernel = !b->kv4 && step && paged_decode_takes(m->pf_qkv, QKV, b->pool[0], b->pool[1], m->qh, m->kvh, D, M, longest);
   B200_CUDA(cudaEventRecord(m->ev0, st));
   B200_CUDA(cudaMemcpyAsync(m->pf_tokens, tokens, (size_t)M * 4, cudaMemcpyHostToDevice, st));
-  B200_CUDA(cudaMemcpyAsync(b->d_seq, row_seq, (size_t)M * 4, cudaMemcpyHostToDevice, st));
-  B200_CUDA(cudaMemcpyAsync(b->d_pos, row_pos, (size_t)M * 4, cudaMemcpyHostToDevice, st));
-  B200_CUDA(cudaMemcpyAsync(b->d_table, b->table.data(), b->table.size() * 4, cudaMemcpyHostToDevice, st));
+  if (b->kv4) {
+    if (int rc = batch_step4(b, *add, M)) return rc;
+  } else {
+    B200_CUDA(cudaMemcpyAsync(b->d_seq, row_seq, (size_t)M * 4, cudaMemcpyHostToDevice, st));
+    B200_CUDA(cudaMemcpyAsync(b->d_pos, row_pos, (size_t)M * 4, cudaMemcpyHostToDevice, st));
+    B200_CUDA(cudaMemcpyAsync(b->d_table, b->table.data(), b->table.size() * 4, cudaMemcpyHostToDevice, st));
+  }
   if (int rc = embed_rows_launch(m->embed, m->pf_tokens, m->pf_x, H, M, st)) return rc;
   for (int l = 0; l < c.n_layers; ++l) {
     Layer &L = m->layers[l];
     if (int rc = linear_rows(m, L.qkv, m->pf_x, H, M, m->pf_qkv, QKV, nullptr, L.in_norm, false)) return rc;
-    if (one_kernel) {
+    if (b->kv4) {
+      const b200_kv4_cache cache{b->pool4[l], b->n_pages, m->kvh, D, b->page};
+      if (int rc = rope_kv_paged_launch(m->pf_qkv, QKV, nullptr, nullptr, m->inv_freq, L.q_norm, L.k_norm, c.eps, m->qh, m->kvh, D, b->page, b->d_seq,
+                                        b->d_pos, b->d_table, b->table_stride, M, st))
+        return rc;
+      if (int rc = b200_kv4_write(&cache, m->pf_qkv + QD, QKV, m->pf_qkv + QD + KD, QKV, B200_F32, b->d_slots, M, st)) return rc;
+      b200_kv4_attention_args a{};
+      a.q = m->pf_qkv;
+      a.out = m->pf_att;
+      a.dtype = B200_F32;
+      a.q_heads = m->qh;
+      a.q_ld = QKV;
+      a.out_ld = QD;
+      a.rows = M;
+      a.n_seqs = b->max_seqs;
+      a.row_start = b->d_row_start;
+      a.lens = b->d_held[b->cur ^ 1];
+      a.block_table = b->d_table;
+      a.table_stride = b->table_stride;
+      a.scale = 1.0f / sqrtf((float)D);
+      if (int rc = b200_kv4_attention(&cache, &a, b->work4, b->work4_bytes, st)) return rc;
+    } else if (one_kernel) {
       if (int rc = paged_decode_launch(m->pf_qkv, QKV, b->pool[2 * l], b->pool[2 * l + 1], m->pf_att, QD, m->inv_freq, L.q_norm, L.k_norm,
                                        c.eps, m->qh, m->kvh, D, b->page, b->d_seq, b->d_pos, b->d_table, b->table_stride, M, longest, st))
         return rc;
@@ -2034,14 +2103,27 @@ static int batch_rows(b200_batch *b, int M, const int32_t *tokens, const int32_t
     return rc;
   if (int rc = argmax_rows_launch(m->pf_logits, c.vocab, logit_rows, b->d_next, st)) return rc;
   B200_CUDA(cudaEventRecord(m->ev1, st));
-  if (logits_host)
+  bool in_order = true;
+  for (int r = 0; order && r < logit_rows; ++r)
+    in_order = in_order && order[r] == r;
+  if (logits_host && in_order)
     B200_CUDA(cudaMemcpyAsync(logits_host, m->pf_logits, (size_t)logit_rows * c.vocab * 4, cudaMemcpyDeviceToHost, st));
+  for (int r = 0; logits_host && !in_order && r < logit_rows; ++r)
+    B200_CUDA(cudaMemcpyAsync(logits_host + (int64_t)order[r] * c.vocab, m->pf_logits + (int64_t)r * c.vocab, (size_t)c.vocab * 4, cudaMemcpyDeviceToHost, st));
+  std::vector<int32_t> next(next_host ? logit_rows : 0);
   if (next_host)
-    B200_CUDA(cudaMemcpyAsync(next_host, b->d_next, (size_t)logit_rows * 4, cudaMemcpyDeviceToHost, st));
+    B200_CUDA(cudaMemcpyAsync(next.data(), b->d_next, (size_t)logit_rows * 4, cudaMemcpyDeviceToHost, st));
+  int32_t status = 0;
+  if (b->kv4)
+    B200_CUDA(cudaMemcpyAsync(&status, b->d_status, 4, cudaMemcpyDeviceToHost, st));
   if (int rc = rows_status_queue(m)) return rc;
   B200_CUDA(cudaStreamSynchronize(st));
+  for (int r = 0; r < (int)next.size(); ++r)
+    next_host[order ? order[r] : r] = next[r];
   B200_CUDA(cudaEventElapsedTime(&b->last_ms, m->ev0, m->ev1));
-  return rows_status(m);
+  if (status != 0)
+    return fail(B200_ESTATE, "batch: the page allocator refused a step (%d)", status);
+  return rows_status(m);   // (the 4-bit cache's attention has no bounded waits in f32)
 }
 
 // pages for positions [len, len + n) of a sequence
@@ -2059,13 +2141,43 @@ static int batch_grow(b200_batch *b, int seq, int n) {
   return B200_OK;
 }
 
-int b200_batch_create(b200_model *m, int max_seqs, int page_size, int n_pages, int max_context, b200_batch **out) {
+// Whether a 4-bit cache has room for these; and what the host keeps of them when their pass is done.
+static int batch_room4(const b200_batch *b, const std::vector<int32_t> &add) {
+  int64_t pages = 0;
+  for (int s = 0; s < b->max_seqs; ++s)
+    if (add[(size_t)s] > 0) {
+      if ((int64_t)b->len[s] + add[(size_t)s] > (int64_t)b->table_stride * b->page)
+        return fail(B200_ELIMIT, "batch: sequence %d would exceed the context limit of %d positions", s, b->table_stride * b->page);
+      pages += batch_pages4(b, s, add[(size_t)s]);
+    }
+  return pages > b->free4 ? fail(B200_ENOMEM, "batch: the page pool is exhausted (%d pages)", b->n_pages) : B200_OK;
+}
+static void batch_done4(b200_batch *b, const std::vector<int32_t> &add) {
+  b->cur ^= 1;
+  for (int s = 0; s < b->max_seqs; ++s)
+    if (add[(size_t)s] > 0) {
+      b->free4 -= batch_pages4(b, s, add[(size_t)s]);
+      b->len[s] += add[(size_t)s];
+    }
+}
+
+static int batch_create(b200_model *m, int max_seqs, int page_size, int n_pages, int max_context, bool kv4, b200_batch **out) {
   if (!m || !out || max_seqs < 1 || page_size < 1 || n_pages < 1 || max_context < 1)
     return fail(B200_EINVAL, "batch_create: bad argument");
   if (!m->finalized || m->tp != 1)
     return fail(B200_ESTATE, "batch_create: a finalised single-GPU model is required");
+  if (kv4) {
+    if (b200_kv4_pool_bytes(n_pages, m->kvh, m->cfg.head_dim, page_size) < 0)
+      return fail(B200_EINVAL, "batch_create: no 4-bit cache of %d pages of %d positions, %d heads of %d", n_pages, page_size, m->kvh, m->cfg.head_dim);
+    if (max_seqs > B200_KV4_ATTENTION_MAX_SEQS)
+      return fail(B200_ELIMIT, "batch_create: %d sequences (at most %d with a 4-bit cache)", max_seqs, B200_KV4_ATTENTION_MAX_SEQS);
+  }
+  if (((int64_t)max_context + page_size - 1) / page_size * page_size > INT32_MAX - 64)
+    return fail(B200_EINVAL, "batch_create: a context of %d positions", max_context);
   b200_batch *b = new b200_batch();
   b->m = m;
+  b->kv4 = kv4;
+  b->free4 = n_pages;
   b->max_seqs = max_seqs;
   b->page = page_size;
   b->n_pages = n_pages;
@@ -2075,18 +2187,38 @@ int b200_batch_create(b200_model *m, int max_seqs, int page_size, int n_pages, i
   for (int i = n_pages - 1; i >= 0; --i)
     b->free_pages.push_back(i);
   const size_t pool_bytes = (size_t)n_pages * m->kvh * page_size * m->cfg.head_dim * 4;
-  b->pool.assign(2 * m->cfg.n_layers, nullptr);
+  b->pool.assign(kv4 ? 0 : 2 * m->cfg.n_layers, nullptr);
+  b->pool4.assign(kv4 ? m->cfg.n_layers : 0, nullptr);
   const bool persistent = m->persistent;
   int rc = B200_OK;
+  for (auto &p : b->pool4)
+    if (rc == B200_OK) rc = session_alloc(m, (void **)&p, (size_t)b200_kv4_pool_bytes(n_pages, m->kvh, m->cfg.head_dim, page_size));
+  if (kv4) {
+    b->work4_bytes = b200_kv4_attention_workspace_bytes(m->qh, m->kvh, m->cfg.head_dim);
+    std::vector<std::pair<void **, size_t>> arrays{{(void **)&b->d_held[0], (size_t)max_seqs * 4}, {(void **)&b->d_held[1], (size_t)max_seqs * 4},
+                                                   {(void **)&b->d_n_free[0], 4}, {(void **)&b->d_n_free[1], 4}, {(void **)&b->d_free, (size_t)n_pages * 4},
+                                                   {(void **)&b->d_add, (size_t)max_seqs * 4}, {(void **)&b->d_row_start, (size_t)(max_seqs + 1) * 4},
+                                                   {(void **)&b->d_status, 4}, {&b->work4, (size_t)b->work4_bytes}};
+    for (auto &a : arrays) {
+      if (rc == B200_OK) rc = session_alloc(m, a.first, a.second);
+      if (rc == B200_OK && cudaMemsetAsync(*a.first, 0, a.second, m->stream) != cudaSuccess)
+        rc = fail(B200_ECUDA, "batch_create: cudaMemset failed");
+    }
+    // the stack of free pages, the first page on top
+    if (rc == B200_OK && (cudaMemcpyAsync(b->d_free, b->free_pages.data(), (size_t)n_pages * 4, cudaMemcpyHostToDevice, m->stream) != cudaSuccess ||
+                          cudaMemcpyAsync(b->d_n_free[0], &n_pages, 4, cudaMemcpyHostToDevice, m->stream) != cudaSuccess ||
+                          cudaStreamSynchronize(m->stream) != cudaSuccess))
+      rc = fail(B200_ECUDA, "batch_create: copying the free pages failed");
+  }
   for (auto &p : b->pool)
     if (rc == B200_OK) rc = session_alloc(m, (void **)&p, pool_bytes);
   if (rc == B200_OK) rc = session_alloc(m, (void **)&b->d_table, b->table.size() * 4);
   b->max_context = b->table_stride * page_size;
-  b->part_rows = max_seqs;
-  if (rc == B200_OK)
+  b->part_rows = kv4 ? 0 : max_seqs;
+  if (rc == B200_OK && !kv4)
     rc = session_alloc(m, (void **)&b->d_part,
                        (size_t)gqa_paged_scratch_floats(b->part_rows, m->qh, m->cfg.head_dim, b->max_context) * 4);
-  if (rc == B200_OK && cudaMemsetAsync(b->d_part, 0, (size_t)b->part_rows * m->qh * 4, m->stream) != cudaSuccess)   // the counters
+  if (rc == B200_OK && !kv4 && cudaMemsetAsync(b->d_part, 0, (size_t)b->part_rows * m->qh * 4, m->stream) != cudaSuccess)   // the counters
     rc = fail(B200_ECUDA, "batch_create: cudaMemset failed");
   if (rc != B200_OK) {
     b200_batch_destroy(b);
@@ -2102,9 +2234,22 @@ int b200_batch_create(b200_model *m, int max_seqs, int page_size, int n_pages, i
   return B200_OK;
 }
 
+int b200_batch_create(b200_model *m, int max_seqs, int page_size, int n_pages, int max_context, b200_batch **out) {
+  return batch_create(m, max_seqs, page_size, n_pages, max_context, false, out);
+}
+int b200_batch_create_kv4(b200_model *m, int max_seqs, int page_size, int n_pages, int max_context, b200_batch **out) {
+  return batch_create(m, max_seqs, page_size, n_pages, max_context, true, out);
+}
+
 void b200_batch_destroy(b200_batch *b) {
   if (!b) return;
   for (auto p : b->pool) cudaFree(p);
+  for (auto p : b->pool4) cudaFree(p);
+  for (int i = 0; i < 2; ++i) {
+    cudaFree(b->d_held[i]);
+    cudaFree(b->d_n_free[i]);
+  }
+  cudaFree(b->d_free); cudaFree(b->d_add); cudaFree(b->d_row_start); cudaFree(b->d_status); cudaFree(b->d_slots); cudaFree(b->work4);
   cudaFree(b->d_table); cudaFree(b->d_seq); cudaFree(b->d_pos); cudaFree(b->d_next);
   cudaFree(b->d_part);
   delete b;
@@ -2126,6 +2271,16 @@ int b200_batch_remove(b200_batch *b, int seq) {
   if (!b || seq < 0 || seq >= b->max_seqs || b->len[seq] < 0)
     return fail(B200_EINVAL, "batch_remove: no such sequence");
   const int pages = (b->len[seq] + b->page - 1) / b->page;
+  if (b->kv4) {
+    std::vector<int32_t> add((size_t)b->max_seqs, 0);
+    add[(size_t)seq] = -1;
+    if (int rc = batch_step4(b, add, 0)) return rc;
+    B200_CUDA(cudaStreamSynchronize(b->m->stream));
+    b->cur ^= 1;
+    b->free4 += pages;
+    b->len[seq] = -1;
+    return B200_OK;
+  }
   for (int i = 0; i < pages; ++i)
     b->free_pages.push_back(b->table[(size_t)seq * b->table_stride + i]);
   b->len[seq] = -1;
@@ -2135,7 +2290,7 @@ int b200_batch_remove(b200_batch *b, int seq) {
 int b200_batch_length(const b200_batch *b, int seq) {
   return (b && seq >= 0 && seq < b->max_seqs) ? b->len[seq] : -1;
 }
-int b200_batch_free_pages(const b200_batch *b) { return b ? (int)b->free_pages.size() : 0; }
+int b200_batch_free_pages(const b200_batch *b) { return !b ? 0 : b->kv4 ? b->free4 : (int)b->free_pages.size(); }
 float b200_batch_last_ms(const b200_batch *b) { return b ? b->last_ms : 0.f; }
 
 int b200_batch_prefill(b200_batch *b, int seq, const int32_t *tokens, int n, float *logits_host, int *next_token) {
@@ -2144,13 +2299,22 @@ int b200_batch_prefill(b200_batch *b, int seq, const int32_t *tokens, int n, flo
   for (int i = 0; i < n; ++i)
     if (tokens[i] < 0 || tokens[i] >= b->m->cfg.vocab)
       return fail(B200_EINVAL, "batch_prefill: token %d at row %d out of range", tokens[i], i);
-  if (int rc = batch_grow(b, seq, n)) return rc;
+  std::vector<int32_t> add(b->kv4 ? (size_t)b->max_seqs : 0, 0);
+  if (b->kv4) {
+    add[(size_t)seq] = n;
+    if (int rc = batch_room4(b, add)) return rc;
+  } else if (int rc = batch_grow(b, seq, n)) {
+    return rc;
+  }
   std::vector<int32_t> rs((size_t)n, seq), rp((size_t)n);
   for (int i = 0; i < n; ++i)
     rp[(size_t)i] = b->len[seq] + i;
   int32_t nxt = 0;
-  if (int rc = batch_rows(b, n, tokens, rs.data(), rp.data(), false, logits_host, &nxt)) return rc;
-  b->len[seq] += n;
+  if (int rc = batch_rows(b, n, tokens, rs.data(), rp.data(), false, logits_host, &nxt, &add)) return rc;
+  if (b->kv4)
+    batch_done4(b, add);
+  else
+    b->len[seq] += n;
   if (next_token) *next_token = nxt;
   return B200_OK;
 }
@@ -2168,6 +2332,24 @@ int b200_batch_decode(b200_batch *b, int n, const int *seqs, const int32_t *toke
     if (tokens[i] < 0 || tokens[i] >= b->m->cfg.vocab)
       return fail(B200_EINVAL, "batch_decode: token %d of sequence %d out of range", tokens[i], s);
     seen[(size_t)s] = 1;
+  }
+  if (b->kv4) {   // the rows in the order of their sequences
+    std::vector<int32_t> add((size_t)b->max_seqs, 0), sorted((size_t)n);
+    std::vector<int> order((size_t)n);
+    for (int i = 0; i < n; ++i) {
+      add[(size_t)seqs[i]] = 1;
+      order[(size_t)i] = i;
+    }
+    if (int rc = batch_room4(b, add)) return rc;
+    std::sort(order.begin(), order.end(), [&](int x, int y) { return seqs[x] < seqs[y]; });
+    for (int i = 0; i < n; ++i) {
+      sorted[(size_t)i] = tokens[order[(size_t)i]];
+      rp[(size_t)i] = b->len[seqs[order[(size_t)i]]];
+      rs[(size_t)i] = seqs[order[(size_t)i]];
+    }
+    if (int rc = batch_rows(b, n, sorted.data(), rs.data(), rp.data(), true, logits_host, next_tokens, &add, order.data())) return rc;
+    batch_done4(b, add);
+    return B200_OK;
   }
   for (int i = 0; i < n; ++i)
     if (int rc = batch_grow(b, seqs[i], 1)) return rc;

@@ -34,7 +34,7 @@ constexpr int kRopeThreads = 512;
 struct RopeRows {
   float *qkv;
   int64_t ld;
-  float *k_cache, *v_cache;   // or pools
+  float *k_cache, *v_cache;   // or pools; PAGED: null where the rows go to a cache of another kind, by a kernel of its own
   const float *inv_freq, *q_norm, *k_norm;
   float eps;
   int q_heads, kv_heads, D;
@@ -75,8 +75,10 @@ template <bool PAGED, int V> __global__ void __launch_bounds__(kRopeThreads) rop
   }
   // of kv head h: row0 + h * step
   const int64_t step = PAGED ? p.page : p.max_len;
-  const int64_t row0 = PAGED ? (int64_t)p.block_table[(int64_t)p.row_seq[m] * p.table_stride + pos / p.page] * p.kv_heads * p.page + pos % p.page
-                             : pos;
+  const bool writes = !PAGED || p.k_cache != nullptr;
+  const int64_t row0 = !PAGED ? pos
+                       : writes ? (int64_t)p.block_table[(int64_t)p.row_seq[m] * p.table_stride + pos / p.page] * p.kv_heads * p.page + pos % p.page
+                                : 0;
   __syncthreads();
   kernel_wait();
   float *row = p.qkv + (int64_t)m * p.ld;
@@ -85,6 +87,8 @@ template <bool PAGED, int V> __global__ void __launch_bounds__(kRopeThreads) rop
     const int h = head - p.q_heads;
     RopeVec<V> a, b;
     if (h >= p.kv_heads) {   // v
+      if (!writes)
+        break;
       float *v = p.v_cache + (row0 + (h - p.kv_heads) * step) * D;
       for (int j = lane * V; j < half; j += 32 * V) {
         a.load(x + j);
@@ -107,7 +111,7 @@ template <bool PAGED, int V> __global__ void __launch_bounds__(kRopeThreads) rop
       }
       r = rsqrtf(__fadd_rn(__fmul_rn(warp_sum(ss), 1.0f / (float)D), p.eps));
     }
-    float *k = h < 0 ? nullptr : p.k_cache + (row0 + h * step) * D;
+    float *k = h < 0 || !writes ? nullptr : p.k_cache + (row0 + h * step) * D;
     for (int j = lane * V; j < half; j += 32 * V) {
       a.load(x + j);
       b.load(x + half + j);

@@ -263,12 +263,16 @@ class BatchSession:
     (b200_batch_*): prefill a prompt per sequence, then advance any subset of
     them by one token per step.  Not part of buddy-mlir's interface (its
     sessions are single-sequence); per sequence the results are those of
-    ModelSession."""
+    ModelSession.  kv_bits=4 holds the cache in 4 bits (b200_batch_create_kv4: a
+    seventh of the memory, results with the rounding of its keys and values)."""
 
-    def __init__(self, model: ModelSession, max_seqs: int, page_size: int, n_pages: int, max_context: int):
+    def __init__(self, model: ModelSession, max_seqs: int, page_size: int, n_pages: int, max_context: int, kv_bits: int = 32):
+        if kv_bits not in (4, 32):
+            raise ValueError(f"kv_bits is 4 or 32, not {kv_bits}")
         self.model, self.lib = model, model.lib
         self._h = C.c_void_p()
-        _lib.check(self.lib.b200_batch_create(model._h, max_seqs, page_size, n_pages, max_context, C.byref(self._h)))
+        create = self.lib.b200_batch_create_kv4 if kv_bits == 4 else self.lib.b200_batch_create
+        _lib.check(create(model._h, max_seqs, page_size, n_pages, max_context, C.byref(self._h)))
 
     def close(self):
         if self._h:

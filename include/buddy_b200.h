@@ -518,6 +518,14 @@ int b200_model_prefill(b200_model *m, const int32_t *tokens, int n_tokens,
 typedef struct b200_batch b200_batch;
 int b200_batch_create(b200_model *m, int max_seqs, int page_size, int n_pages,
                       int max_context, b200_batch **out);
+/* The same over a cache held in 4 bits (b200_kv4_*): 4.5 bits a value instead of 32,
+ * so seven times the positions in the same memory.  Pages of a multiple of 16
+ * positions; head dims 64 and 128; max_seqs up to
+ * B200_KV4_ATTENTION_MAX_SEQS.  Block tables and slots are kept by
+ * b200_page_step on the device; a step is rotated, written and attended to
+ * over what the cache then holds, its own new rows included. */
+int b200_batch_create_kv4(b200_model *m, int max_seqs, int page_size,
+                          int n_pages, int max_context, b200_batch **out);
 void b200_batch_destroy(b200_batch *b);
 int b200_batch_add(b200_batch *b, int *seq);
 int b200_batch_remove(b200_batch *b, int seq);
