@@ -710,7 +710,7 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
     return fail(B200_EINVAL, "kv4_attention: null pointer");
   if (a->dtype != B200_F32 && a->dtype != B200_F16 && a->dtype != B200_BF16)
     return fail(B200_EINVAL, "kv4_attention: element type %d", a->dtype);
-  if (a->rows < 0 || a->n_seqs < 1 || a->table_stride < 1 || a->q_heads < 1 || a->q_heads % c->kv_heads != 0 || (int64_t)a->table_stride * c->page > INT32_MAX - 64)
+  if (a->rows < 0 || a->n_seqs < 1 || a->table_stride < 1 || a->q_heads < 1 || a->q_heads % c->kv_heads != 0 || (int64_t)a->table_stride * c->page > 1 << 30)
     return fail(B200_EINVAL, "kv4_attention: %d rows of %d sequences, tables of %d pages, %d heads on %d", a->rows, a->n_seqs, a->table_stride, a->q_heads,
                 c->kv_heads);
   if (a->n_seqs > B200_KV4_ATTENTION_MAX_SEQS)

@@ -354,16 +354,19 @@ int b200_page_step(const b200_page_step_args *a, void *stream);
  * all can stand in one call.  q head h reads kv head h / (q_heads / kv_heads).
  *   out = softmax(scale * q K^T) V   with the values of the cache,
  * scores, sums and products with f32 accumulators, rounded to `dtype` once.
- * codes exactly.  dtype f32: q and the weights to 2^-22 of themselves; bf16 and
- * f16: q exactly (elements down to 2^-28 of their row's largest), the weights to 2^-11.  A row that sees no position is zero, and so are the rows
- * before row_start[0] and behind the last sequence's.  Positions beyond
+ * Codes count exactly.  dtype f32: q and the weights to 2^-22 of themselves.  bf16
+ * and f16: q exactly (elements down to 2^-28 of their row's largest), the weights
+ * to 2^-11; the sequences with 64 or more query vectors per kv head (rows times q
+ * heads that share it) may take the cache's values rounded to f16 as well, 2^-11
+ * each.  A row that sees no position is zero, and so are the rows before
+ * row_start[0] and behind the last sequence's.  Positions beyond
  * table_stride * page, and those whose table entry is no page of the pool, are
  * not seen.  Nothing that a row does not see (infinities and NaN included)
  * changes it.  workspace: b200_kv4_attention_workspace_bytes() bytes, 256-byte
  * aligned, zeroed once by the caller (every call leaves its counters zero);
  * calls that can overlap on the GPU need one each.  Results do not depend on what runs
  * beside them: the same inputs on the same device give the same bits.  q and out must not overlap.
- * n_seqs up to B200_KV4_ATTENTION_MAX_SEQS. */
+ * n_seqs up to B200_KV4_ATTENTION_MAX_SEQS, table_stride * page up to 2^30. */
 #define B200_KV4_ATTENTION_MAX_SEQS 4096
 typedef struct {
   const void *q;             /* [rows][q_ld], heads side by side             */

@@ -91,7 +91,7 @@ def attend(**kw):
 
 @pytest.mark.parametrize("bad", [{n: None} for n in ("q", "out", "row_start", "lens", "block_table")]
                          + [dict(dtype=3), dict(dtype=-1), dict(q_heads=0), dict(q_heads=3), dict(rows=-1), dict(n_seqs=0), dict(table_stride=0), dict(q_ld=511),
-                            dict(out_ld=100), dict(q=AT + 2), dict(out=AT + 4097, dtype=1), dict(lens=AT + 1), dict(out=AT), dict(table_stride=1 << 28)])
+                            dict(out_ld=100), dict(q=AT + 2), dict(out=AT + 4097, dtype=1), dict(lens=AT + 1), dict(out=AT), dict(table_stride=1 << 28), dict(table_stride=(1 << 26) + 1)])
 def test_attention_that_is_refused(bad):
     refused(_lib.load().b200_kv4_attention(C.byref(cache()), C.byref(attend(**bad)), AT, 1 << 40, None))
 
@@ -115,3 +115,13 @@ def test_the_allocator_model_hands_pages_round():
     p = u.Pages([3, 5, 0], [[7, -1], [2, 4], [-1, -1]], [9, 8], 4)
     assert p.step([2, -1, 6], 9, 16)[0] == 0
     assert p.held == [5, 0, 6] and p.free == [9] and p.table == [[7, 4], [2, 4], [2, 8]]
+
+
+def test_a_status_of_no_workspace():
+    refused(_lib.load().b200_kv4_attention_status(None, None))
+
+
+def test_a_batch_of_no_model():
+    out = C.c_void_p()
+    refused(_lib.load().b200_batch_create_kv4(None, 4, 16, 8, 64, C.byref(out)))
+    assert not out
