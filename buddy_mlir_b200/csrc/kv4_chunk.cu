@@ -1,10 +1,9 @@
 // Attention over the 4-bit KV cache for sequences of many rows (a chunk of a prompt, or all of it) on the 5th-generation tensor cores.
 //
 // Where many rows meet a key its 128 codes are better made values once: seven warps turn 128 keys into f16 operands (K [128][D], V
-// transposed [D][128], swizzled), two times 128 query rows are multiplied with them.  A tile of sixteen keys has a power of two of its own, so
-// that its largest value comes to 2^-8 .. 2^-7: code, scale and minimum then meet in one fma with one rounding (codes as the subnormal
-// numbers c 2^-24 and c 2^-20, the scale times 2^24 and 2^20).  K's power goes into the scores' factor, V's into the weights' exponent, whose reference
-// counts it too: weights fit f16 whatever the values are, and need no other normalisation.
+// transposed [D][128], swizzled), two times 128 query rows are multiplied with them.  A code becomes f16 by way of 1024 + c; with its group's scale and
+// minimum it meets in one fma, so with one rounding: a value of the cache is a multiple of 2^-24, where f16 ends, and half a step off above 2^-13.
+// Only a group of the whole range of f16 can reach beyond it, by its scale's rounding, to 65536: that is held at 65504.
 //
 // One thread per row does the softmax in one pass: 32 scores at a time come from tensor memory, their weights go back in their place as the A operand of
 // O += P V, which stays in tensor memory.  Where a score is more than 2^4 above the row's reference, that moves (by whole powers of two), and
@@ -39,7 +38,6 @@ template <int D> struct Shape {
 
 // What the softmax has to know of a block's keys.
 struct Notes {
-  float factor[8], height[8], unit[8];   // of a tile: of its scores; log2 of V's power of two, and that itself (inverted)
   // bits of sixteen keys, by tile: any of the next; K not finite; no page; V not finite, by group
   __align__(16) uint16_t special[8];
   uint16_t k_bad[8], hole[8], v_bad[2][8];
@@ -111,8 +109,22 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ bool finite_pair(uint32_t pair) { return (pair & 0x7c00u) != 0x7c00u && (pair & 0x7c000000u) != 0x7c000000u; }
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
-// of a tile's largest value: the power of two that brings it to 2^-8 .. 2^-7
-__device__ __forceinline__ int lift(float largest) { return min(max(119 - (int)(__float_as_uint(largest) >> 23), -40), 40); }
+// Codes of the low nibble of each byte-pair of w, and of the high one.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) {
+  uint32_t x = (w & 0x000f000fu) | 0x64006400u;                        // 1024 + c
+  asm("add.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0xe400e400u));
+  return x;
+}
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return fma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd400d400u); }   // 1024 + 16 c, / 16 - 64
+// c s + lo; HELD: within +-65504
+template <bool HELD> __device__ __forceinline__ uint32_t value2(uint32_t c, uint32_t s, uint32_t lo) {
+  uint32_t x = fma2(c, s, lo);
+  if constexpr (HELD) {
+    asm("min.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x7bff7bffu));
+    asm("max.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0xfbfffbffu));
+  }
+  return x;
+}
 
 // A CTA's share of an item: blocks b0 .. b1 - 1 of `all`.
 struct Segment {
@@ -335,46 +347,35 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
             if (c < 3)
               tmem_load32(col_s + 32 * (c + 1), s[(c + 1) & 1]);
             const uint32_t m = HIDDEN ? sees(c) : 0u, bad = HIDDEN ? Notes::word(notes.k_bad, c) & m : 0u;
-            float f[2], b[2], top = -INFINITY;
+            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              f[h] = factor * notes.factor[2 * c + h];
-              b[h] = notes.height[2 * c + h];
-              float x[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                const int k = 16 * h + e;
-                if constexpr (HIDDEN) {
-                  w[k] = m >> k & 1 ? w[k] : 0xff800000u;
-                  w[k + 1] = m >> (k + 1) & 1 ? w[k + 1] : 0xff800000u;
-                }
-                x[e / 2 & 1] = max3(x[e / 2 & 1], __uint_as_float(w[k]), __uint_as_float(w[k + 1]));
+            for (int k = 0; k < 32; k += 2) {
+              if constexpr (HIDDEN) {
+                w[k] = m >> k & 1 ? w[k] : 0xff800000u;
+                w[k + 1] = m >> (k + 1) & 1 ? w[k + 1] : 0xff800000u;
               }
-              top = fmaxf(top, fmaf(fmaxf(x[0], x[1]), f[h], b[h]));
+              x[k / 2 & 3] = max3(x[k / 2 & 3], __uint_as_float(w[k]), __uint_as_float(w[k + 1]));
             }
+            const float top = fmaxf(max3(x[0], x[1], x[2]), x[3]) * factor;
             if (__any_sync(0xffffffffu, top > r + (kKv4Top + kKv4Lag)))
               move(top, c);
             uint32_t out[16];
+            const uint64_t ff = pack2(factor, factor), rr = pack2(-r, -r);
+            uint64_t sum[2] = {};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint64_t ff = pack2(f[h], f[h]), bb = pack2(b[h] - r, b[h] - r);
-              uint64_t sum = 0;
-#pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                const int k = 16 * h + e;
-                float2 x = unpack2(fma_2(pack2(__uint_as_float(w[k]), __uint_as_float(w[k + 1])), ff, bb));
-                x.x = ex2(x.x);
-                x.y = ex2(x.y);
-                if constexpr (HIDDEN) {
-                  x.x = bad >> k & 1 ? NAN : m >> k & 1 ? x.x : 0.f;
-                  x.y = bad >> (k + 1) & 1 ? NAN : m >> (k + 1) & 1 ? x.y : 0.f;
-                }
-                sum = add_2(sum, pack2(x.x, x.y));
-                out[8 * h + e / 2] = pack_f16(x.x, x.y);
+            for (int k = 0; k < 32; k += 2) {
+              float2 x = unpack2(fma_2(pack2(__uint_as_float(w[k]), __uint_as_float(w[k + 1])), ff, rr));
+              x.x = ex2(x.x);
+              x.y = ex2(x.y);
+              if constexpr (HIDDEN) {
+                x.x = bad >> k & 1 ? NAN : m >> k & 1 ? x.x : 0.f;
+                x.y = bad >> (k + 1) & 1 ? NAN : m >> (k + 1) & 1 ? x.y : 0.f;
               }
-              const float2 both = unpack2(sum);
-              l = fmaf(both.x + both.y, notes.unit[2 * c + h], l);
+              sum[k / 2 & 1] = add_2(sum[k / 2 & 1], pack2(x.x, x.y));
+              out[k / 2] = pack_f16(x.x, x.y);
             }
+            const float2 both = unpack2(add_2(sum[0], sum[1]));
+            l += both.x + both.y;
             tmem_store16(col_s + 16 * c, out);
             if constexpr (HIDDEN)
 #pragma unroll
@@ -554,12 +555,19 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
                 f(raw.vp[u][e][gr], 2 * t + e + 8 * u, v_bad[gr]);
             }
         };
-        every([&](uint32_t &pair, int, uint32_t &) {   // (x - x is zero, but for infinities and NaN)
-          const __half2 x = *reinterpret_cast<const __half2 *>(&pair), d = __hsub2(x, x);
-          strange |= *reinterpret_cast<const uint32_t *>(&d);
-        });
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) {   // (the value of code 15, beyond f16 or nothing finite: x - x is not zero)
+          const uint32_t at[3][2] = {{raw.kp[0][gr], raw.kp[1][gr]}, {raw.vp[0][0][gr], raw.vp[0][1][gr]}, {raw.vp[1][0][gr], raw.vp[1][1][gr]}};
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            const uint32_t top = fma2(0x4b804b80u, __byte_perm(at[i][0], at[i][1], 0x5410), __byte_perm(at[i][0], at[i][1], 0x7632));
+            const __half2 x = *reinterpret_cast<const __half2 *>(&top), d = __hsub2(x, x);
+            strange |= *reinterpret_cast<const uint32_t *>(&d);
+          }
+        }
+        const bool beyond = __any_sync(0xffffffffu, strange != 0);
         bool any_bad = false;
-        if (from < 0 || key0 + kKv4Tile > most || __any_sync(0xffffffffu, strange != 0)) {
+        if (from < 0 || key0 + kKv4Tile > most || beyond) {
           every([&](uint32_t &pair, int key, uint32_t &bad) {
             const bool seen = from >= 0 && key0 + key < most;
             if (!seen || !finite_pair(pair)) {
@@ -576,30 +584,12 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
           }
           any_bad = all != 0;
         }
-        float k_most = 0.f, v_most = 0.f;
-#pragma unroll
-        for (int gr = 0; gr < GROUPS; ++gr)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float2 f = halves(raw.kp[u][gr]);
-            k_most = max3(k_most, fabsf(f.y), fabsf(fmaf(15.f, f.x, f.y)));
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float2 v = halves(raw.vp[u][e][gr]);
-              v_most = max3(v_most, fabsf(v.y), fabsf(fmaf(15.f, v.x, v.y)));
-            }
-          }
-        const int k_lift = lift(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(k_most))));
-        const int v_lift = lift(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v_most))));
         // ---- K: words of eight dims of a key
         if (block >= kStages)
           wait(ok, &bars.k_empty[stage], (block / kStages - 1) & 1, 733);
         if (lane == 0) {   // (after the wait: the block four before is done with)
           Notes &notes = bars.notes[block % kNotes];
           const uint32_t hole = from < 0 && key0 < most ? 0xffffu : 0u;
-          notes.factor[tile] = power(-k_lift);
-          notes.height[tile] = (float)-v_lift;
-          notes.unit[tile] = power(v_lift);
           notes.k_bad[tile] = (uint16_t)k_bad;
           notes.hole[tile] = (uint16_t)hole;
 #pragma unroll
@@ -609,45 +599,54 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
         }
         // (rows of K and of V^T that a lane writes are g, modulo eight)
         const uint32_t k_at = s_k + stage * H::KV_BYTES + tile * (kKv4Tile * 128), v_at = s_v + stage * H::KV_BYTES + tile / 4 * (D * 128);
-        const float one = power(k_lift), unit = power(v_lift);
+        auto make_k = [&](auto held) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int gr = 0; gr < GROUPS; ++gr) {
-            const float2 f = halves(raw.kp[h][gr]);
-            const float s = f.x * one, l = f.y * one;
-            const uint32_t low = pack_f16(s * 16777216.f, s * 16777216.f), high = pack_f16(s * 1048576.f, s * 1048576.f), lo = pack_f16(l, l);
+            for (int gr = 0; gr < GROUPS; ++gr) {
+              const uint32_t s = __byte_perm(raw.kp[h][gr], 0, 0x1010), lo = __byte_perm(raw.kp[h][gr], 0, 0x3232);
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              const uint32_t x = raw.k[h][2 * gr + w], y = x >> 8;
-              store4(k_at + gr * (kKeys * 128) + h * 1024 + (((4 * w + t) ^ gq) << 4), fma2(x & 0x000f000fu, low, lo), fma2(x & 0x00f000f0u, high, lo),
-                   fma2(y & 0x000f000fu, low, lo), fma2(y & 0x00f000f0u, high, lo));
+              for (int w = 0; w < 2; ++w) {
+                const uint32_t x = raw.k[h][2 * gr + w], y = x >> 8;
+                constexpr bool HELD = decltype(held)::value;
+                store4(k_at + gr * (kKeys * 128) + h * 1024 + (((4 * w + t) ^ gq) << 4), value2<HELD>(low_codes(x), s, lo), value2<HELD>(high_codes(x), s, lo),
+                       value2<HELD>(low_codes(y), s, lo), value2<HELD>(high_codes(y), s, lo));
+              }
             }
-          }
+        };
+        if (beyond)
+          make_k(std::true_type());
+        else
+          make_k(std::false_type());
         // ---- V: words of dims 16 w + g (+ 8) and keys 2 t, 2 t + 1 (+ 8)
         if (block >= kStages)
           wait(ok, &bars.v_empty[stage], (block / kStages - 1) & 1, 734);
         const int c = tile % 4 * 2;
+        auto make_v = [&](auto held) {
+          constexpr bool HELD = decltype(held)::value;
 #pragma unroll
-        for (int gr = 0; gr < GROUPS; ++gr) {
-          uint32_t low[2], high[2], lo[2];
+          for (int gr = 0; gr < GROUPS; ++gr) {
+            uint32_t s[2], lo[2];
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float2 a = halves(raw.vp[u][0][gr]), b = halves(raw.vp[u][1][gr]);
-            low[u] = pack_f16(a.x * unit * 16777216.f, b.x * unit * 16777216.f);
-            high[u] = pack_f16(a.x * unit * 1048576.f, b.x * unit * 1048576.f);
-            lo[u] = pack_f16(a.y * unit, b.y * unit);
+            for (int u = 0; u < 2; ++u) {
+              s[u] = __byte_perm(raw.vp[u][0][gr], raw.vp[u][1][gr], 0x5410);
+              lo[u] = __byte_perm(raw.vp[u][0][gr], raw.vp[u][1][gr], 0x7632);
+            }
+#pragma unroll
+            for (int w = 4 * gr; w < 4 * gr + 4; ++w) {
+              const uint32_t x = raw.v[w], y = x >> 8;
+              const uint32_t to0 = v_at + w * 2048 + ((c ^ gq) << 4), to1 = v_at + w * 2048 + (((c + 1) ^ gq) << 4);
+              store1(to0, value2<HELD>(low_codes(x), s[0], lo[0]));
+              store1(to0 + 1024, value2<HELD>(high_codes(x), s[0], lo[0]));
+              store1(to1, value2<HELD>(low_codes(y), s[1], lo[1]));
+              store1(to1 + 1024, value2<HELD>(high_codes(y), s[1], lo[1]));
+            }
           }
-#pragma unroll
-          for (int w = 4 * gr; w < 4 * gr + 4; ++w) {
-            const uint32_t x = raw.v[w], y = x >> 8;
-            const uint32_t to0 = v_at + w * 2048 + ((c ^ gq) << 4), to1 = v_at + w * 2048 + (((c + 1) ^ gq) << 4);
-            store1(to0, fma2(x & 0x000f000fu, low[0], lo[0]));
-            store1(to0 + 1024, fma2(x & 0x00f000f0u, high[0], lo[0]));
-            store1(to1, fma2(y & 0x000f000fu, low[1], lo[1]));
-            store1(to1 + 1024, fma2(y & 0x00f000f0u, high[1], lo[1]));
-          }
-        }
+        };
+        if (beyond)
+          make_v(std::true_type());
+        else
+          make_v(std::false_type());
         fence_proxy();
         __syncwarp();
         if (lane == 0) {

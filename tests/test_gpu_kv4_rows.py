@@ -58,6 +58,28 @@ def test_one_group_of_one_head_that_is_not_finite(kind, which):
         assert after[:, :, :64].isfinite().all()
 
 
+def rewrite(b, s, j, x):
+    """Position j of sequence s holds x [kv heads, D] instead, in K and V."""
+    row = dev(np.ascontiguousarray(x, np.float32).reshape(1, -1))
+    u.write(b.cache, row, row, "f32", dev(np.array([slot(b, s, j)], np.int64)))
+    b.host.pool = b.pool.cpu().numpy()
+
+
+@KINDS
+@pytest.mark.parametrize("size", [1e-6, 1.0, 3e3, np.inf])
+def test_how_large_a_key_is_changes_no_row_that_does_not_see_it(kind, size):
+    """A position of other magnitude than the fifteen beside it, up to f16's whole range (where a group's scale rounds beyond it)."""
+    b = Batch([301], [90], 6, 2, 64, 16, kind, 47)
+    before = b.run().clone().reshape(90, 6, 64)
+    x = np.where(b.rng.standard_normal((2, 64)) < 0, -1.0, 1.0)
+    rewrite(b, 0, 250, np.where(x < 0, -size, size) if size == np.inf else x * size * (1 + b.rng.random((2, 64))))
+    assert (b.run().reshape(90, 6, 64)[:39] == before[:39]).all()         # (row 39 is the first to see it)
+    b.scale = 2.0 ** -20 if size > 1 else b.scale
+    if kind == "f16" and size == np.inf:
+        return                                                            # (65536 is no f16)
+    b.check(every=3)
+
+
 @KINDS
 def test_pages_outside_the_pool_are_not_seen(kind):
     b = Batch([170, 100, 40], [70, 64, 40], 4, 2, 128, 16, kind, 32)
