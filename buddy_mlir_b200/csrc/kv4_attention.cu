@@ -9,6 +9,10 @@
 //
 // The reference r of a row's weights is not its largest score but the largest of score + log2 of the key's larger V scale, so that the weights
 // that meet codes, p s, are at most 2^12 and near 2^8 where they count, whatever the scales are; sums and totals carry the same factor.
+//
+// Sixteen warps of a CTA share an item's tiles, each with four tiles on their way (cp.async), and join in shared memory.  64 rows of 2000 to 4096 keys, 32
+// heads on 8 of 128 dims, bf16: 62 us, 3.7 TB/s, 0.56 of a copy's rate.  A tile is some 290 instructions of a warp, 114 clocks of an SM; issue slots are
+// half full and the tensor pipe a quarter, so chains of latencies bound it at four warps a scheduler (128 registers a thread: q, sums and two tiles).
 #include "kv4_plan.cuh"
 
 #include <algorithm>
