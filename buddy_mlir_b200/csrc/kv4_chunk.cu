@@ -1,6 +1,6 @@
 // Attention over the 4-bit KV cache for sequences of many rows (a chunk of a prompt, or all of it) on the 5th-generation tensor cores.
 //
-// Where many rows meet a key its 128 codes are better made values once: seven warps turn 128 keys into f16 operands (K [128][D], V
+// Where many rows meet a key its 128 codes are better made values once: six warps turn 128 keys into f16 operands (K [128][D], V
 // transposed [D][128], swizzled), two times 128 query rows are multiplied with them.  A code becomes f16 by way of 1024 + c; with its group's scale and
 // minimum it meets in one fma, so with one rounding: a value of the cache is a multiple of 2^-24, where f16 ends, and half a step off above 2^-13.
 // Only a group of the whole range of f16 can reach beyond it, by its scale's rounding, to 65536: that is held at 65504.
@@ -11,10 +11,9 @@
 // Two sets of 128 rows take turns: one's products run under the other's softmax.  (S 2 x 128 columns, O 2 x D.)
 // A key's values that are not finite are zero in the operands, and what sees them becomes NaN afterwards: nothing reaches rows that do not.
 //
-// 1001 rows at 4000 keys, 32 heads on 8 of 128 dims, bf16: 123 us, 468 TFLOP/s, 0.28 of a dense product's rate.  A block of 128 keys takes an SM 7000 clocks,
+// 1001 rows at 4000 keys, 32 heads on 8 of 128 dims, bf16: 120 us, 479 TFLOP/s, 0.29 of a dense product's rate.  A block of 128 keys takes an SM 7000 clocks,
 // 1500 of them for its products: a set's softmax (3400) and the way of its weights through both products (2400) follow each other.
-#include "kv4_plan.cuh"
-#include "tensor_core.cuh"
+#include "kv4_rows.cuh"
 
 #include <algorithm>
 #include <type_traits>
@@ -23,10 +22,8 @@ namespace b200 {
 
 namespace {
 
-constexpr int kRows = 128, kSets = 2;               // query rows of a set
-constexpr int kKeys = 128, kShift = 7;              // of a block
-constexpr int kTiles = kKeys / kKv4Tile;            // of a block
-constexpr int kSoftmaxWarps = 4 * kSets, kMakers = 7, kThreads = 32 * (kSoftmaxWarps + kMakers + 1);
+constexpr int kSets = 2;                            // of kRows
+constexpr int kSoftmaxWarps = 4 * kSets, kMakers = 6, kThreads = 32 * (kSoftmaxWarps + kMakers + 1);
 constexpr int kStages = 2, kNotes = 4;
 constexpr uint32_t kCols = 512;
 constexpr int kLeastKeys = 256;
@@ -34,7 +31,7 @@ constexpr int kLeastKeys = 256;
 template <int D> struct Shape {
   static constexpr int GROUPS = D / kKv4Group, BYTES = kv4_tile_bytes(D);
   static constexpr uint32_t Q_BYTES = kRows * D * 2, KV_BYTES = kKeys * D * 2;
-  static constexpr int PART = kSets * kRows * (D + 2 + GROUPS);   // floats: sums [D / 4][rows][4], references, totals, marks
+  static constexpr int PART = rows_part<D, kSets * kRows>();
   static constexpr int SMEM = 1024 + kSets * Q_BYTES + 2 * kStages * KV_BYTES;
   static constexpr uint32_t COL_S = 0, COL_O = kSets * kKeys;
 };
@@ -49,69 +46,12 @@ struct Notes {
 struct Bars {
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[kSets], p_ready[kSets], o_full[kSets], q_full[kSets];
   uint32_t tmem_base;
-  int abort_flag, last, from, to;
+  int abort_flag;
+  Meeting meeting;
   long long sums[2 * (kThreads / 32) + 1];
   Notes notes[kNotes];
 };
 
-// kind::f16 instruction descriptor: D = f32, A = B = f16, both K-major, M = 128.
-template <int N> __host__ __device__ constexpr uint32_t idesc() {
-  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-}
-// Executed by a whole warp in uniform control flow, issued by the lane whose `leader` is set.
-template <int N> __device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, l;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 l, %5, 0;\n"
-      " @l tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc<N>()), "r"(accumulate), "r"(leader)
-      : "memory");
-}
-template <int N> __device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, l;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 l, %5, 0;\n"
-      " @l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc<N>()), "r"(accumulate), "r"(leader)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&v)[32]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
-               "%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
-               "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
-               "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-               : "memory");
-}
-// (the values are there after the wait, and the compiler takes them from it)
-__device__ __forceinline__ void tmem_arrived(uint32_t (&v)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
-                 "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]),
-                 "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]),
-                 "+r"(v[31])
-               :
-               : "memory");
-}
-__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// (Operands in shared memory: rows of 128 bytes, 128-byte swizzle: 16-byte chunk c of row r lies at chunk c ^ (r & 7).)
-__device__ __forceinline__ void store4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {   // (an address in shared memory)
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-__device__ __forceinline__ void store1(uint32_t at, uint32_t a) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(a) : "memory"); }
-__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-__device__ __forceinline__ bool finite_pair(uint32_t pair) { return (pair & 0x7c00u) != 0x7c00u && (pair & 0x7c000000u) != 0x7c000000u; }
-__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 // Codes of the low nibble of each byte-pair of w, and of the high one.
 __device__ __forceinline__ uint32_t low_codes(uint32_t w) {
   uint32_t x = (w & 0x000f000fu) | 0x64006400u;                        // 1024 + c
@@ -128,59 +68,6 @@ template <bool HELD> __device__ __forceinline__ uint32_t value2(uint32_t c, uint
   }
   return x;
 }
-
-// A CTA's share of an item: blocks b0 .. b1 - 1 of `all`.
-struct Segment {
-  Place at;
-  int b0, b1, all;
-  int first, tokens;      // the item's positions
-  int base;               // of the sequence
-  int r0;
-};
-// The segments of a CTA, in order; every role walks them by itself.
-struct Walk {
-  Place at, stop;
-  bool over;
-  __device__ __forceinline__ Walk(const KeyPlan<kShift, 1200> &plan) {
-    const int lane = threadIdx.x & 31;
-    const long long x = plan.border(blockIdx.x + min(lane, 1));
-    over = __shfl_sync(0xffffffffu, x, 0) == __shfl_sync(0xffffffffu, x, 1);
-    at = Place{plan.n, 0, 0, 0};
-    if (x < plan.total)
-      at = plan.locate(x);
-    stop.s = __shfl_sync(0xffffffffu, at.s, 1);
-    stop.slot = __shfl_sync(0xffffffffu, at.slot, 1);
-    stop.rt = __shfl_sync(0xffffffffu, at.rt, 1);
-    stop.tile = __shfl_sync(0xffffffffu, at.tile, 1);
-    at.s = __shfl_sync(0xffffffffu, at.s, 0);
-    at.slot = __shfl_sync(0xffffffffu, at.slot, 0);
-    at.rt = __shfl_sync(0xffffffffu, at.rt, 0);
-    at.tile = __shfl_sync(0xffffffffu, at.tile, 0);
-  }
-  __device__ __forceinline__ bool next(const KeyPlan<kShift, 1200> &plan, Segment &g) {
-    while (!over && at.s < plan.n) {
-      const Sequence q = plan.sequence(at.s);
-      g.all = plan.item_tiles(q, at.rt);
-      const bool here = stop.s == at.s && stop.slot == at.slot && stop.rt == at.rt;
-      if (at.tile >= g.all && !here) {
-        plan.next_item(at, q);
-        continue;
-      }
-      g.at = at;
-      g.b0 = at.tile;
-      g.b1 = here ? min(stop.tile, g.all) : g.all;
-      g.first = at.rt * plan.tokens;
-      g.tokens = min(plan.tokens, q.n - g.first);
-      g.base = q.base;
-      g.r0 = q.r0;
-      over = here;
-      if (!here)
-        plan.next_item(at, q);
-      return g.b0 < g.b1;
-    }
-    return false;
-  }
-};
 
 template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_constant__ Kv4Params p) {
   using H = Shape<D>;
@@ -220,7 +107,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
   kernel_go();   // not before the allocation: see tensor_core.cuh
   kernel_wait();
   const int room = p.a.table_stride * p.page;
-  KeyPlan<kShift, 1200> plan;
+  RowsPlan plan;
   plan.build<kThreads>(p, s_plan, bars.sums, kLeastKeys);
   if (p.fill) {
     const int lo = plan.r0[0], hi = max(lo, plan.r0[plan.n]), none = lo + p.a.rows - hi, cols = p.a.q_heads * D;
@@ -402,14 +289,6 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
       float *part = p.parts + ((int64_t)blockIdx.x * 2 + (g.b0 == 0)) * H::PART;
       const int at = set * kRows + row;
       const int64_t to = live ? row_at(p, g.r0 + g.first + set * half, g.at.slot, row, p.a.out_ld, D) : 0;
-      auto write_out = [&](int d, const float (&o)[4], float total, const bool (&nan)[GROUPS]) {
-        const float over = total == 0.f ? 0.f : 1.f / total;
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          x[e] = nan[d / kKv4Group] ? NAN : total == 0.f ? 0.f : o[e] * over;
-        put4<TYPE>(p, to + d, make_float4(x[0], x[1], x[2], x[3]));
-      };
       if (any) {
         wait(ok, &bars.o_full[set], segments & 1, 732);
         ++segments;
@@ -424,7 +303,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
             for (int e = 0; e < 32; e += 4) {
               const float o[4] = {__uint_as_float(w[e]), __uint_as_float(w[e + 1]), __uint_as_float(w[e + 2]), __uint_as_float(w[e + 3])};
               if (whole)
-                write_out(c + e, o, l, marks);
+                put_over<TYPE>(p, to + c + e, o, l, marks[(c + e) / kKv4Group]);
               else
                 __stcg(reinterpret_cast<float4 *>(part) + (c + e) / 4 * (kSets * kRows) + at, make_float4(o[0], o[1], o[2], o[3]));
             }
@@ -440,60 +319,11 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
             rest[(2 + gr) * kSets * kRows + at] = marks[gr] ? 1.f : 0.f;
         }
       }
-      if (whole)
-        continue;
-      __threadfence();
-      asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
-      if (warp == 0) {
-        int from, until;
-        const bool last = plan.arrive(p.counters, g.at, g.b1 - g.b0, from, until);
-        if (lane == 0) {
-          bars.last = last;
-          bars.from = from;
-          bars.to = until;
-        }
-      }
-      asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxWarps * 32) : "memory");
-      if (!bars.last || !live)
-        continue;
-      __threadfence();
-      const int from = bars.from, until = bars.to;
-      auto other = [&](int b) { return p.parts + ((int64_t)b * 2 + (b == from)) * H::PART; };
-      auto rest = [&](int b, int i) { return __ldcg(other(b) + kSets * kRows * (D + i) + at); };
-      float top = kKv4Seed, total = 0.f;
-      bool nan[GROUPS] = {};
-#pragma unroll 4
-      for (int b = from; b <= until; ++b)
-        top = fmaxf(top, rest(b, 0));
-#pragma unroll 2
-      for (int b = from; b <= until; ++b) {
-        total = fmaf(rest(b, 1), ex2(rest(b, 0) - top), total);
-#pragma unroll
-        for (int gr = 0; gr < GROUPS; ++gr)
-          nan[gr] = nan[gr] || rest(b, 2 + gr) != 0.f;
-      }
-#pragma unroll 1
-      for (int d = 0; d < D; d += 32) {
-        float o[8][4] = {};
-#pragma unroll 2
-        for (int b = from; b <= until; ++b) {
-          const float f = ex2(rest(b, 0) - top);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(other(b)) + (d / 4 + i) * (kSets * kRows) + at);
-            o[i][0] = fmaf(v.x, f, o[i][0]);
-            o[i][1] = fmaf(v.y, f, o[i][1]);
-            o[i][2] = fmaf(v.z, f, o[i][2]);
-            o[i][3] = fmaf(v.w, f, o[i][3]);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          write_out(d + 4 * i, o[i], total, nan);
-      }
+      if (!whole)
+        meet<D, TYPE, kSets * kRows, 32 * kSoftmaxWarps>(p, plan, g, bars.meeting, at, live, to);
     }
   } else if (works && warp < kSoftmaxWarps + kMakers) {
-    // ---- makers: every seventh tile each -------------------------------------------------------------------------------------------
+    // ---- makers: every sixth tile each -------------------------------------------------------------------------------------------
     const int mw = warp - kSoftmaxWarps, gq = lane >> 2, t = lane & 3;
     const uint32_t s_k = smem_u32(ks) + gq * 128, s_v = smem_u32(vs) + gq * 128 + 4 * t;
     struct Raw {
@@ -743,9 +573,9 @@ RaisedOn g_raised[4];
 constexpr int kMostSeqs = 1500;   // whose plan fits beside the operands
 
 template <int D, int TYPE> int chunk_launch(RaisedOn &raised, const Kv4Params &p, cudaStream_t st) {
-  if (int rc = raise_shared_limit(raised, (const void *)kv4_chunk_kernel<D, TYPE>, Shape<D>::SMEM + KeyPlan<kShift, 1200>::bytes(kMostSeqs)))
+  if (int rc = raise_shared_limit(raised, (const void *)kv4_chunk_kernel<D, TYPE>, Shape<D>::SMEM + RowsPlan::bytes(kMostSeqs)))
     return rc;
-  return launch_after(kv4_chunk_kernel<D, TYPE>, dim3(kKv4Ctas), kThreads, Shape<D>::SMEM + KeyPlan<kShift, 1200>::bytes(p.a.n_seqs), st, p);
+  return launch_after(kv4_chunk_kernel<D, TYPE>, dim3(kKv4Ctas), kThreads, Shape<D>::SMEM + RowsPlan::bytes(p.a.n_seqs), st, p);
 }
 
 } // namespace
