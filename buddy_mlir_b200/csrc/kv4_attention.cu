@@ -25,7 +25,7 @@ constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr int kRows = 8;            // query rows of an item: a position's heads (several positions', if they are few)
 constexpr int kSlots = 4;           // tiles that a warp has in flight or in hand
 constexpr int kChunkRows = 64;     // query vectors of a sequence and kv head from which on tcgen05 has them
-constexpr int kLeastKeys = 512;     // of a CTA, where there are not more CTAs than that asks for
+constexpr int kLeastKeys = 512, kSplit = 1000;     // of a CTA, where there are not more CTAs than that asks for
 constexpr float kLeastScale = 5.9604645e-8f;   // (f16's smallest: a group of equal values has the scale 0)
 
 __host__ __device__ constexpr int part_floats(int D) { return kRows * (D + 4) + 2 * kRows; }   // sums in rows of D + 4, maxima, totals
@@ -384,8 +384,8 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_at
     s_left[warp].has_a = s_left[warp].has_b = false;
   if (tid < 2)
     s_ctas[tid][0] = 0;
-  KeyPlan<4, 1000> plan;
-  plan.build<kThreads>(p, s_all + kWarps * RING, s_sum, kLeastKeys);
+  KeyPlan<4> plan;
+  plan.build<kThreads>(p, s_all + kWarps * RING, s_sum, kLeastKeys, kSplit);
   // rows of no sequence
   if (p.fill) {
     const int lo = plan.r0[0], hi = max(lo, plan.r0[n]), none = lo + p.a.rows - hi, cols = p.a.q_heads * D;
@@ -677,9 +677,9 @@ RaisedOn g_raised[6];
 
 template <int D, int TYPE> int attention_launch(RaisedOn &raised, const Kv4Params &p, cudaStream_t st) {
   const int fixed = kWarps * kSlots * kv4_tile_bytes(D);
-  if (int rc = raise_shared_limit(raised, (const void *)kv4_attention_kernel<D, TYPE>, fixed + KeyPlan<4, 1000>::bytes(B200_KV4_ATTENTION_MAX_SEQS)))
+  if (int rc = raise_shared_limit(raised, (const void *)kv4_attention_kernel<D, TYPE>, fixed + KeyPlan<4>::bytes(B200_KV4_ATTENTION_MAX_SEQS)))
     return rc;
-  return launch_after(kv4_attention_kernel<D, TYPE>, dim3(kKv4Ctas), kThreads, fixed + KeyPlan<4, 1000>::bytes(p.a.n_seqs), st, p);
+  return launch_after(kv4_attention_kernel<D, TYPE>, dim3(kKv4Ctas), kThreads, fixed + KeyPlan<4>::bytes(p.a.n_seqs), st, p);
 }
 
 } // namespace
@@ -758,7 +758,8 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
   cudaStream_t st = (cudaStream_t)stream;
   // Sequences of many rows go to tcgen05, in a launch of their own; who has how many rows is known on the device only, so both launches are made where
   // the mean does not say that there are none of one kind.
-  if (kv4_chunk_takes(a->dtype, p.G, a->n_seqs) && (int64_t)a->rows * p.G >= kChunkRows && (int64_t)a->rows * p.G >= 24 * (int64_t)a->n_seqs) {
+  const bool exact = a->dtype == B200_F32;
+  if ((exact ? kv4_exact_takes(p.G, a->n_seqs) : kv4_chunk_takes(p.G, a->n_seqs)) && (int64_t)a->rows * p.G >= kChunkRows && (int64_t)a->rows * p.G >= 24 * (int64_t)a->n_seqs) {
     const int from = (kChunkRows + p.G - 1) / p.G;
     Kv4Params chunk = p;
     if (a->n_seqs > 1) {
@@ -766,7 +767,7 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
       chunk.least_rows = from;
       chunk.fill = 0;
     }
-    if (int rc = kv4_chunk_launch(chunk, c->head_dim, st))
+    if (int rc = exact ? kv4_exact_launch(chunk, c->head_dim, st) : kv4_chunk_launch(chunk, c->head_dim, st))
       return rc;
     if (a->n_seqs == 1)
       return B200_OK;

@@ -26,7 +26,7 @@ constexpr int kSets = 2;                            // of kRows
 constexpr int kSoftmaxWarps = 4 * kSets, kMakers = 6, kThreads = 32 * (kSoftmaxWarps + kMakers + 1);
 constexpr int kStages = 2, kNotes = 4;
 constexpr uint32_t kCols = 512;
-constexpr int kLeastKeys = 256;
+constexpr int kLeastKeys = 256, kSplit = 1200;
 
 template <int D> struct Shape {
   static constexpr int GROUPS = D / kKv4Group, BYTES = kv4_tile_bytes(D);
@@ -108,7 +108,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
   kernel_wait();
   const int room = p.a.table_stride * p.page;
   RowsPlan plan;
-  plan.build<kThreads>(p, s_plan, bars.sums, kLeastKeys);
+  plan.build<kThreads>(p, s_plan, bars.sums, kLeastKeys, kSplit);
   if (p.fill) {
     const int lo = plan.r0[0], hi = max(lo, plan.r0[plan.n]), none = lo + p.a.rows - hi, cols = p.a.q_heads * D;
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)none * cols; i += (int64_t)gridDim.x * kThreads) {
@@ -228,14 +228,11 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
         };
         auto weigh = [&](auto hidden) {
           constexpr bool HIDDEN = decltype(hidden)::value;
-          uint32_t s[2][32];
-          tmem_load32(col_s, s[0]);
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            uint32_t (&w)[32] = s[c & 1];
+            uint32_t w[32];
+            tmem_load32(col_s + 32 * c, w);
             tmem_arrived(w);
-            if (c < 3)
-              tmem_load32(col_s + 32 * (c + 1), s[(c + 1) & 1]);
             const uint32_t m = HIDDEN ? sees(c) : 0u, bad = HIDDEN ? Notes::word(notes.k_bad, c) & m : 0u;
             float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -582,7 +579,7 @@ template <int D, int TYPE> int chunk_launch(RaisedOn &raised, const Kv4Params &p
 
 int64_t kv4_chunk_part_floats(int D) { return 2 * (D == 128 ? Shape<128>::PART : Shape<64>::PART); }
 
-bool kv4_chunk_takes(int dtype, int G, int n_seqs) { return (dtype == B200_F16 || dtype == B200_BF16) && G <= kRows && n_seqs <= kMostSeqs; }
+bool kv4_chunk_takes(int G, int n_seqs) { return G <= kRows && n_seqs <= kMostSeqs; }
 
 int kv4_chunk_launch(Kv4Params p, int D, cudaStream_t st) {
   p.heads = p.G;

@@ -1,0 +1,674 @@
+// Attention over the 4-bit KV cache for sequences of many f32 rows (a prompt, or a chunk of one) on the 5th-generation tensor cores.
+//
+// Products of f32's accuracy out of f16 operands: q and the weights are two f16 terms each (22 bits, after a power of two of the row), and so is what is left
+// of a value once it is centred.  With v = (c - 8) s + m, m = lo + 8 s,
+//   q.k = sum over dims of q (c - 8) s + sum over groups of m (sum of q)       sum p v = sum p (c - 8) s + sum p m:
+// (c - 8) s has 15 bits at most, so that its rounding to f16 and what that leaves are two terms without any error, made by a product and an fma; the parts with m
+// are a few f32 operations of the thread that has the row.  Three of the four products of terms are summed, the small ones first; centred sums stay
+// small, which matters because the tensor cores' sums round towards zero.
+//
+// Eight warps make the operands of 128 keys, a tile of sixteen each: K of a block while the softmax has the one before it, then V when that block's product
+// is done.  Four warps do the softmax, a thread per row, as in kv4_chunk.cu; scores of two blocks have their own columns (2 x 128, and D for O).
+//
+// A prompt of 1000 rows, 12 heads on 2 of 128 dims: 51 us (the few-rows form 70): 96 items on as many CTAs, the longest of eight blocks, and a block takes 6700 clocks,
+// 6200 of them the softmax at one warp a scheduler, 2300 the products.  Items that CTAs share come together too slowly to be worth it (78 us).
+#include "kv4_rows.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace b200 {
+
+namespace {
+
+constexpr int kSoftmaxWarps = 4, kMakers = kTiles, kThreads = 32 * (kSoftmaxWarps + kMakers + 1);
+constexpr int kNotes = 4;
+constexpr uint32_t kCols = 512;
+constexpr int kLeastKeys = 256, kSplit = 1200;
+
+template <int D> struct Shape {
+  static constexpr int GROUPS = D / kKv4Group, BYTES = kv4_tile_bytes(D);
+  static constexpr uint32_t TERM = kRows * D * 2;   // bytes of a term of q, K or V
+  static constexpr int PART = rows_part<D, kRows>();
+  static constexpr int SMEM = 1024 + 6 * TERM;
+  static constexpr uint32_t COL_S = 0, COL_O = 2 * kKeys;
+};
+
+// What the softmax has to know of a block's keys.
+struct Notes {
+  __align__(16) float k_mid[2][kKeys], v_mid[2][kKeys];   // m, by group
+  // bits of sixteen keys, by tile: any of the next; K not finite; no page; V not finite, by group
+  __align__(16) uint16_t special[8];
+  uint16_t k_bad[8], hole[8], v_bad[2][8];
+  __device__ __forceinline__ static uint32_t word(const uint16_t *x, int c) { return reinterpret_cast<const uint32_t *>(x)[c]; }   // of keys 32 c ..
+};
+struct Bars {
+  uint64_t k_full, v_full, s_full[2], p_ready[2], pv_done, q_full;
+  uint32_t tmem_base;
+  int abort_flag;
+  Meeting meeting;
+  long long sums[2 * (kThreads / 32) + 1];
+  Notes notes[kNotes];
+};
+
+// c - 8 of the low nibble of each byte-pair of w, and of the high one
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) {
+  uint32_t x = (w & 0x000f000fu) | 0x64006400u;                        // 1024 + c
+  asm("add.rn.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0xe408e408u));
+  return x;
+}
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return fma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u); }   // 1024 + 16 c, / 16 - 72
+// c s as two terms; HELD: the first within +-65504
+template <bool HELD> __device__ __forceinline__ void terms(uint32_t c, uint32_t s, uint32_t &high, uint32_t &low) {
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(high) : "r"(c), "r"(s));
+  if constexpr (HELD) {
+    asm("min.f16x2 %0, %0, %1;" : "+r"(high) : "r"(0x7bff7bffu));
+    asm("max.f16x2 %0, %0, %1;" : "+r"(high) : "r"(0xfbfffbffu));
+  }
+  low = fma2(c, s, high ^ 0x80008000u);
+}
+
+template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel(const __grid_constant__ Kv4Params p) {
+  using H = Shape<D>;
+  constexpr int GROUPS = H::GROUPS;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t *qs = reinterpret_cast<uint8_t *>(((uintptr_t)smem + 1023) & ~(uintptr_t)1023);
+  uint8_t *ks = qs + 2 * H::TERM, *vs = ks + 2 * H::TERM, *s_plan = vs + 2 * H::TERM;   // (the larger terms, then the smaller ones)
+  __shared__ Bars bars;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  volatile int *ab = &bars.abort_flag;
+  int *error = p.counters + kKv4Ctas;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars.k_full, kMakers);
+    mbar_init(&bars.v_full, kMakers);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_ready[i], kSoftmaxWarps);
+    }
+    mbar_init(&bars.pv_done, 1);
+    mbar_init(&bars.q_full, kSoftmaxWarps);
+    bars.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kSoftmaxWarps + kMakers) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)), "n"(kCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars.tmem_base, 0);
+  kernel_go();   // not before the allocation: see tensor_core.cuh
+  kernel_wait();
+  const int room = p.a.table_stride * p.page;
+  RowsPlan plan;
+  plan.build<kThreads>(p, s_plan, bars.sums, kLeastKeys, kSplit);
+  if (p.fill) {
+    const int lo = plan.r0[0], hi = max(lo, plan.r0[plan.n]), none = lo + p.a.rows - hi, cols = p.a.q_heads * D;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)none * cols; i += (int64_t)gridDim.x * kThreads) {
+      const int r = (int)(i / cols);
+      put<B200_F32>(p, (int64_t)(r < lo ? r : hi + r - lo) * p.a.out_ld + i % cols, 0.f);
+    }
+  }
+  const bool works = plan.total > 0 && (int)blockIdx.x < plan.ctas;
+  auto wait = [&](bool &ok, uint64_t *bar, uint32_t parity, int code) {   // whole warps leave the poll; who gave up goes on without waiting
+    if (ok)
+      ok = __all_sync(0xffffffffu, mbar_wait(bar, parity & 1, ab, error, code));
+  };
+
+  if (works && warp < kSoftmaxWarps) {
+    // ---- softmax: a thread per row --------------------------------------------------------------------------------------------
+    const int row = warp * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16), col_o = lanes + H::COL_O;
+    bool ok = true;
+    uint32_t made = 0;
+    Walk walk(plan);
+    Segment g;
+    while (walk.next(plan, g)) {
+      const uint32_t n = g.b1 - g.b0;
+      float r = kKv4Seed, l = 0.f, factor, sum_q[GROUPS] = {};
+      uint64_t bias[GROUPS] = {};               // sums of p m, over even and odd keys
+      bool marks[GROUPS] = {};                  // V groups that become NaN
+      const int token = row / p.G;
+      const bool live = token < min(g.tokens, p.tokens);
+      const int seen_by = live ? clamp((long long)g.base + g.first + token + 1, 0, room) : 0;
+      {
+        // ---- q: times a power of two, as two f16
+        // (row by row, four dims a lane)
+        constexpr int LANES = D / 4;              // of a row
+        const int64_t mine = live ? row_at(p, g.r0 + g.first, g.at.slot, row, p.a.q_ld, D) : -1;
+        const int d = 4 * (lane % LANES);
+        factor = 0.f;
+        constexpr int BATCH = 16;
+        float batch[BATCH][4];
+        auto fetch = [&](int i, float (&x)[4]) {
+          const int64_t at = __shfl_sync(0xffffffffu, mine, 32 / LANES * i + lane / LANES);
+          const float *q = (const float *)p.a.q + max(at, (int64_t)0) + d;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[e] = 0.f;
+          if (at >= 0 && p.wide_q)
+            *reinterpret_cast<float4 *>(x) = __ldg(reinterpret_cast<const float4 *>(q));
+          else if (at >= 0)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x[e] = __ldg(q + e);
+        };
+#pragma unroll 1
+        for (int from = 0; from < LANES; from += BATCH) {   // (of 64 dims: two rows at once)
+          float most[BATCH], sum[BATCH];
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b)
+            fetch(from + b, batch[b]);
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) {
+            const float (&x)[4] = batch[b];
+            most[b] = max3(fmaxf(fabsf(x[0]), fabsf(x[1])), fabsf(x[2]), fabsf(x[3]));
+            sum[b] = (x[0] + x[1]) + (x[2] + x[3]);
+          }
+#pragma unroll
+          for (int o = 1; o < LANES; o <<= 1)   // (all rows' steps side by side)
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b)
+              most[b] = fmaxf(most[b], __shfl_xor_sync(0xffffffffu, most[b], o));
+#pragma unroll
+          for (int o = 1; o < 16; o <<= 1)
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b)
+              sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], o);
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) {
+            const float (&x)[4] = batch[b];
+            const int up = min(max(14 + 127 - (int)(__float_as_uint(most[b]) >> 23), -113), 100), r0 = warp * 32 + 32 / LANES * (from + b) + lane / LANES;
+            const float by = power(up);
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr) {   // (the lane that has this row)
+              const float s = __shfl_sync(0xffffffffu, sum[b], GROUPS == 2 ? 16 * gr : lane % 2 * 16);
+              sum_q[gr] = lane / (32 / LANES) == from + b ? s * p.log2_scale : sum_q[gr];
+            }
+            const float unit = __shfl_sync(0xffffffffu, power(-up), GROUPS == 2 ? 0 : lane % 2 * 16);
+            factor = lane / (32 / LANES) == from + b ? unit : factor;
+            const float a[4] = {x[0] * by, x[1] * by, x[2] * by, x[3] * by};
+            const uint32_t high[2] = {pack_f16(a[0], a[1]), pack_f16(a[2], a[3])};
+            const float2 f = halves(high[0]), h = halves(high[1]);
+            const uint32_t to = smem_u32(qs) + r0 * 128 + d / 64 * (kRows * 128) + ((d / 8 % 8 ^ (r0 & 7)) << 4) + d % 8 * 2;
+            store2(to, high[0], high[1]);
+            store2(to + H::TERM, pack_f16(a[0] - f.x, a[1] - f.y), pack_f16(a[2] - h.x, a[3] - h.y));
+          }
+        }
+        factor *= p.log2_scale;
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr)
+          if (!(sum_q[gr] - sum_q[gr] == 0.f))   // (a row with an infinity, or NaN, has no scores)
+            factor = NAN;
+        fence_proxy();
+        fence_before();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&bars.q_full);
+      }
+      for (uint32_t j = 0; j < n; ++j) {
+        const uint32_t block = made + j, col_s = lanes + H::COL_S + (block & 1) * kKeys;
+        const int key0 = (g.b0 + j) * kKeys, seen = min(max(seen_by - key0, 0), kKeys);   // keys of the block that this row sees
+        wait(ok, &bars.s_full[block & 1], block >> 1, 741);
+        fence_after();
+        // (the makers wrote them before the products that have been waited for could begin; another block's come four blocks later)
+        const Notes &notes = bars.notes[block % kNotes];
+        const uint4 any_special = *reinterpret_cast<const uint4 *>(notes.special);
+        const bool special = (any_special.x | any_special.y | any_special.z | any_special.w) != 0;
+        const bool masked = special || __any_sync(0xffffffffu, live && seen < kKeys);
+        auto sees = [&](int c) {   // of keys 32 c ..: a bit each
+          const int k = seen - 32 * c;
+          return (k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1) & ~Notes::word(notes.hole, c);
+        };
+        // a row's reference moves, at the keys 32 c and on
+        auto move = [&](float top, int c) {
+          const bool moves = top > r + (kKv4Top + kKv4Lag);
+          const float to = moves ? ceilf(top) - kKv4Top : r, keep = ex2(r - to);   // (each row for itself)
+          r = to;
+          l *= keep;
+#pragma unroll
+          for (int gr = 0; gr < GROUPS; ++gr)
+            bias[gr] = mul_2(bias[gr], pack2(keep, keep));
+          auto times = [&](uint32_t at, bool pairs) {
+            uint32_t w[32];
+            tmem_load32(at, w);
+            tmem_arrived(w);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (pairs) {
+                const float2 x = halves(w[e]);
+                w[e] = pack_f16(x.x * keep, x.y * keep);
+              } else {
+                w[e] = __float_as_uint(__uint_as_float(w[e]) * keep);
+              }
+            tmem_store32(at, w);
+          };
+          if (j > 0) {
+            wait(ok, &bars.pv_done, block - 1, 742);
+            fence_after();
+#pragma unroll 1
+            for (int i = 0; i < D; i += 32)
+              times(col_o + i, false);
+          }
+          if (c > 0) {   // weights of this block
+            tmem_wait_store();
+#pragma unroll 1
+            for (int i = 0; i < c; ++i)
+              times(col_s + 32 * i, true);
+            tmem_wait_store();
+          }
+        };
+        auto weigh = [&](auto hidden) {
+          constexpr bool HIDDEN = decltype(hidden)::value;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[32];
+            tmem_load32(col_s + 32 * c, w);
+            tmem_arrived(w);
+            const uint32_t m = HIDDEN ? sees(c) : 0u, bad = HIDDEN ? Notes::word(notes.k_bad, c) & m : 0u;
+            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            const uint64_t ff = pack2(factor, factor);
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {   // scores
+              uint64_t mid[2] = {};
+#pragma unroll
+              for (int gr = 0; gr < GROUPS; ++gr) {
+                const float4 f = *reinterpret_cast<const float4 *>(notes.k_mid[gr] + 32 * c + k);
+                const uint64_t by = pack2(sum_q[gr], sum_q[gr]);
+                mid[0] = gr == 0 ? mul_2(pack2(f.x, f.y), by) : fma_2(pack2(f.x, f.y), by, mid[0]);
+                mid[1] = gr == 0 ? mul_2(pack2(f.z, f.w), by) : fma_2(pack2(f.z, f.w), by, mid[1]);
+              }
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                const float2 y = unpack2(fma_2(pack2(__uint_as_float(w[k + e]), __uint_as_float(w[k + e + 1])), ff, mid[e / 2]));
+                w[k + e] = !HIDDEN || m >> (k + e) & 1 ? __float_as_uint(y.x) : 0xff800000u;
+                w[k + e + 1] = !HIDDEN || m >> (k + e + 1) & 1 ? __float_as_uint(y.y) : 0xff800000u;
+                x[k / 2 + e / 2 & 3] = max3(x[k / 2 + e / 2 & 3], __uint_as_float(w[k + e]), __uint_as_float(w[k + e + 1]));
+              }
+            }
+            const float top = fmaxf(max3(x[0], x[1], x[2]), x[3]);
+            if (__any_sync(0xffffffffu, top > r + (kKv4Top + kKv4Lag)))
+              move(top, c);
+            const uint64_t rr = pack2(-r, -r);
+            uint64_t sum[2] = {};
+            uint32_t out[32];
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+              uint64_t both[2];
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                float2 y = unpack2(add_2(pack2(__uint_as_float(w[k + e]), __uint_as_float(w[k + e + 1])), rr));
+                y.x = ex2(y.x);
+                y.y = ex2(y.y);
+                if constexpr (HIDDEN) {
+                  y.x = bad >> (k + e) & 1 ? NAN : m >> (k + e) & 1 ? y.x : 0.f;
+                  y.y = bad >> (k + e + 1) & 1 ? NAN : m >> (k + e + 1) & 1 ? y.y : 0.f;
+                }
+                both[e / 2] = pack2(y.x, y.y);
+                sum[e / 2] = add_2(sum[e / 2], both[e / 2]);
+                const uint32_t high = pack_f16(y.x, y.y);
+                const float2 f = halves(high);
+                out[(k + e) / 2] = high;
+                out[16 + (k + e) / 2] = pack_f16(y.x - f.x, y.y - f.y);
+              }
+#pragma unroll
+              for (int gr = 0; gr < GROUPS; ++gr) {
+                const float4 f = *reinterpret_cast<const float4 *>(notes.v_mid[gr] + 32 * c + k);
+                bias[gr] = fma_2(both[0], pack2(f.x, f.y), bias[gr]);
+                bias[gr] = fma_2(both[1], pack2(f.z, f.w), bias[gr]);
+              }
+            }
+            const float2 all = unpack2(add_2(sum[0], sum[1]));
+            l += all.x + all.y;
+            tmem_store32(col_s + 32 * c, out);   // (in the place of the scores that they were)
+            if constexpr (HIDDEN)
+#pragma unroll
+              for (int gr = 0; gr < GROUPS; ++gr)
+                marks[gr] = marks[gr] || (Notes::word(notes.v_bad[gr], c) & m) != 0;
+          }
+        };
+        if (masked)
+          weigh(std::true_type());
+        else
+          weigh(std::false_type());
+        if (j > 0)   // every product is waited for before the next can begin: a wait tells one phase from its neighbours only
+          wait(ok, &bars.pv_done, block - 1, 743);
+        tmem_wait_store();
+        fence_before();
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(&bars.p_ready[block & 1]);
+      }
+      made += n;
+      // ---- the rows' sums: out, or a part ------------------------------------------------------------------------------------------
+      const bool whole = g.b0 == 0 && g.b1 == g.all;
+      float *part = p.parts + ((int64_t)blockIdx.x * 2 + (g.b0 == 0)) * H::PART;
+      const int64_t to = live ? row_at(p, g.r0 + g.first, g.at.slot, row, p.a.out_ld, D) : 0;
+      wait(ok, &bars.pv_done, made - 1, 749);
+      fence_after();
+#pragma unroll
+      for (int gr = 0; gr < GROUPS; ++gr) {
+        const float2 f = unpack2(bias[gr]);
+        const float b = f.x + f.y;
+#pragma unroll 1
+        for (int c = kKv4Group * gr; c < kKv4Group * (gr + 1); c += 32) {
+          uint32_t w[32];
+          tmem_load32(col_o + c, w);
+          tmem_arrived(w);
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float o[4] = {__uint_as_float(w[e]) + b, __uint_as_float(w[e + 1]) + b, __uint_as_float(w[e + 2]) + b, __uint_as_float(w[e + 3]) + b};
+              if (whole)
+                put_over<B200_F32>(p, to + c + e, o, l, marks[gr]);
+              else
+                __stcg(reinterpret_cast<float4 *>(part) + (c + e) / 4 * kRows + row, make_float4(o[0], o[1], o[2], o[3]));
+            }
+          }
+        }
+      }
+      fence_before();
+      if (whole)
+        continue;
+      if (live) {
+        float *rest = part + kRows * D;
+        rest[row] = r;
+        rest[kRows + row] = l;
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr)
+          rest[(2 + gr) * kRows + row] = marks[gr] ? 1.f : 0.f;
+      }
+      meet<D, B200_F32, kRows, 32 * kSoftmaxWarps>(p, plan, g, bars.meeting, row, live, to);
+    }
+  } else if (works && warp < kSoftmaxWarps + kMakers) {
+    // ---- makers: a tile of every block each ------------------------------------------------------------------------------------------
+    const int tile = warp - kSoftmaxWarps, gq = lane >> 2, t = lane & 3;
+    // (rows of K and of V^T that a lane writes are g, modulo eight)
+    const uint32_t k_at = smem_u32(ks) + gq * 128 + tile * (kKv4Tile * 128), v_at = smem_u32(vs) + gq * 128 + 4 * t + tile / 4 * (D * 128);
+    struct Raw {
+      uint32_t k[2][D / 32], v[D / 16];               // codes of rows g and g + 8; words of V
+      uint32_t kp[2][GROUPS], vp[2][2][GROUPS];       // pairs of rows g and g + 8; of keys 2 t + e + 8 u
+    };
+    auto load = [&](Raw &x, int from) {
+      const uint8_t *at = p.pool + (int64_t)max(from, 0) * H::BYTES;   // (a tile that nobody sees: its pairs become zero)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = gq + 8 * h;
+        if constexpr (D == 128) {
+          *reinterpret_cast<uint4 *>(x.k[h]) = __ldg(reinterpret_cast<const uint4 *>(at + j * 64 + t * 16));
+          *reinterpret_cast<uint4 *>(x.v + 4 * h) = __ldg(reinterpret_cast<const uint4 *>(at + kv4_v_codes(D) + h * 512 + lane * 16));
+          *reinterpret_cast<uint2 *>(x.kp[h]) = __ldg(reinterpret_cast<const uint2 *>(at + kv4_k_pairs(D) + j * 8));
+          *reinterpret_cast<uint4 *>(x.vp[h]) = __ldg(reinterpret_cast<const uint4 *>(at + kv4_v_pairs(D) + (2 * t + 8 * h) * 8));
+        } else {
+          *reinterpret_cast<uint2 *>(x.k[h]) = __ldg(reinterpret_cast<const uint2 *>(at + j * 32 + t * 8));
+          if (h == 0)
+            *reinterpret_cast<uint4 *>(x.v) = __ldg(reinterpret_cast<const uint4 *>(at + kv4_v_codes(D) + lane * 16));
+          x.kp[h][0] = __ldg(reinterpret_cast<const uint32_t *>(at + kv4_k_pairs(D) + j * 4));
+          *reinterpret_cast<uint2 *>(x.vp[h]) = __ldg(reinterpret_cast<const uint2 *>(at + kv4_v_pairs(D) + (2 * t + 8 * h) * 4));
+        }
+      }
+    };
+    bool ok = true;
+    uint32_t made = 0;
+    Walk walk(plan);
+    Segment g;
+    while (walk.next(plan, g)) {
+      const int most = clamp((long long)g.base + g.first + g.tokens, 0, room);   // keys that any row sees
+      const int n = g.b1 - g.b0;
+      auto source = [&](int i) {   // of this warp's tile of block i: its number in the pool, or -1
+        const int x = kTiles * (g.b0 + i) + tile;
+        return i >= n || x * kKv4Tile >= most ? -1 : tile_source(p, g.at.s, g.at.slot, x);
+      };
+      int now = source(lane), next = source(32 + lane);
+      Raw raw, ahead;
+      uint32_t v[D / 16], vp[2][2][GROUPS];   // of the block before
+      bool v_beyond = false;
+      int from, then = __shfl_sync(0xffffffffu, now, 0);
+      load(ahead, then);
+      for (int i = 0; i <= n; ++i) {
+        raw = ahead;
+        from = then;
+        if (((i + 1) & 31) == 0) {
+          now = next;
+          next = source(i + 33 + lane);
+        }
+        then = __shfl_sync(0xffffffffu, now, (i + 1) & 31);
+        if (i < n)
+          load(ahead, then);   // (of the block after the last: tile 0 of the pool, not used)
+        const uint32_t block = made + i;
+        const int key0 = (g.b0 + i) * kKeys + kKv4Tile * tile;
+        bool beyond = false;
+        if (i < n) {
+          // ---- pairs: those of keys that nobody sees, and those that are not finite, are zero
+          uint32_t k_bad = 0, v_bad[GROUPS] = {}, strange = 0;
+          auto every = [&](auto f) {   // f(pair, key of the tile, mask of what is bad)
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                f(raw.kp[u][gr], gq + 8 * u, k_bad);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  f(raw.vp[u][e][gr], 2 * t + e + 8 * u, v_bad[gr]);
+              }
+          };
+          every([&](uint32_t &pair, int, uint32_t &) {   // (8 s beyond f16, or something not finite: x - x is not zero)
+            uint32_t x;
+            asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(x) : "r"(pair), "r"(0x3c004800u));
+            const __half2 y = *reinterpret_cast<const __half2 *>(&x), d = __hsub2(y, y);
+            strange |= *reinterpret_cast<const uint32_t *>(&d);
+          });
+          beyond = __any_sync(0xffffffffu, strange != 0);
+          bool any_bad = false;
+          if (from < 0 || key0 + kKv4Tile > most || beyond) {
+            every([&](uint32_t &pair, int key, uint32_t &bad) {
+              const bool seen = from >= 0 && key0 + key < most;
+              if (!seen || !finite_pair(pair)) {
+                bad |= seen ? 1u << key : 0u;
+                pair = 0u;
+              }
+            });
+            k_bad = __reduce_or_sync(0xffffffffu, k_bad);
+            uint32_t all = k_bad;
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr) {
+              v_bad[gr] = __reduce_or_sync(0xffffffffu, v_bad[gr]);
+              all |= v_bad[gr];
+            }
+            any_bad = all != 0;
+          }
+          // ---- K: words of eight dims of a key
+          if (block > 0)
+            wait(ok, &bars.s_full[(block - 1) & 1], (block - 1) >> 1, 744);
+          Notes &notes = bars.notes[block % kNotes];   // (the block four before is done with)
+          auto mid = [](uint32_t pair) {
+            const float2 f = halves(pair);
+            return fmaf(8.f, f.x, f.y);
+          };
+#pragma unroll
+          for (int gr = 0; gr < GROUPS; ++gr)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              if (t == 0)
+                notes.k_mid[gr][kKv4Tile * tile + gq + 8 * u] = mid(raw.kp[u][gr]);
+              if (gq == 0)
+                *reinterpret_cast<float2 *>(notes.v_mid[gr] + kKv4Tile * tile + 2 * t + 8 * u) = make_float2(mid(raw.vp[u][0][gr]), mid(raw.vp[u][1][gr]));
+            }
+          if (lane == 0) {
+            const uint32_t hole = from < 0 && key0 < most ? 0xffffu : 0u;
+            notes.k_bad[tile] = (uint16_t)k_bad;
+            notes.hole[tile] = (uint16_t)hole;
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr)
+              notes.v_bad[gr][tile] = (uint16_t)v_bad[gr];
+            notes.special[tile] = (uint16_t)(any_bad ? 1u : hole);
+          }
+          auto make_k = [&](auto held) {
+            constexpr bool HELD = decltype(held)::value;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int gr = 0; gr < GROUPS; ++gr) {
+                const uint32_t s = __byte_perm(raw.kp[h][gr], 0, 0x1010);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                  const uint32_t x = raw.k[h][2 * gr + w], y = x >> 8, at = k_at + gr * (kKeys * 128) + h * 1024 + (((4 * w + t) ^ gq) << 4);
+                  uint32_t high[4], low[4];
+                  terms<HELD>(low_codes(x), s, high[0], low[0]);
+                  terms<HELD>(high_codes(x), s, high[1], low[1]);
+                  terms<HELD>(low_codes(y), s, high[2], low[2]);
+                  terms<HELD>(high_codes(y), s, high[3], low[3]);
+                  store4(at, high[0], high[1], high[2], high[3]);
+                  store4(at + H::TERM, low[0], low[1], low[2], low[3]);
+                }
+              }
+          };
+          if (beyond)
+            make_k(std::true_type());
+          else
+            make_k(std::false_type());
+          fence_proxy();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive(&bars.k_full);
+        }
+        if (i > 0) {
+          // ---- V of the block before: words of dims 16 w + g (+ 8) and keys 2 t, 2 t + 1 (+ 8)
+          if (block > 1)
+            wait(ok, &bars.pv_done, block - 2, 745);
+          const int c = tile % 4 * 2;
+          auto make_v = [&](auto held) {
+            constexpr bool HELD = decltype(held)::value;
+#pragma unroll
+            for (int gr = 0; gr < GROUPS; ++gr) {
+              const uint32_t s[2] = {__byte_perm(vp[0][0][gr], vp[0][1][gr], 0x5410), __byte_perm(vp[1][0][gr], vp[1][1][gr], 0x5410)};
+#pragma unroll
+              for (int w = 4 * gr; w < 4 * gr + 4; ++w) {
+                const uint32_t x = v[w];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                  const uint32_t at = v_at + w * 2048 + (((c + u) ^ gq) << 4);
+                  uint32_t high, low;
+                  terms<HELD>(low_codes(x >> 8 * u), s[u], high, low);
+                  store1(at, high);
+                  store1(at + H::TERM, low);
+                  terms<HELD>(high_codes(x >> 8 * u), s[u], high, low);
+                  store1(at + 1024, high);
+                  store1(at + 1024 + H::TERM, low);
+                }
+              }
+            }
+          };
+          if (v_beyond)
+            make_v(std::true_type());
+          else
+            make_v(std::false_type());
+          fence_proxy();
+          __syncwarp();
+          if (lane == 0)
+            mbar_arrive(&bars.v_full);
+        }
+        if (i < n) {
+#pragma unroll
+          for (int w = 0; w < D / 16; ++w)
+            v[w] = raw.v[w];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int gr = 0; gr < GROUPS; ++gr)
+                vp[u][e][gr] = raw.vp[u][e][gr];
+          v_beyond = beyond;
+        }
+      }
+      made += n;
+    }
+  } else if (works) {
+    // ---- tensor core issue --------------------------------------------------------------------------------------------------------
+    uint32_t leader;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(leader));
+    const uint64_t dq = smem_desc(smem_u32(qs)), dk = smem_desc(smem_u32(ks)), dv = smem_desc(smem_u32(vs));
+    bool ok = true;
+    uint32_t made = 0, segments = 0;
+    // the small products first: terms of the first operand and of the second
+    constexpr uint32_t FIRST[3] = {1, 0, 0}, SECOND[3] = {0, 1, 0};
+    auto scores = [&](uint32_t block) {
+      wait(ok, &bars.k_full, block, 746);
+      if (!ok)
+        return;
+      fence_after();
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss<kKeys>(leader, tmem + H::COL_S + (block & 1) * kKeys, dq + ((FIRST[i] * H::TERM + (k >> 2) * (kRows * 128) + (k & 3) * 32) >> 4),
+                        dk + ((SECOND[i] * H::TERM + (k >> 2) * (kKeys * 128) + (k & 3) * 32) >> 4), (i | k) != 0);
+      if (leader)
+        tc_commit(&bars.s_full[block & 1]);
+    };
+    Walk walk(plan);
+    Segment g;
+    while (ok && walk.next(plan, g)) {
+      const uint32_t n = g.b1 - g.b0;
+      wait(ok, &bars.q_full, segments++, 747);
+      if (!ok)
+        break;
+      scores(made);
+      for (uint32_t j = 0; j < n && ok; ++j) {
+        const uint32_t block = made + j;
+        if (j + 1 < n)
+          scores(block + 1);
+        wait(ok, &bars.p_ready[block & 1], block >> 1, 748);
+        wait(ok, &bars.v_full, block, 750);
+        if (!ok)
+          break;
+        fence_after();
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)   // (weights: of 32 keys sixteen columns of each term)
+            mma_ts<D>(leader, tmem + H::COL_O, tmem + H::COL_S + (block & 1) * kKeys + (k >> 1) * 32 + FIRST[i] * 16 + (k & 1) * 8,
+                      dv + ((SECOND[i] * H::TERM + (k >> 2) * (D * 128) + (k & 3) * 32) >> 4), (j | i | k) != 0);
+        if (leader)
+          tc_commit(&bars.pv_done);
+      }
+      made += n;
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == kSoftmaxWarps + kMakers) {
+    if (*ab) {   // products of an abandoned block may still be in flight: let them land
+      const unsigned long long t0 = now_ns();
+      while (now_ns() - t0 < 2000000ull) {
+      }
+    }
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kCols) : "memory");
+  }
+}
+
+RaisedOn g_raised[2];
+constexpr int kMostSeqs = 1000;   // whose plan fits beside the operands
+
+template <int D> int exact_launch(RaisedOn &raised, const Kv4Params &p, cudaStream_t st) {
+  if (int rc = raise_shared_limit(raised, (const void *)kv4_exact_kernel<D>, Shape<D>::SMEM + RowsPlan::bytes(kMostSeqs)))
+    return rc;
+  return launch_after(kv4_exact_kernel<D>, dim3(kKv4Ctas), kThreads, Shape<D>::SMEM + RowsPlan::bytes(p.a.n_seqs), st, p);
+}
+
+} // namespace
+
+bool kv4_exact_takes(int G, int n_seqs) { return G <= kRows && n_seqs <= kMostSeqs; }
+
+int kv4_exact_launch(Kv4Params p, int D, cudaStream_t st) {
+  p.heads = p.G;
+  p.subs = 1;
+  p.tokens = kRows / p.G;
+  p.over_heads = (65536 + p.heads - 1) / p.heads;
+  return D == 128 ? exact_launch<128>(g_raised[0], p, st) : exact_launch<64>(g_raised[1], p, st);
+}
+
+} // namespace b200

@@ -138,9 +138,9 @@ struct Place {
   int s, slot, rt, tile;
 };
 
-// SHIFT: log2 of a tile's keys.  An item that CTAs share costs them what some SPLIT keys do (its parts' way through L2): where whole items leave
+// SHIFT: log2 of a tile's keys.  An item that CTAs share costs them what some `split` keys do (its parts' way through L2): where whole items leave
 // nobody with that much more than an even share, CTAs have whole items.
-template <int SHIFT, int SPLIT> struct KeyPlan {
+template <int SHIFT> struct KeyPlan {
   const long long *cost;   // [n + 1], in shared memory as the others
   const int *r0, *base;    // [n + 1], [n]: a sequence's rows, and the position of the first
   const int *items;        // [n + 1]: items before it
@@ -152,7 +152,7 @@ template <int SHIFT, int SPLIT> struct KeyPlan {
   static __host__ __device__ constexpr int bytes(int n) { return 20 * (n + 1); }
 
   // By all THREADS of the CTA; sums: 2 * THREADS / 32 + 1 words of shared memory.
-  template <int THREADS> __device__ __forceinline__ void build(const Kv4Params &p, void *memory, long long *sums, int least_keys) {
+  template <int THREADS> __device__ __forceinline__ void build(const Kv4Params &p, void *memory, long long *sums, int least_keys, int split) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, room = p.a.table_stride * p.page;
     n = p.a.n_seqs;
     tokens = p.tokens;
@@ -235,7 +235,7 @@ template <int SHIFT, int SPLIT> struct KeyPlan {
     const long long chunk = small ? (int)total / ctas : total / ctas;
     window = chunk > kKv4Many ? kKv4Snap / 4 : (int)min((long long)kKv4Snap, chunk / 2 - 1);
     const int each = (all_items + (int)gridDim.x - 1) / (int)gridDim.x;
-    whole = all_items < kNone && (long long)each * most <= chunk + SPLIT;
+    whole = all_items < kNone && (long long)each * most <= chunk + split;
     if (whole)
       ctas = max(1, min((int)gridDim.x, all_items));
   }
@@ -369,9 +369,11 @@ __device__ __forceinline__ int tile_source(const Kv4Params &p, int s, int kv, in
   return id < 0 || id >= p.n_pages ? -1 : (id * p.kv_heads + kv) * per_page + t % per_page;
 }
 
-// kv4_chunk.cu: sequences of many rows, on tcgen05
+// sequences of many rows, on tcgen05: kv4_chunk.cu (16-bit rows), kv4_exact.cu (f32)
 int64_t kv4_chunk_part_floats(int D);   // of a CTA's two parts
-bool kv4_chunk_takes(int dtype, int G, int n_seqs);
+bool kv4_chunk_takes(int G, int n_seqs);
 int kv4_chunk_launch(Kv4Params p, int D, cudaStream_t st);
+bool kv4_exact_takes(int G, int n_seqs);
+int kv4_exact_launch(Kv4Params p, int D, cudaStream_t st);
 
 } // namespace b200

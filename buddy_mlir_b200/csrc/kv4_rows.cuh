@@ -9,7 +9,7 @@ namespace b200 {
 constexpr int kRows = 128;                          // query rows of a product
 constexpr int kKeys = 128, kShift = 7;              // of a block
 constexpr int kTiles = kKeys / kKv4Tile;            // of a block
-using RowsPlan = KeyPlan<kShift, 1200>;
+using RowsPlan = KeyPlan<kShift>;
 
 // kind::f16 instruction descriptor: D = f32, A = B = f16, both K-major, M = 128.
 template <int N> __host__ __device__ constexpr uint32_t idesc() {
@@ -56,6 +56,7 @@ __device__ __forceinline__ void fence_proxy() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ void store4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {   // (an address in shared memory)
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ void store2(uint32_t at, uint32_t a, uint32_t b) { asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(a), "r"(b) : "memory"); }
 __device__ __forceinline__ void store1(uint32_t at, uint32_t a) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(a) : "memory"); }
 __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;

@@ -1,4 +1,4 @@
-"""b200_kv4_attention with many rows of a sequence in 16-bit types: where it can go wrong that its few-rows form cannot."""
+"""b200_kv4_attention with many rows of a sequence: where it can go wrong that its few-rows form cannot."""
 import numpy as np
 import pytest
 
@@ -7,7 +7,7 @@ from buddy_mlir_b200 import _lib
 from test_gpu_kv4 import Batch, dev, poison
 
 pytestmark = pytest.mark.gpu
-KINDS = pytest.mark.parametrize("kind", ["f16", "bf16"])
+KINDS = pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 
 
 def sound(b):
@@ -142,7 +142,7 @@ def test_scales(kind, scale):
 
 
 def test_large_and_small_queries():
-    for kind in ("f16", "bf16"):
+    for kind in ("f32", "f16", "bf16"):
         for q_scale in (20.0, 1e-4, 0.0):
             Batch([300], [140], 8, 2, 128, 16, kind, 38, q_scale=q_scale).check(every=5)
 
@@ -172,18 +172,18 @@ def test_a_prompt_beside_decode_steps(kind):
     Batch(lens, [280] + [1] * 20 + [64], 8, 2, 64, 16, kind, 41).check(every=11)
 
 
-@pytest.mark.parametrize("n,long", [(1500, 300), (1501, 300), (4096, 600)])
-def test_a_prompt_among_very_many_sequences(n, long):
+@pytest.mark.parametrize("kind,n,long", [("bf16", 1500, 300), ("bf16", 1501, 300), ("f32", 1000, 200), ("f32", 1001, 200), ("bf16", 4096, 600)])
+def test_a_prompt_among_very_many_sequences(kind, n, long):
     """Around the number of sequences from which on the few-rows form has all of them, and the most that a call takes."""
     rng = np.random.default_rng(n)
     lens = [int(x) for x in rng.integers(0, 4, n)]
     counts = [int(x) for x in rng.integers(0, 2, n)]
     lens[n // 2], counts[n // 2] = long, long
-    Batch(lens, counts, 128, 1, 64, 16, "bf16", 42).check(every=101)
+    Batch(lens, counts, 128, 1, 64, 16, kind, 42).check(every=101)
 
 
 def test_keys_of_one_prompt_over_the_whole_chip():
-    for kind in ("f16", "bf16"):
+    for kind in ("f32", "f16", "bf16"):
         b = Batch([9000, 40], [66, 1], 8, 8, 64, 64, kind, 43)
         first = b.check(every=13).clone()
         for _ in range(10):
