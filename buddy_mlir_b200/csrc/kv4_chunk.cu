@@ -1,6 +1,6 @@
 // Attention over the 4-bit KV cache for sequences of many rows (a chunk of a prompt, or all of it) on the 5th-generation tensor cores.
 //
-// Where many rows meet a key its 128 codes are better made values once: six warps turn 128 keys into f16 operands (K [128][D], V
+// Where many rows meet a key its 128 codes are better made values once: seven warps turn 128 keys into f16 operands (K [128][D], V
 // transposed [D][128], swizzled), two times 128 query rows are multiplied with them.  A code becomes f16 by way of 1024 + c; with its group's scale and
 // minimum it meets in one fma, so with one rounding: a value of the cache is a multiple of 2^-24, where f16 ends, and half a step off above 2^-13.
 // Only a group of the whole range of f16 can reach beyond it, by its scale's rounding, to 65536: that is held at 65504.
@@ -11,7 +11,7 @@
 // Two sets of 128 rows take turns: one's products run under the other's softmax.  (S 2 x 128 columns, O 2 x D.)
 // A key's values that are not finite are zero in the operands, and what sees them becomes NaN afterwards: nothing reaches rows that do not.
 //
-// 1001 rows at 4000 keys, 32 heads on 8 of 128 dims, bf16: 120 us, 479 TFLOP/s, 0.29 of a dense product's rate.  A block of 128 keys takes an SM 7000 clocks,
+// 1001 rows at 4000 keys, 32 heads on 8 of 128 dims, bf16: 115 us, 499 TFLOP/s, 0.30 of a dense product's rate.  A block of 128 keys takes an SM 7000 clocks,
 // 1500 of them for its products: a set's softmax (3400) and the way of its weights through both products (2400) follow each other.
 #include "kv4_rows.cuh"
 
@@ -23,7 +23,7 @@ namespace b200 {
 namespace {
 
 constexpr int kSets = 2;                            // of kRows
-constexpr int kSoftmaxWarps = 4 * kSets, kMakers = 6, kThreads = 32 * (kSoftmaxWarps + kMakers + 1);
+constexpr int kSoftmaxWarps = 4 * kSets, kMakers = 7, kThreads = 32 * (kSoftmaxWarps + kMakers + 1);
 constexpr int kStages = 2, kNotes = 4;
 constexpr uint32_t kCols = 512;
 constexpr int kLeastKeys = 256, kSplit = 1200;
@@ -320,7 +320,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
         meet<D, TYPE, kSets * kRows, 32 * kSoftmaxWarps>(p, plan, g, bars.meeting, at, live, to);
     }
   } else if (works && warp < kSoftmaxWarps + kMakers) {
-    // ---- makers: every sixth tile each -------------------------------------------------------------------------------------------
+    // ---- makers: every seventh tile each -------------------------------------------------------------------------------------------
     const int mw = warp - kSoftmaxWarps, gq = lane >> 2, t = lane & 3;
     const uint32_t s_k = smem_u32(ks) + gq * 128, s_v = smem_u32(vs) + gq * 128 + 4 * t;
     struct Raw {

@@ -7,8 +7,9 @@
 // are a few f32 operations of the thread that has the row.  Three of the four products of terms are summed, the small ones first; centred sums stay
 // small, which matters because the tensor cores' sums round towards zero.
 //
-// Eight warps make the operands of 128 keys, a tile of sixteen each: K of a block while the softmax has the one before it, then V when that block's product
-// is done.  Four warps do the softmax, a thread per row, as in kv4_chunk.cu; scores of two blocks have their own columns (2 x 128, and D for O).
+// Seven warps make the operands of 128 keys: K of a block while the softmax has the one before it, V when the product of the block before is done.  Eight
+// do the softmax, two threads per row: scores of half a block each, the larger of their maxima (through shared memory) decides whether the row's
+// reference moves, weights.  Scores of two blocks have their own columns (2 x 128, and D for O).
 //
 // A prompt of 1000 rows, 12 heads on 2 of 128 dims: 51 us (the few-rows form 70): 96 items on as many CTAs, the longest of eight blocks, and a block takes 6700 clocks,
 // 6200 of them the softmax at one warp a scheduler, 2300 the products.  Items that CTAs share come together too slowly to be worth it (78 us).
@@ -21,7 +22,7 @@ namespace b200 {
 
 namespace {
 
-constexpr int kSoftmaxWarps = 4, kMakers = kTiles, kThreads = 32 * (kSoftmaxWarps + kMakers + 1);
+constexpr int kSoftmaxWarps = 8, kMakers = 7, kThreads = 32 * (kSoftmaxWarps + kMakers + 1);
 constexpr int kNotes = 4;
 constexpr uint32_t kCols = 512;
 constexpr int kLeastKeys = 256, kSplit = 1200;
@@ -47,6 +48,9 @@ struct Bars {
   uint32_t tmem_base;
   int abort_flag;
   Meeting meeting;
+  float row[kRows][4];         // its scores' factor, sums of q
+  float top[2][2][kRows];      // of a row's half of a block: largest score
+  float4 half[2][kRows];       // of a row's half of the keys: total, sums with m, marks
   long long sums[2 * (kThreads / 32) + 1];
   Notes notes[kNotes];
 };
@@ -80,8 +84,8 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
   int *error = p.counters + kKv4Ctas;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bars.k_full, kMakers);
-    mbar_init(&bars.v_full, kMakers);
+    mbar_init(&bars.k_full, kTiles);
+    mbar_init(&bars.v_full, kTiles);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.p_ready[i], kSoftmaxWarps);
@@ -118,49 +122,47 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
   };
 
   if (works && warp < kSoftmaxWarps) {
-    // ---- softmax: a thread per row --------------------------------------------------------------------------------------------
-    const int row = warp * 32 + lane;
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16), col_o = lanes + H::COL_O;
+    // ---- softmax: two threads per row, of half a block's keys each ----------------------------------------------------------------------
+    const int row = (warp & 3) * 32 + lane, side = warp >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), col_o = lanes + H::COL_O + side * (D / 2);
+    auto pair_meets = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };   // (the two warps of the same rows)
     bool ok = true;
     uint32_t made = 0;
     Walk walk(plan);
     Segment g;
     while (walk.next(plan, g)) {
       const uint32_t n = g.b1 - g.b0;
-      float r = kKv4Seed, l = 0.f, factor, sum_q[GROUPS] = {};
+      float r = kKv4Seed, l = 0.f, sum_q[GROUPS];
       uint64_t bias[GROUPS] = {};               // sums of p m, over even and odd keys
-      bool marks[GROUPS] = {};                  // V groups that become NaN
+      uint32_t marks = 0;                       // V groups that become NaN
       const int token = row / p.G;
       const bool live = token < min(g.tokens, p.tokens);
       const int seen_by = live ? clamp((long long)g.base + g.first + token + 1, 0, room) : 0;
       {
-        // ---- q: times a power of two, as two f16
-        // (row by row, four dims a lane)
-        constexpr int LANES = D / 4;              // of a row
+        // ---- q: times a power of two, as two f16; row by row, four dims a lane
+        constexpr int LANES = D / 4, BATCH = 8;   // lanes of a row (of 64 dims: two rows at once); loads side by side
         const int64_t mine = live ? row_at(p, g.r0 + g.first, g.at.slot, row, p.a.q_ld, D) : -1;
         const int d = 4 * (lane % LANES);
-        factor = 0.f;
-        constexpr int BATCH = 16;
-        float batch[BATCH][4];
-        auto fetch = [&](int i, float (&x)[4]) {
-          const int64_t at = __shfl_sync(0xffffffffu, mine, 32 / LANES * i + lane / LANES);
-          const float *q = (const float *)p.a.q + max(at, (int64_t)0) + d;
+#pragma unroll 1
+        for (int from = 0; from < LANES / 2; from += BATCH) {
+          float batch[BATCH][4], most[BATCH], sum[BATCH];
+          // (this warp's rows: the first or second half of the 32)
+          auto which = [&](int b) { return 16 * side + 32 / LANES * (from + b) + lane / LANES; };
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[e] = 0.f;
-          if (at >= 0 && p.wide_q)
-            *reinterpret_cast<float4 *>(x) = __ldg(reinterpret_cast<const float4 *>(q));
-          else if (at >= 0)
+          for (int b = 0; b < BATCH; ++b) {
+            float (&x)[4] = batch[b];
+            const int64_t at = __shfl_sync(0xffffffffu, mine, which(b));
+            const float *q = (const float *)p.a.q + max(at, (int64_t)0) + d;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              x[e] = __ldg(q + e);
-        };
-#pragma unroll 1
-        for (int from = 0; from < LANES; from += BATCH) {   // (of 64 dims: two rows at once)
-          float most[BATCH], sum[BATCH];
+              x[e] = 0.f;
+            if (at >= 0 && p.wide_q)
+              *reinterpret_cast<float4 *>(x) = __ldg(reinterpret_cast<const float4 *>(q));
+            else if (at >= 0)
 #pragma unroll
-          for (int b = 0; b < BATCH; ++b)
-            fetch(from + b, batch[b]);
+              for (int e = 0; e < 4; ++e)
+                x[e] = __ldg(q + e);
+          }
 #pragma unroll
           for (int b = 0; b < BATCH; ++b) {
             const float (&x)[4] = batch[b];
@@ -180,36 +182,36 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
 #pragma unroll
           for (int b = 0; b < BATCH; ++b) {
             const float (&x)[4] = batch[b];
-            const int up = min(max(14 + 127 - (int)(__float_as_uint(most[b]) >> 23), -113), 100), r0 = warp * 32 + 32 / LANES * (from + b) + lane / LANES;
+            const int up = min(max(14 + 127 - (int)(__float_as_uint(most[b]) >> 23), -113), 100), at = (warp & 3) * 32 + which(b);
             const float by = power(up);
-#pragma unroll
-            for (int gr = 0; gr < GROUPS; ++gr) {   // (the lane that has this row)
-              const float s = __shfl_sync(0xffffffffu, sum[b], GROUPS == 2 ? 16 * gr : lane % 2 * 16);
-              sum_q[gr] = lane / (32 / LANES) == from + b ? s * p.log2_scale : sum_q[gr];
-            }
-            const float unit = __shfl_sync(0xffffffffu, power(-up), GROUPS == 2 ? 0 : lane % 2 * 16);
-            factor = lane / (32 / LANES) == from + b ? unit : factor;
+            if (lane % LANES == 0)
+              bars.row[at][0] = power(-up) * p.log2_scale;
+            if (lane % 16 == 0)
+              bars.row[at][1 + lane % LANES / 16] = sum[b] * p.log2_scale;
             const float a[4] = {x[0] * by, x[1] * by, x[2] * by, x[3] * by};
             const uint32_t high[2] = {pack_f16(a[0], a[1]), pack_f16(a[2], a[3])};
             const float2 f = halves(high[0]), h = halves(high[1]);
-            const uint32_t to = smem_u32(qs) + r0 * 128 + d / 64 * (kRows * 128) + ((d / 8 % 8 ^ (r0 & 7)) << 4) + d % 8 * 2;
+            const uint32_t to = smem_u32(qs) + at * 128 + d / 64 * (kRows * 128) + ((d / 8 % 8 ^ (at & 7)) << 4) + d % 8 * 2;
             store2(to, high[0], high[1]);
             store2(to + H::TERM, pack_f16(a[0] - f.x, a[1] - f.y), pack_f16(a[2] - h.x, a[3] - h.y));
           }
         }
-        factor *= p.log2_scale;
-#pragma unroll
-        for (int gr = 0; gr < GROUPS; ++gr)
-          if (!(sum_q[gr] - sum_q[gr] == 0.f))   // (a row with an infinity, or NaN, has no scores)
-            factor = NAN;
         fence_proxy();
         fence_before();
         __syncwarp();
         if (lane == 0)
           mbar_arrive(&bars.q_full);
+        pair_meets();
+      }
+      float factor = bars.row[row][0];
+#pragma unroll
+      for (int gr = 0; gr < GROUPS; ++gr) {
+        sum_q[gr] = bars.row[row][1 + gr];
+        if (!(sum_q[gr] - sum_q[gr] == 0.f))    // (a row with an infinity, or NaN, has no scores)
+          factor = NAN;
       }
       for (uint32_t j = 0; j < n; ++j) {
-        const uint32_t block = made + j, col_s = lanes + H::COL_S + (block & 1) * kKeys;
+        const uint32_t block = made + j, col_s = lanes + H::COL_S + (block & 1) * kKeys + side * (kKeys / 2);
         const int key0 = (g.b0 + j) * kKeys, seen = min(max(seen_by - key0, 0), kKeys);   // keys of the block that this row sees
         wait(ok, &bars.s_full[block & 1], block >> 1, 741);
         fence_after();
@@ -222,56 +224,21 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
           const int k = seen - 32 * c;
           return (k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1) & ~Notes::word(notes.hole, c);
         };
-        // a row's reference moves, at the keys 32 c and on
-        auto move = [&](float top, int c) {
-          const bool moves = top > r + (kKv4Top + kKv4Lag);
-          const float to = moves ? ceilf(top) - kKv4Top : r, keep = ex2(r - to);   // (each row for itself)
-          r = to;
-          l *= keep;
-#pragma unroll
-          for (int gr = 0; gr < GROUPS; ++gr)
-            bias[gr] = mul_2(bias[gr], pack2(keep, keep));
-          auto times = [&](uint32_t at, bool pairs) {
-            uint32_t w[32];
-            tmem_load32(at, w);
-            tmem_arrived(w);
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (pairs) {
-                const float2 x = halves(w[e]);
-                w[e] = pack_f16(x.x * keep, x.y * keep);
-              } else {
-                w[e] = __float_as_uint(__uint_as_float(w[e]) * keep);
-              }
-            tmem_store32(at, w);
-          };
-          if (j > 0) {
-            wait(ok, &bars.pv_done, block - 1, 742);
-            fence_after();
-#pragma unroll 1
-            for (int i = 0; i < D; i += 32)
-              times(col_o + i, false);
-          }
-          if (c > 0) {   // weights of this block
-            tmem_wait_store();
-#pragma unroll 1
-            for (int i = 0; i < c; ++i)
-              times(col_s + 32 * i, true);
-            tmem_wait_store();
-          }
-        };
-        auto weigh = [&](auto hidden) {
+        // ---- scores, back in their place, and the largest
+        float top = -INFINITY;
+        auto score = [&](auto hidden) {
           constexpr bool HIDDEN = decltype(hidden)::value;
+          const uint64_t ff = pack2(factor, factor);
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
+          for (int i = 0; i < 2; ++i) {
+            const int c = 2 * side + i;
             uint32_t w[32];
-            tmem_load32(col_s + 32 * c, w);
+            tmem_load32(col_s + 32 * i, w);
             tmem_arrived(w);
-            const uint32_t m = HIDDEN ? sees(c) : 0u, bad = HIDDEN ? Notes::word(notes.k_bad, c) & m : 0u;
+            const uint32_t m = HIDDEN ? sees(c) : 0u;
             float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            const uint64_t ff = pack2(factor, factor);
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) {   // scores
+            for (int k = 0; k < 32; k += 4) {
               uint64_t mid[2] = {};
 #pragma unroll
               for (int gr = 0; gr < GROUPS; ++gr) {
@@ -288,12 +255,54 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
                 x[k / 2 + e / 2 & 3] = max3(x[k / 2 + e / 2 & 3], __uint_as_float(w[k + e]), __uint_as_float(w[k + e + 1]));
               }
             }
-            const float top = fmaxf(max3(x[0], x[1], x[2]), x[3]);
-            if (__any_sync(0xffffffffu, top > r + (kKv4Top + kKv4Lag)))
-              move(top, c);
-            const uint64_t rr = pack2(-r, -r);
+            tmem_store32(col_s + 32 * i, w);
+            top = fmaxf(top, fmaxf(max3(x[0], x[1], x[2]), x[3]));
+          }
+        };
+        if (masked)
+          score(std::true_type());
+        else
+          score(std::false_type());
+        bars.top[block & 1][side][row] = top;
+        tmem_wait_store();
+        pair_meets();
+        top = fmaxf(top, bars.top[block & 1][1 - side][row]);
+        // ---- a row's reference moves (both threads know it, and have half of the sums each)
+        if (__any_sync(0xffffffffu, top > r + (kKv4Top + kKv4Lag))) {
+          const bool moves = top > r + (kKv4Top + kKv4Lag);
+          const float to = moves ? ceilf(top) - kKv4Top : r, keep = ex2(r - to);   // (each row for itself)
+          r = to;
+          l *= keep;
+#pragma unroll
+          for (int gr = 0; gr < GROUPS; ++gr)
+            bias[gr] = mul_2(bias[gr], pack2(keep, keep));
+          if (j > 0) {
+            wait(ok, &bars.pv_done, block - 1, 742);
+            fence_after();
+#pragma unroll 1
+            for (int i = 0; i < D / 2; i += 32) {
+              uint32_t w[32];
+              tmem_load32(col_o + i, w);
+              tmem_arrived(w);
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                w[e] = __float_as_uint(__uint_as_float(w[e]) * keep);
+              tmem_store32(col_o + i, w);
+            }
+          }
+        }
+        // ---- weights, as two f16 in the place of the scores that they were
+        auto weigh = [&](auto hidden) {
+          constexpr bool HIDDEN = decltype(hidden)::value;
+          const uint64_t rr = pack2(-r, -r);
+#pragma unroll 1
+          for (int i = 0; i < 2; ++i) {
+            const int c = 2 * side + i;
+            uint32_t w[32], out[32];
+            tmem_load32(col_s + 32 * i, w);
+            tmem_arrived(w);
+            const uint32_t m = HIDDEN ? sees(c) : 0u, bad = HIDDEN ? Notes::word(notes.k_bad, c) & m : 0u;
             uint64_t sum[2] = {};
-            uint32_t out[32];
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
               uint64_t both[2];
@@ -322,11 +331,11 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
             }
             const float2 all = unpack2(add_2(sum[0], sum[1]));
             l += all.x + all.y;
-            tmem_store32(col_s + 32 * c, out);   // (in the place of the scores that they were)
+            tmem_store32(col_s + 32 * i, out);
             if constexpr (HIDDEN)
 #pragma unroll
               for (int gr = 0; gr < GROUPS; ++gr)
-                marks[gr] = marks[gr] || (Notes::word(notes.v_bad[gr], c) & m) != 0;
+                marks |= (Notes::word(notes.v_bad[gr], c) & m) != 0 ? 1u << gr : 0u;
           }
         };
         if (masked)
@@ -342,51 +351,62 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
           mbar_arrive(&bars.p_ready[block & 1]);
       }
       made += n;
-      // ---- the rows' sums: out, or a part ------------------------------------------------------------------------------------------
+      // ---- the rows' sums: out, or a part; half of the dims each ----------------------------------------------------------------------
+      {
+        float b[GROUPS];
+#pragma unroll
+        for (int gr = 0; gr < GROUPS; ++gr) {
+          const float2 f = unpack2(bias[gr]);
+          b[gr] = f.x + f.y;
+        }
+        bars.half[side][row] = make_float4(l, b[0], b[GROUPS - 1], __uint_as_float(marks));
+      }
+      pair_meets();
+      const float4 x = bars.half[0][row], y = bars.half[1][row];
+      l = x.x + y.x;
+      marks = __float_as_uint(x.w) | __float_as_uint(y.w);
+      const int gr = GROUPS == 2 ? side : 0;
+      const float b = gr == 0 ? x.y + y.y : x.z + y.z;
       const bool whole = g.b0 == 0 && g.b1 == g.all;
       float *part = p.parts + ((int64_t)blockIdx.x * 2 + (g.b0 == 0)) * H::PART;
       const int64_t to = live ? row_at(p, g.r0 + g.first, g.at.slot, row, p.a.out_ld, D) : 0;
       wait(ok, &bars.pv_done, made - 1, 749);
       fence_after();
-#pragma unroll
-      for (int gr = 0; gr < GROUPS; ++gr) {
-        const float2 f = unpack2(bias[gr]);
-        const float b = f.x + f.y;
 #pragma unroll 1
-        for (int c = kKv4Group * gr; c < kKv4Group * (gr + 1); c += 32) {
-          uint32_t w[32];
-          tmem_load32(col_o + c, w);
-          tmem_arrived(w);
-          if (live) {
+      for (int c = 0; c < D / 2; c += 32) {
+        uint32_t w[32];
+        tmem_load32(col_o + c, w);
+        tmem_arrived(w);
+        if (live) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const float o[4] = {__uint_as_float(w[e]) + b, __uint_as_float(w[e + 1]) + b, __uint_as_float(w[e + 2]) + b, __uint_as_float(w[e + 3]) + b};
-              if (whole)
-                put_over<B200_F32>(p, to + c + e, o, l, marks[gr]);
-              else
-                __stcg(reinterpret_cast<float4 *>(part) + (c + e) / 4 * kRows + row, make_float4(o[0], o[1], o[2], o[3]));
-            }
+          for (int e = 0; e < 32; e += 4) {
+            const float o[4] = {__uint_as_float(w[e]) + b, __uint_as_float(w[e + 1]) + b, __uint_as_float(w[e + 2]) + b, __uint_as_float(w[e + 3]) + b};
+            const int d = side * (D / 2) + c + e;
+            if (whole)
+              put_over<B200_F32>(p, to + d, o, l, marks >> gr & 1);
+            else
+              __stcg(reinterpret_cast<float4 *>(part) + d / 4 * kRows + row, make_float4(o[0], o[1], o[2], o[3]));
           }
         }
       }
       fence_before();
       if (whole)
         continue;
-      if (live) {
+      if (live && side == 0) {
         float *rest = part + kRows * D;
         rest[row] = r;
         rest[kRows + row] = l;
 #pragma unroll
-        for (int gr = 0; gr < GROUPS; ++gr)
-          rest[(2 + gr) * kRows + row] = marks[gr] ? 1.f : 0.f;
+        for (int i = 0; i < GROUPS; ++i)
+          rest[(2 + i) * kRows + row] = marks >> i & 1 ? 1.f : 0.f;
       }
-      meet<D, B200_F32, kRows, 32 * kSoftmaxWarps>(p, plan, g, bars.meeting, row, live, to);
+      meet<D, B200_F32, kRows, 32 * kSoftmaxWarps>(p, plan, g, bars.meeting, row, live, to, side * (D / 2), (side + 1) * (D / 2));
     }
   } else if (works && warp < kSoftmaxWarps + kMakers) {
-    // ---- makers: a tile of every block each ------------------------------------------------------------------------------------------
-    const int tile = warp - kSoftmaxWarps, gq = lane >> 2, t = lane & 3;
+    // ---- makers: every seventh tile each; K of a tile, then V of the one before ------------------------------------------------------------
+    const int mw = warp - kSoftmaxWarps, gq = lane >> 2, t = lane & 3;
     // (rows of K and of V^T that a lane writes are g, modulo eight)
-    const uint32_t k_at = smem_u32(ks) + gq * 128 + tile * (kKv4Tile * 128), v_at = smem_u32(vs) + gq * 128 + 4 * t + tile / 4 * (D * 128);
+    const uint32_t s_k = smem_u32(ks) + gq * 128, s_v = smem_u32(vs) + gq * 128 + 4 * t;
     struct Raw {
       uint32_t k[2][D / 32], v[D / 16];               // codes of rows g and g + 8; words of V
       uint32_t kp[2][GROUPS], vp[2][2][GROUPS];       // pairs of rows g and g + 8; of keys 2 t + e + 8 u
@@ -416,18 +436,21 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
     Segment g;
     while (walk.next(plan, g)) {
       const int most = clamp((long long)g.base + g.first + g.tokens, 0, room);   // keys that any row sees
-      const int n = g.b1 - g.b0;
-      auto source = [&](int i) {   // of this warp's tile of block i: its number in the pool, or -1
-        const int x = kTiles * (g.b0 + i) + tile;
-        return i >= n || x * kKv4Tile >= most ? -1 : tile_source(p, g.at.s, g.at.slot, x);
+      const int n = g.b1 - g.b0, tiles = kTiles * n;
+      auto source = [&](int i) {   // of this warp's i-th tile: its number in the pool, or -1
+        const int q = mw + kMakers * i, x = kTiles * g.b0 + q;
+        return q >= tiles || x * kKv4Tile >= most ? -1 : tile_source(p, g.at.s, g.at.slot, x);
       };
       int now = source(lane), next = source(32 + lane);
       Raw raw, ahead;
       uint32_t v[D / 16], vp[2][2][GROUPS];   // of the block before
       bool v_beyond = false;
+      uint32_t v_block = 0;
+      int v_tile = -1;
       int from, then = __shfl_sync(0xffffffffu, now, 0);
       load(ahead, then);
-      for (int i = 0; i <= n; ++i) {
+      for (int i = 0, q = mw; q < tiles || v_tile >= 0; ++i, q += kMakers) {
+        const bool more = q < tiles;   // (after the last tile its V is left)
         raw = ahead;
         from = then;
         if (((i + 1) & 31) == 0) {
@@ -435,12 +458,12 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
           next = source(i + 33 + lane);
         }
         then = __shfl_sync(0xffffffffu, now, (i + 1) & 31);
-        if (i < n)
-          load(ahead, then);   // (of the block after the last: tile 0 of the pool, not used)
-        const uint32_t block = made + i;
-        const int key0 = (g.b0 + i) * kKeys + kKv4Tile * tile;
+        if (more)
+          load(ahead, then);   // (behind the last: tile 0 of the pool, not used)
+        const uint32_t block = made + q / kTiles;
+        const int tile = q % kTiles, key0 = (g.b0 + q / kTiles) * kKeys + kKv4Tile * tile;
         bool beyond = false;
-        if (i < n) {
+        if (more) {
           // ---- pairs: those of keys that nobody sees, and those that are not finite, are zero
           uint32_t k_bad = 0, v_bad[GROUPS] = {}, strange = 0;
           auto every = [&](auto f) {   // f(pair, key of the tile, mask of what is bad)
@@ -505,6 +528,7 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
               notes.v_bad[gr][tile] = (uint16_t)v_bad[gr];
             notes.special[tile] = (uint16_t)(any_bad ? 1u : hole);
           }
+          const uint32_t k_at = s_k + tile * (kKv4Tile * 128);
           auto make_k = [&](auto held) {
             constexpr bool HELD = decltype(held)::value;
 #pragma unroll
@@ -534,11 +558,12 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
           if (lane == 0)
             mbar_arrive(&bars.k_full);
         }
-        if (i > 0) {
-          // ---- V of the block before: words of dims 16 w + g (+ 8) and keys 2 t, 2 t + 1 (+ 8)
-          if (block > 1)
-            wait(ok, &bars.pv_done, block - 2, 745);
-          const int c = tile % 4 * 2;
+        if (v_tile >= 0) {
+          // ---- V of the tile before: words of dims 16 w + g (+ 8) and keys 2 t, 2 t + 1 (+ 8)
+          if (v_block > 0)
+            wait(ok, &bars.pv_done, v_block - 1, 745);
+          const int c = v_tile % 4 * 2;
+          const uint32_t v_at = s_v + v_tile / 4 * (D * 128);
           auto make_v = [&](auto held) {
             constexpr bool HELD = decltype(held)::value;
 #pragma unroll
@@ -570,7 +595,9 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
           if (lane == 0)
             mbar_arrive(&bars.v_full);
         }
-        if (i < n) {
+        v_tile = more ? tile : -1;
+        v_block = block;
+        if (more) {
 #pragma unroll
           for (int w = 0; w < D / 16; ++w)
             v[w] = raw.v[w];
@@ -651,7 +678,7 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
 }
 
 RaisedOn g_raised[2];
-constexpr int kMostSeqs = 1000;   // whose plan fits beside the operands
+constexpr int kMostSeqs = 800;   // whose plan fits beside the operands
 
 template <int D> int exact_launch(RaisedOn &raised, const Kv4Params &p, cudaStream_t st) {
   if (int rc = raise_shared_limit(raised, (const void *)kv4_exact_kernel<D>, Shape<D>::SMEM + RowsPlan::bytes(kMostSeqs)))

@@ -139,7 +139,7 @@ struct Meeting {
 };
 // This CTA's part is in memory; by THREADS threads of its first warps, a row (`at`) each.  Who completes the item adds its parts up, in their order.
 template <int D, int TYPE, int ROWS, int THREADS>
-__device__ __forceinline__ void meet(const Kv4Params &p, const RowsPlan &plan, const Segment &g, Meeting &m, int at, bool live, int64_t to) {
+__device__ __forceinline__ void meet(const Kv4Params &p, const RowsPlan &plan, const Segment &g, Meeting &m, int at, bool live, int64_t to, int d0 = 0, int d1 = D) {
   constexpr int GROUPS = D / kKv4Group, PART = rows_part<D, ROWS>();
   __threadfence();
   asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
@@ -172,7 +172,7 @@ __device__ __forceinline__ void meet(const Kv4Params &p, const RowsPlan &plan, c
       nan[gr] = nan[gr] || rest(b, 2 + gr) != 0.f;
   }
 #pragma unroll 1
-  for (int d = 0; d < D; d += 32) {
+  for (int d = d0; d < d1; d += 32) {
     float o[8][4] = {};
 #pragma unroll 2
     for (int b = from; b <= until; ++b) {
