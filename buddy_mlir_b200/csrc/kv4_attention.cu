@@ -758,7 +758,7 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
   cudaStream_t st = (cudaStream_t)stream;
   // Sequences of many rows go to tcgen05, in a launch of their own; who has how many rows is known on the device only, so both launches are made where
   // the mean does not say that there are none of one kind.
-  const bool exact = a->dtype == B200_F32;
+  const bool exact = a->dtype != B200_BF16;   // (a bf16 result is rounded eight times as far as f16 operands are)
   if ((exact ? kv4_exact_takes(p.G, a->n_seqs) : kv4_chunk_takes(p.G, a->n_seqs)) && (int64_t)a->rows * p.G >= kChunkRows && (int64_t)a->rows * p.G >= 24 * (int64_t)a->n_seqs) {
     const int from = (kChunkRows + p.G - 1) / p.G;
     Kv4Params chunk = p;

@@ -1,4 +1,4 @@
-// Attention over the 4-bit KV cache for sequences of many rows (a chunk of a prompt, or all of it) on the 5th-generation tensor cores.
+// Attention over the 4-bit KV cache for sequences of many bf16 rows (a chunk of a prompt, or all of it) on the 5th-generation tensor cores.
 //
 // Where many rows meet a key its 128 codes are better made values once: seven warps turn 128 keys into f16 operands (K [128][D], V
 // transposed [D][128], swizzled), two times 128 query rows are multiplied with them.  A code becomes f16 by way of 1024 + c; with its group's scale and
@@ -69,9 +69,9 @@ template <bool HELD> __device__ __forceinline__ uint32_t value2(uint32_t c, uint
   return x;
 }
 
-template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_constant__ Kv4Params p) {
+template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel(const __grid_constant__ Kv4Params p) {
   using H = Shape<D>;
-  constexpr int GROUPS = H::GROUPS;
+  constexpr int GROUPS = H::GROUPS, TYPE = B200_BF16;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t *qs = reinterpret_cast<uint8_t *>(((uintptr_t)smem + 1023) & ~(uintptr_t)1023);
   uint8_t *ks = qs + kSets * H::Q_BYTES, *vs = ks + kStages * H::KV_BYTES, *s_plan = vs + kStages * H::KV_BYTES;
@@ -153,7 +153,7 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
           for (int c = 0; c < D / 2; ++c)
             w[c] = live ? ((const uint16_t *)p.a.q)[q_row + 2 * c] | (uint32_t)((const uint16_t *)p.a.q)[q_row + 2 * c + 1] << 16 : 0u;
         }
-        auto two = [](uint32_t x) { return TYPE == B200_F16 ? halves(x) : make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); };
+        auto two = [](uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); };
         float most = 0.f, sum = 0.f;
 #pragma unroll
         for (int c = 0; c < D / 2; ++c) {
@@ -566,13 +566,13 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ch
   }
 }
 
-RaisedOn g_raised[4];
+RaisedOn g_raised[2];
 constexpr int kMostSeqs = 1500;   // whose plan fits beside the operands
 
-template <int D, int TYPE> int chunk_launch(RaisedOn &raised, const Kv4Params &p, cudaStream_t st) {
-  if (int rc = raise_shared_limit(raised, (const void *)kv4_chunk_kernel<D, TYPE>, Shape<D>::SMEM + RowsPlan::bytes(kMostSeqs)))
+template <int D> int chunk_launch(RaisedOn &raised, const Kv4Params &p, cudaStream_t st) {
+  if (int rc = raise_shared_limit(raised, (const void *)kv4_chunk_kernel<D>, Shape<D>::SMEM + RowsPlan::bytes(kMostSeqs)))
     return rc;
-  return launch_after(kv4_chunk_kernel<D, TYPE>, dim3(kKv4Ctas), kThreads, Shape<D>::SMEM + RowsPlan::bytes(p.a.n_seqs), st, p);
+  return launch_after(kv4_chunk_kernel<D>, dim3(kKv4Ctas), kThreads, Shape<D>::SMEM + RowsPlan::bytes(p.a.n_seqs), st, p);
 }
 
 } // namespace
@@ -586,9 +586,7 @@ int kv4_chunk_launch(Kv4Params p, int D, cudaStream_t st) {
   p.subs = 1;
   p.tokens = kSets * (kRows / p.G);
   p.over_heads = (65536 + p.heads - 1) / p.heads;
-  if (p.a.dtype == B200_F16)
-    return D == 128 ? chunk_launch<128, B200_F16>(g_raised[0], p, st) : chunk_launch<64, B200_F16>(g_raised[1], p, st);
-  return D == 128 ? chunk_launch<128, B200_BF16>(g_raised[2], p, st) : chunk_launch<64, B200_BF16>(g_raised[3], p, st);
+  return D == 128 ? chunk_launch<128>(g_raised[0], p, st) : chunk_launch<64>(g_raised[1], p, st);
 }
 
 } // namespace b200

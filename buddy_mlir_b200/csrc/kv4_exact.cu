@@ -1,15 +1,15 @@
-// Attention over the 4-bit KV cache for sequences of many f32 rows (a prompt, or a chunk of one) on the 5th-generation tensor cores.
+// Attention over the 4-bit KV cache for sequences of many f32 or f16 rows (a prompt, or a chunk of one) on the 5th-generation tensor cores.
 //
-// Products of f32's accuracy out of f16 operands: q and the weights are two f16 terms each (22 bits, after a power of two of the row), and so is what is left
+// Products of f32's accuracy out of f16 operands: q and the weights are two f16 terms each (22 bits, after a power of two of the row; q of f16 is one), and so is what is left
 // of a value once it is centred.  With v = (c - 8) s + m, m = lo + 8 s,
 //   q.k = sum over dims of q (c - 8) s + sum over groups of m (sum of q)       sum p v = sum p (c - 8) s + sum p m:
 // (c - 8) s has 15 bits at most, so that its rounding to f16 and what that leaves are two terms without any error, made by a product and an fma; the parts with m
-// are a few f32 operations of the thread that has the row.  Three of the four products of terms are summed, the small ones first; centred sums stay
-// small, which matters because the tensor cores' sums round towards zero.
+// are a few f32 operations of the thread that has the row.  Three of the four products of terms are summed, the small ones first, and a block's product is added to
+// those before it outside the tensor cores, whose sums round towards zero: eight such steps count, of centred values.
 //
 // Seven warps make the operands of 128 keys: K of a block while the softmax has the one before it, V when the product of the block before is done.  Eight
 // do the softmax, two threads per row: scores of half a block each, the larger of their maxima (through shared memory) decides whether the row's
-// reference moves, weights.  Scores of two blocks have their own columns (2 x 128, and D for O).
+// reference moves, weights.  Scores of two blocks have their own columns (2 x 128), O and its sum D each.
 //
 // A prompt of 1000 rows, 12 heads on 2 of 128 dims: 51 us (the few-rows form 70): 96 items on as many CTAs, the longest of eight blocks, and a block takes 6700 clocks,
 // 6200 of them the softmax at one warp a scheduler, 2300 the products.  Items that CTAs share come together too slowly to be worth it (78 us).
@@ -32,7 +32,7 @@ template <int D> struct Shape {
   static constexpr uint32_t TERM = kRows * D * 2;   // bytes of a term of q, K or V
   static constexpr int PART = rows_part<D, kRows>();
   static constexpr int SMEM = 1024 + 6 * TERM;
-  static constexpr uint32_t COL_S = 0, COL_O = 2 * kKeys;
+  static constexpr uint32_t COL_S = 0, COL_O = 2 * kKeys, COL_SUM = COL_O + kRows;   // (a block's product; those of the blocks before)
 };
 
 // What the softmax has to know of a block's keys.
@@ -72,7 +72,7 @@ template <bool HELD> __device__ __forceinline__ void terms(uint32_t c, uint32_t 
   low = fma2(c, s, high ^ 0x80008000u);
 }
 
-template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel(const __grid_constant__ Kv4Params p) {
+template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel(const __grid_constant__ Kv4Params p) {
   using H = Shape<D>;
   constexpr int GROUPS = H::GROUPS;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -112,7 +112,7 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
     const int lo = plan.r0[0], hi = max(lo, plan.r0[plan.n]), none = lo + p.a.rows - hi, cols = p.a.q_heads * D;
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)none * cols; i += (int64_t)gridDim.x * kThreads) {
       const int r = (int)(i / cols);
-      put<B200_F32>(p, (int64_t)(r < lo ? r : hi + r - lo) * p.a.out_ld + i % cols, 0.f);
+      put<TYPE>(p, (int64_t)(r < lo ? r : hi + r - lo) * p.a.out_ld + i % cols, 0.f);
     }
   }
   const bool works = plan.total > 0 && (int)blockIdx.x < plan.ctas;
@@ -124,7 +124,7 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
   if (works && warp < kSoftmaxWarps) {
     // ---- softmax: two threads per row, of half a block's keys each ----------------------------------------------------------------------
     const int row = (warp & 3) * 32 + lane, side = warp >> 2;
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), col_o = lanes + H::COL_O + side * (D / 2);
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), col_o = lanes + H::COL_O + side * (D / 2), col_sum = lanes + H::COL_SUM + side * (D / 2);
     auto pair_meets = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory"); };   // (the two warps of the same rows)
     bool ok = true;
     uint32_t made = 0;
@@ -152,16 +152,15 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
           for (int b = 0; b < BATCH; ++b) {
             float (&x)[4] = batch[b];
             const int64_t at = __shfl_sync(0xffffffffu, mine, which(b));
-            const float *q = (const float *)p.a.q + max(at, (int64_t)0) + d;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               x[e] = 0.f;
             if (at >= 0 && p.wide_q)
-              *reinterpret_cast<float4 *>(x) = __ldg(reinterpret_cast<const float4 *>(q));
+              load_wide<TYPE>(p.a.q, at + d, x);
             else if (at >= 0)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                x[e] = __ldg(q + e);
+                x[e] = load_as_float(p.a.q, TYPE, at + d + e);
           }
 #pragma unroll
           for (int b = 0; b < BATCH; ++b) {
@@ -190,10 +189,12 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
               bars.row[at][1 + lane % LANES / 16] = sum[b] * p.log2_scale;
             const float a[4] = {x[0] * by, x[1] * by, x[2] * by, x[3] * by};
             const uint32_t high[2] = {pack_f16(a[0], a[1]), pack_f16(a[2], a[3])};
-            const float2 f = halves(high[0]), h = halves(high[1]);
             const uint32_t to = smem_u32(qs) + at * 128 + d / 64 * (kRows * 128) + ((d / 8 % 8 ^ (at & 7)) << 4) + d % 8 * 2;
             store2(to, high[0], high[1]);
-            store2(to + H::TERM, pack_f16(a[0] - f.x, a[1] - f.y), pack_f16(a[2] - h.x, a[3] - h.y));
+            if constexpr (TYPE == B200_F32) {
+              const float2 f = halves(high[0]), h = halves(high[1]);
+              store2(to + H::TERM, pack_f16(a[0] - f.x, a[1] - f.y), pack_f16(a[2] - h.x, a[3] - h.y));
+            }
           }
         }
         fence_proxy();
@@ -213,6 +214,27 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
       for (uint32_t j = 0; j < n; ++j) {
         const uint32_t block = made + j, col_s = lanes + H::COL_S + (block & 1) * kKeys + side * (kKeys / 2);
         const int key0 = (g.b0 + j) * kKeys, seen = min(max(seen_by - key0, 0), kKeys);   // keys of the block that this row sees
+        if (j > 0) {
+          // ---- the block before's product joins the sum, with rounding to nearest
+          // (every product is waited for before the next can begin: a wait tells one phase from its neighbours only)
+          wait(ok, &bars.pv_done, block - 1, 743);
+          fence_after();
+#pragma unroll 1
+          for (int i = 0; i < D / 2; i += 32) {
+            uint32_t w[32], sum[32];
+            tmem_load32(col_o + i, w);
+            tmem_arrived(w);
+            if (j > 1) {
+              tmem_load32(col_sum + i, sum);
+              tmem_arrived(sum);
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                w[e] = __float_as_uint(__uint_as_float(w[e]) + __uint_as_float(sum[e]));
+            }
+            tmem_store32(col_sum + i, w);
+          }
+          tmem_wait_store();
+        }
         wait(ok, &bars.s_full[block & 1], block >> 1, 741);
         fence_after();
         // (the makers wrote them before the products that have been waited for could begin; another block's come four blocks later)
@@ -276,20 +298,17 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
 #pragma unroll
           for (int gr = 0; gr < GROUPS; ++gr)
             bias[gr] = mul_2(bias[gr], pack2(keep, keep));
-          if (j > 0) {
-            wait(ok, &bars.pv_done, block - 1, 742);
-            fence_after();
+          if (j > 0)
 #pragma unroll 1
             for (int i = 0; i < D / 2; i += 32) {
               uint32_t w[32];
-              tmem_load32(col_o + i, w);
+              tmem_load32(col_sum + i, w);
               tmem_arrived(w);
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 w[e] = __float_as_uint(__uint_as_float(w[e]) * keep);
-              tmem_store32(col_o + i, w);
+              tmem_store32(col_sum + i, w);
             }
-          }
         }
         // ---- weights, as two f16 in the place of the scores that they were
         auto weigh = [&](auto hidden) {
@@ -342,8 +361,6 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
           weigh(std::true_type());
         else
           weigh(std::false_type());
-        if (j > 0)   // every product is waited for before the next can begin: a wait tells one phase from its neighbours only
-          wait(ok, &bars.pv_done, block - 1, 743);
         tmem_wait_store();
         fence_before();
         __syncwarp();
@@ -377,13 +394,21 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
         uint32_t w[32];
         tmem_load32(col_o + c, w);
         tmem_arrived(w);
+        if (n > 1) {
+          uint32_t sum[32];
+          tmem_load32(col_sum + c, sum);
+          tmem_arrived(sum);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            w[e] = __float_as_uint(__uint_as_float(w[e]) + __uint_as_float(sum[e]));
+        }
         if (live) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             const float o[4] = {__uint_as_float(w[e]) + b, __uint_as_float(w[e + 1]) + b, __uint_as_float(w[e + 2]) + b, __uint_as_float(w[e + 3]) + b};
             const int d = side * (D / 2) + c + e;
             if (whole)
-              put_over<B200_F32>(p, to + d, o, l, marks >> gr & 1);
+              put_over<TYPE>(p, to + d, o, l, marks >> gr & 1);
             else
               __stcg(reinterpret_cast<float4 *>(part) + d / 4 * kRows + row, make_float4(o[0], o[1], o[2], o[3]));
           }
@@ -400,7 +425,7 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
         for (int i = 0; i < GROUPS; ++i)
           rest[(2 + i) * kRows + row] = marks >> i & 1 ? 1.f : 0.f;
       }
-      meet<D, B200_F32, kRows, 32 * kSoftmaxWarps>(p, plan, g, bars.meeting, row, live, to, side * (D / 2), (side + 1) * (D / 2));
+      meet<D, TYPE, kRows, 32 * kSoftmaxWarps>(p, plan, g, bars.meeting, row, live, to, side * (D / 2), (side + 1) * (D / 2));
     }
   } else if (works && warp < kSoftmaxWarps + kMakers) {
     // ---- makers: every seventh tile each; K of a tile, then V of the one before ------------------------------------------------------------
@@ -622,17 +647,18 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
     uint32_t made = 0, segments = 0;
     // the small products first: terms of the first operand and of the second
     constexpr uint32_t FIRST[3] = {1, 0, 0}, SECOND[3] = {0, 1, 0};
+    constexpr int LEAST = TYPE == B200_F32 ? 0 : 1;   // (q of f16 is one term)
     auto scores = [&](uint32_t block) {
       wait(ok, &bars.k_full, block, 746);
       if (!ok)
         return;
       fence_after();
 #pragma unroll
-      for (int i = 0; i < 3; ++i)
+      for (int i = LEAST; i < 3; ++i)
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           mma_ss<kKeys>(leader, tmem + H::COL_S + (block & 1) * kKeys, dq + ((FIRST[i] * H::TERM + (k >> 2) * (kRows * 128) + (k & 3) * 32) >> 4),
-                        dk + ((SECOND[i] * H::TERM + (k >> 2) * (kKeys * 128) + (k & 3) * 32) >> 4), (i | k) != 0);
+                        dk + ((SECOND[i] * H::TERM + (k >> 2) * (kKeys * 128) + (k & 3) * 32) >> 4), (i - LEAST | k) != 0);
       if (leader)
         tc_commit(&bars.s_full[block & 1]);
     };
@@ -658,7 +684,7 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k)   // (weights: of 32 keys sixteen columns of each term)
             mma_ts<D>(leader, tmem + H::COL_O, tmem + H::COL_S + (block & 1) * kKeys + (k >> 1) * 32 + FIRST[i] * 16 + (k & 1) * 8,
-                      dv + ((SECOND[i] * H::TERM + (k >> 2) * (D * 128) + (k & 3) * 32) >> 4), (j | i | k) != 0);
+                      dv + ((SECOND[i] * H::TERM + (k >> 2) * (D * 128) + (k & 3) * 32) >> 4), (i | k) != 0);
         if (leader)
           tc_commit(&bars.pv_done);
       }
@@ -677,13 +703,13 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_exact_kernel
   }
 }
 
-RaisedOn g_raised[2];
+RaisedOn g_raised[4];
 constexpr int kMostSeqs = 800;   // whose plan fits beside the operands
 
-template <int D> int exact_launch(RaisedOn &raised, const Kv4Params &p, cudaStream_t st) {
-  if (int rc = raise_shared_limit(raised, (const void *)kv4_exact_kernel<D>, Shape<D>::SMEM + RowsPlan::bytes(kMostSeqs)))
+template <int D, int TYPE> int exact_launch(RaisedOn &raised, const Kv4Params &p, cudaStream_t st) {
+  if (int rc = raise_shared_limit(raised, (const void *)kv4_exact_kernel<D, TYPE>, Shape<D>::SMEM + RowsPlan::bytes(kMostSeqs)))
     return rc;
-  return launch_after(kv4_exact_kernel<D>, dim3(kKv4Ctas), kThreads, Shape<D>::SMEM + RowsPlan::bytes(p.a.n_seqs), st, p);
+  return launch_after(kv4_exact_kernel<D, TYPE>, dim3(kKv4Ctas), kThreads, Shape<D>::SMEM + RowsPlan::bytes(p.a.n_seqs), st, p);
 }
 
 } // namespace
@@ -695,7 +721,9 @@ int kv4_exact_launch(Kv4Params p, int D, cudaStream_t st) {
   p.subs = 1;
   p.tokens = kRows / p.G;
   p.over_heads = (65536 + p.heads - 1) / p.heads;
-  return D == 128 ? exact_launch<128>(g_raised[0], p, st) : exact_launch<64>(g_raised[1], p, st);
+  if (p.a.dtype == B200_F16)
+    return D == 128 ? exact_launch<128, B200_F16>(g_raised[0], p, st) : exact_launch<64, B200_F16>(g_raised[1], p, st);
+  return D == 128 ? exact_launch<128, B200_F32>(g_raised[2], p, st) : exact_launch<64, B200_F32>(g_raised[3], p, st);
 }
 
 } // namespace b200

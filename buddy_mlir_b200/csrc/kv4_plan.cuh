@@ -369,7 +369,7 @@ __device__ __forceinline__ int tile_source(const Kv4Params &p, int s, int kv, in
   return id < 0 || id >= p.n_pages ? -1 : (id * p.kv_heads + kv) * per_page + t % per_page;
 }
 
-// sequences of many rows, on tcgen05: kv4_chunk.cu (16-bit rows), kv4_exact.cu (f32)
+// sequences of many rows, on tcgen05: kv4_chunk.cu (bf16), kv4_exact.cu (f32 and f16)
 int64_t kv4_chunk_part_floats(int D);   // of a CTA's two parts
 bool kv4_chunk_takes(int G, int n_seqs);
 int kv4_chunk_launch(Kv4Params p, int D, cudaStream_t st);

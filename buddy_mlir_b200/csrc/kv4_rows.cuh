@@ -1,4 +1,4 @@
-// What the forms of the 4-bit cache's attention for sequences of many rows share (kv4_chunk.cu: 16-bit rows, kv4_exact.cu: f32): blocks of 128 keys by 128 query
+// What the forms of the 4-bit cache's attention for sequences of many rows share (kv4_chunk.cu: bf16, kv4_exact.cu: f32 and f16): blocks of 128 keys by 128 query
 // rows on tcgen05, an item's parts and how they meet.
 #pragma once
 #include "kv4_plan.cuh"
