@@ -26,6 +26,7 @@ constexpr int kRows = 8;            // query rows of an item: a position's heads
 constexpr int kSlots = 4;           // tiles that a warp has in flight or in hand
 constexpr int kChunkRows = 64;     // query vectors of a sequence and kv head from which on tcgen05 has them
 constexpr int kLeastKeys = 512, kSplit = 1000;     // of a CTA, where there are not more CTAs than that asks for
+constexpr float kFew = 0.9f;           // of a lane's sum of weights: a key that has more of it is one of few
 constexpr float kLeastScale = 5.9604645e-8f;   // (f16's smallest: a group of equal values has the scale 0)
 
 __host__ __device__ constexpr int part_floats(int D) { return kRows * (D + 4) + 2 * kRows; }   // sums in rows of D + 4, maxima, totals
@@ -269,6 +270,11 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
         s[n][e] = ex2(s[n][e] - r[e & 1]);
         l[e & 1] += s[n][e];
       }
+      // Weights are rounded to f16, as the result is; of many keys that averages out.  Where a key is a quarter of a lane's or more, what the rounding left counts
+      // too.  (bf16 results are rounded eight times as far, f32 weights have two terms.)
+      bool few = false;
+      if constexpr (TYPE == B200_F16)
+        few = __any_sync(0xffffffffu, fmaxf(s[n][0], s[n][2]) > kFew * l[0] || fmaxf(s[n][1], s[n][3]) > kFew * l[1]);
 #pragma unroll
       for (int gr = 0; gr < GROUPS; ++gr) {
         float w[4];
@@ -298,6 +304,21 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
         }
         uint32_t vw[4];
         *reinterpret_cast<uint4 *>(vw) = *reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + gr * 512 + lane * 16);
+        if constexpr (TYPE == B200_F16)
+          if (few) {
+            const uint32_t kept[2] = {pack_f16(w[0], w[1]), pack_f16(w[2], w[3])};
+            const float2 x = halves(kept[0]), y = halves(kept[1]);
+            const float left[4] = {w[0] - x.x, w[1] - x.y, w[2] - y.x, w[3] - y.y};
+            const uint32_t b2 = transpose8(pack_f16(left[0], left[1])), b3 = transpose8(pack_f16(left[2], left[3]));
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              bias[gr][e] = fmaf(-kCentre, left[e] + left[2 + e], bias[gr][e]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t a[4] = {low_codes(vw[i]), high_codes(vw[i]), low_codes(vw[i] >> 8), high_codes(vw[i] >> 8)};
+              mma(o[4 * gr + i], a, b2, b3);
+            }
+          }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if constexpr (!EXACT) {
