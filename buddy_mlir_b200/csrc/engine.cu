@@ -2113,9 +2113,11 @@ static int batch_rows(b200_batch *b, int M, const int32_t *tokens, const int32_t
   std::vector<int32_t> next(next_host ? logit_rows : 0);
   if (next_host)
     B200_CUDA(cudaMemcpyAsync(next.data(), b->d_next, (size_t)logit_rows * 4, cudaMemcpyDeviceToHost, st));
-  int32_t status = 0;
-  if (b->kv4)
+  int32_t status = 0, gave_up = 0;
+  if (b->kv4) {
     B200_CUDA(cudaMemcpyAsync(&status, b->d_status, 4, cudaMemcpyDeviceToHost, st));
+    B200_CUDA(cudaMemcpyAsync(&gave_up, b200::kv4_attention_error(b->work4), 4, cudaMemcpyDeviceToHost, st));
+  }
   if (int rc = rows_status_queue(m)) return rc;
   B200_CUDA(cudaStreamSynchronize(st));
   for (int r = 0; r < (int)next.size(); ++r)
@@ -2123,7 +2125,11 @@ static int batch_rows(b200_batch *b, int M, const int32_t *tokens, const int32_t
   B200_CUDA(cudaEventElapsedTime(&b->last_ms, m->ev0, m->ev1));
   if (status != 0)
     return fail(B200_ESTATE, "batch: the page allocator refused a step (%d)", status);
-  return rows_status(m);   // (the 4-bit cache's attention has no bounded waits in f32)
+  if (gave_up != 0) {
+    B200_CUDA(cudaMemsetAsync(b->work4, 0, (size_t)b->work4_bytes, st));
+    return fail(B200_ECUDA, "batch: a bounded wait of the attention gave up (code %d)", gave_up);
+  }
+  return rows_status(m);
 }
 
 // pages for positions [len, len + n) of a sequence
@@ -2172,7 +2178,7 @@ static int batch_create(b200_model *m, int max_seqs, int page_size, int n_pages,
     if (max_seqs > B200_KV4_ATTENTION_MAX_SEQS)
       return fail(B200_ELIMIT, "batch_create: %d sequences (at most %d with a 4-bit cache)", max_seqs, B200_KV4_ATTENTION_MAX_SEQS);
   }
-  if (((int64_t)max_context + page_size - 1) / page_size * page_size > INT32_MAX - 64)
+  if (((int64_t)max_context + page_size - 1) / page_size * page_size > (kv4 ? 1 << 30 : INT32_MAX - 64))   // (4-bit: what its attention takes)
     return fail(B200_EINVAL, "batch_create: a context of %d positions", max_context);
   b200_batch *b = new b200_batch();
   b->m = m;

@@ -21,5 +21,7 @@ int kv4_check(const char *call, const b200_kv4_cache *c);
 int page_step_launch(const b200_page_step_args &a, cudaStream_t st);
 int kv4_write_launch(const b200_kv4_cache &c, const void *k, int64_t k_ld, const void *v, int64_t v_ld, int dtype, const int64_t *slots, int rows,
                      cudaStream_t st);
+// kv4_attention.cu: the word of a workspace that says which bounded wait gave up (0: none)
+const int *kv4_attention_error(const void *workspace);
 
 } // namespace b200

@@ -705,6 +705,8 @@ template <int D, int TYPE> int attention_launch(RaisedOn &raised, const Kv4Param
 
 } // namespace
 
+const int *kv4_attention_error(const void *workspace) { return (const int *)workspace + kKv4Ctas; }
+
 } // namespace b200
 
 using namespace b200;
@@ -722,8 +724,8 @@ int b200_kv4_attention_status(void *workspace, void *stream) {
     return fail(B200_EINVAL, "kv4_attention_status: null workspace");
   if (int rc = ensure_device())
     return rc;
-  int code = 0, *at = (int *)workspace + kKv4Ctas;
-  B200_CUDA(cudaMemcpyAsync(&code, at, 4, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
+  int code = 0;
+  B200_CUDA(cudaMemcpyAsync(&code, kv4_attention_error(workspace), 4, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
   B200_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
   return code == 0 ? B200_OK : fail(B200_ECUDA, "kv4_attention: a bounded wait gave up (code %d)", code);
 }

@@ -1,7 +1,7 @@
 // Attention over the 4-bit KV cache for sequences of many f32 or f16 rows (a prompt, or a chunk of one) on the 5th-generation tensor cores.
 //
-// Products of f32's accuracy out of f16 operands: q and the weights are two f16 terms each (22 bits, after a power of two of the row; q of f16 is one), and so is what is left
-// of a value once it is centred.  With v = (c - 8) s + m, m = lo + 8 s,
+// Products of f32's accuracy out of f16 operands: q and the weights are two f16 terms each (22 bits, after a power of two of the row; q of f16 is one), and so
+// is what is left of a value once it is centred.  With v = (c - 8) s + m, m = lo + 8 s,
 //   q.k = sum over dims of q (c - 8) s + sum over groups of m (sum of q)       sum p v = sum p (c - 8) s + sum p m:
 // (c - 8) s has 15 bits at most, so that its rounding to f16 and what that leaves are two terms without any error, made by a product and an fma; the parts with m
 // are a few f32 operations of the thread that has the row.  Three of the four products of terms are summed, the small ones first, and a block's product is added to
@@ -11,8 +11,10 @@
 // do the softmax, two threads per row: scores of half a block each, the larger of their maxima (through shared memory) decides whether the row's
 // reference moves, weights.  Scores of two blocks have their own columns (2 x 128), O and its sum D each.
 //
-// A prompt of 1000 rows, 12 heads on 2 of 128 dims: 51 us (the few-rows form 70): 96 items on as many CTAs, the longest of eight blocks, and a block takes 6700 clocks,
-// 6200 of them the softmax at one warp a scheduler, 2300 the products.  Items that CTAs share come together too slowly to be worth it (78 us).
+// A prompt of 1000 f32 rows, 12 heads on 2 of 128 dims: 53 us (the few-rows form 70), errors 2.8e-7 of the result; 4000 rows: 412 us, 119 TFLOP/s.  A block takes some
+// 8000 clocks, 5400 of them the softmax, and 2300 for the products: a tile's K takes a maker 2300, its V 1450, and of seven makers one has two tiles.  Eight
+// (17 warps of 96 registers) spill, 63 us; one thread per row and eight makers take as long here and 13 % longer at 4000 rows.  Items that CTAs share come together too
+// slowly to be worth it (78 us).  f16, 1001 rows at 4000 keys, 32 heads on 8: 256 us (kv4_chunk.cu, whose errors would be 2.5 times f16's rounding: 115).
 #include "kv4_rows.cuh"
 
 #include <algorithm>

@@ -356,9 +356,9 @@ int b200_page_step(const b200_page_step_args *a, void *stream);
  * scores, sums and products with f32 accumulators, rounded to `dtype` once.
  * Codes count exactly.  dtype f32: q and the weights to 2^-22 of themselves.  bf16
  * and f16: q exactly (elements down to 2^-28 of their row's largest), the weights
- * to 2^-11; the sequences with 64 or more query vectors per kv head (rows times q
- * heads that share it) may take the cache's values rounded to f16 as well, 2^-11
- * each.  A row that sees no position is zero, and so are the rows before
+ * to 2^-11 (f16: those that are most of a sum to 2^-22).  bf16 sequences with 64 or
+ * more query vectors per kv head (rows times q heads that share it) may take the
+ * cache's values rounded to f16 as well, 2^-11 each.  A row that sees no position is zero, and so are the rows before
  * row_start[0] and behind the last sequence's.  Positions beyond
  * table_stride * page, and those whose table entry is no page of the pool, are
  * not seen.  Nothing that a row does not see (infinities and NaN included)
@@ -386,7 +386,8 @@ int b200_kv4_attention(const b200_kv4_cache *c,
                        const b200_kv4_attention_args *a, void *workspace,
                        int64_t workspace_bytes, void *stream);
 /* Waits for `stream`: B200_ECUDA when a bounded wait of a call with this workspace gave up
- * since it was zeroed (its results are not to be used then). */
+ * since it was zeroed (its results are not to be used then; zero it again before
+ * the next call). */
 int b200_kv4_attention_status(void *workspace, void *stream);
 
 /* ------------------------------------------------------------------------
