@@ -779,20 +779,30 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
   p.tokens = p.subs == 1 ? kRows / p.G : 1;
   p.over_heads = (65536 + p.heads - 1) / p.heads;
   cudaStream_t st = (cudaStream_t)stream;
-  // Sequences of many rows go to tcgen05, in a launch of their own; who has how many rows is known on the device only, so both launches are made where
-  // the mean does not say that there are none of one kind.
+  // Sequences of many rows go to tcgen05, in a launch of their own, if there is enough to do (kWork: products of a query vector and a key): a form's beginnings and
+  // ends take 35 (bf16) or 50 us where the few-rows form has 12.  Who has how many rows is known on the device only, so both launches are made where the sizes
+  // leave it open, and both see from the lengths whose the sequences are.
+  // (Few rows, many rows, us; 1000 keys, f32 12 heads on 2, else 32 on 8: f32 20 x 22 rows 54 / 59, 20 x 43 96 / 59; bf16 20 x 16 53 / 71, 20 x 32 88 / 73; f16 20 x 32
+  // 91 / 103, 20 x 64 162 / 150; one sequence of 11 rows of f32 18 / 49.)
   const bool exact = a->dtype != B200_BF16;   // (a bf16 result is rounded eight times as far as f16 operands are)
-  if ((exact ? kv4_exact_takes(p.G, a->n_seqs) : kv4_chunk_takes(p.G, a->n_seqs)) && (int64_t)a->rows * p.G >= kChunkRows && (int64_t)a->rows * p.G >= 24 * (int64_t)a->n_seqs) {
-    const int from = (kChunkRows + p.G - 1) / p.G;
+  const double work = a->dtype == B200_F32 ? 5.5e6 : exact ? 30e6 : 15e6, vectors = (double)a->rows * a->q_heads;
+  if ((exact ? kv4_exact_takes(p.G, a->n_seqs) : kv4_chunk_takes(p.G, a->n_seqs)) && (int64_t)a->rows * p.G >= kChunkRows &&
+      (int64_t)a->rows * p.G >= 24 * (int64_t)a->n_seqs && vectors * a->table_stride * c->page >= work) {
+    const bool only = a->n_seqs == 1 && vectors * a->rows / 2 >= work;   // (rows that see one another, if nothing before them)
     Kv4Params chunk = p;
-    if (a->n_seqs > 1) {
-      p.most_rows = from - 1;
-      chunk.least_rows = from;
+    chunk.least_rows = (kChunkRows + p.G - 1) / p.G;
+    chunk.many = true;
+    if (only) {
+      chunk.least_rows = 1;
+    } else {
+      p.most_rows = chunk.least_rows - 1;
+      p.many_rows = chunk.many_rows = chunk.least_rows;
+      p.least_work = chunk.least_work = std::max<int64_t>(1, (int64_t)(work / a->q_heads));
       chunk.fill = 0;
     }
     if (int rc = exact ? kv4_exact_launch(chunk, c->head_dim, st) : kv4_chunk_launch(chunk, c->head_dim, st))
       return rc;
-    if (a->n_seqs == 1)
+    if (only)
       return B200_OK;
   }
 #define B200_D(D_)                                                                                                                    \

@@ -3,6 +3,8 @@
 #pragma once
 #include "kv4.cuh"
 
+#include <climits>
+
 namespace b200 {
 
 constexpr int kKv4Ctas = 148;          // of a launch at most
@@ -21,6 +23,9 @@ struct Kv4Params {
   int heads, tokens, subs;          // of an item: q heads, positions; items that share a position's kv head
   int over_heads;                   // 2^16 / heads, rounded up
   int least_rows, most_rows;        // sequences of this launch: by their rows
+  int many_rows;                    // from how many rows on a sequence counts as one of many;
+  long long least_work;             // where less work than this is in those (rows times keys), the few-rows form has them too (0: not looked at)
+  bool many;                        // this launch is the many-rows form
   int fill;                         // 1: rows of no sequence are zeroed here
   float log2_scale;
   bool wide_q, wide_out, wide_q16;  // rows are aligned to four elements; to 16 bytes
@@ -158,10 +163,31 @@ template <int SHIFT> struct KeyPlan {
     tokens = p.tokens;
     slots = p.kv_heads * p.subs;
     long long *s_cost = reinterpret_cast<long long *>(memory);
-    int *s_r0 = reinterpret_cast<int *>(s_cost + n + 1), *s_base = s_r0 + n + 1, *s_items = s_base + n, *longest = reinterpret_cast<int *>(sums + 2 * (THREADS / 32));
-    if (tid == 0)
-      *longest = 0;
+    int *s_r0 = reinterpret_cast<int *>(s_cost + n + 1), *s_base = s_r0 + n + 1, *s_items = s_base + n;
     const int per = (n + THREADS - 1) / THREADS, first = min(n, tid * per), last = min(n, first + per);
+    int least_rows = p.least_rows, most_rows = p.most_rows;
+    if (p.least_work > 0) {   // (both launches come to the same)
+      unsigned long long work = 0;
+      for (int s = first; s < last; ++s) {
+        const int rows = max(clamp(p.a.row_start[s + 1], 0, p.a.rows) - clamp(p.a.row_start[s], 0, p.a.rows), 0);
+        if (rows >= p.many_rows)
+          work += (unsigned long long)rows * (unsigned)(clamp((long long)p.a.lens[s] - rows, 0, room) + rows / 2);
+      }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1)
+        work += __shfl_xor_sync(0xffffffffu, work, o);
+      if (lane == 0)
+        sums[warp] = (long long)work;
+      __syncthreads();
+      work = 0;
+      for (int w = 0; w < THREADS / 32; ++w)
+        work += (unsigned long long)sums[w];
+      __syncthreads();
+      if (work < (unsigned long long)p.least_work) {
+        least_rows = p.many ? INT_MAX : 0;
+        most_rows = INT_MAX;
+      }
+    }
     long long sum = 0;
     int count = 0, most = 0;
     for (int s = first; s < last; ++s) {
@@ -174,7 +200,7 @@ template <int SHIFT> struct KeyPlan {
       const Sequence q(a, b, at, tokens);
       s_cost[s] = sum;
       s_items[s] = count;
-      if (rows >= p.least_rows && rows <= p.most_rows) {
+      if (rows >= least_rows && rows <= most_rows) {
         sum += slots * q.before(q.tiles, tokens);
         count = (int)min((long long)count + (long long)slots * q.tiles, (long long)kNone);
         most = max(most, q.past + rows + kKv4Item);
