@@ -26,7 +26,9 @@ constexpr int kRows = 8;            // query rows of an item: a position's heads
 constexpr int kSlots = 4;           // tiles that a warp has in flight or in hand
 constexpr int kChunkRows = 64;     // query vectors of a sequence and kv head from which on tcgen05 has them
 constexpr int kLeastKeys = 512, kSplit = 1000;     // of a CTA, where there are not more CTAs than that asks for
-constexpr float kFew = 0.9f;           // of a lane's sum of weights: a key that has more of it is one of few
+// of a lane's sum of weights: a key that has more of it is one of few (short f16 contexts: errors 2.1e-4, as with 0.25, where a step of 200 sequences takes 5 % longer; all
+// rounded 3.0e-4 and 8 % shorter)
+constexpr float kFew = 0.9f;
 constexpr float kLeastScale = 5.9604645e-8f;   // (f16's smallest: a group of equal values has the scale 0)
 
 __host__ __device__ constexpr int part_floats(int D) { return kRows * (D + 4) + 2 * kRows; }   // sums in rows of D + 4, maxima, totals
@@ -270,8 +272,7 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
         s[n][e] = ex2(s[n][e] - r[e & 1]);
         l[e & 1] += s[n][e];
       }
-      // Weights are rounded to f16, as the result is; of many keys that averages out.  Where a key is a quarter of a lane's or more, what the rounding left counts
-      // too.  (bf16 results are rounded eight times as far, f32 weights have two terms.)
+      // Weights are rounded to f16, as the result is; of many keys that averages out.  Where a key is most of a lane's, what the rounding left counts too.  (bf16 results are rounded eight times as far, f32 weights have two terms.)
       bool few = false;
       if constexpr (TYPE == B200_F16)
         few = __any_sync(0xffffffffu, fmaxf(s[n][0], s[n][2]) > kFew * l[0] || fmaxf(s[n][1], s[n][3]) > kFew * l[1]);
@@ -779,7 +780,7 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
   p.tokens = p.subs == 1 ? kRows / p.G : 1;
   p.over_heads = (65536 + p.heads - 1) / p.heads;
   cudaStream_t st = (cudaStream_t)stream;
-  // Sequences of many rows go to tcgen05, in a launch of their own, if there is enough to do (kWork: products of a query vector and a key): a form's beginnings and
+  // Sequences of many rows go to tcgen05, in a launch of their own, if there is enough to do (pairs of a query vector and a key): the form's beginnings and
   // ends take 35 (bf16) or 50 us where the few-rows form has 12.  Who has how many rows is known on the device only, so both launches are made where the sizes
   // leave it open, and both see from the lengths whose the sequences are.
   // (Few rows, many rows, us; 1000 keys, f32 12 heads on 2, else 32 on 8: f32 20 x 22 rows 54 / 59, 20 x 43 96 / 59; bf16 20 x 16 53 / 71, 20 x 32 88 / 73; f16 20 x 32

@@ -14,7 +14,7 @@
 // A prompt of 1000 f32 rows, 12 heads on 2 of 128 dims: 53 us (the few-rows form 70), errors 2.8e-7 of the result; 4000 rows: 412 us, 119 TFLOP/s.  A block takes some
 // 8000 clocks, 5400 of them the softmax, and 2300 for the products: a tile's K takes a maker 2300, its V 1450, and of seven makers one has two tiles.  Eight
 // (17 warps of 96 registers) spill, 63 us; one thread per row and eight makers take as long here and 13 % longer at 4000 rows.  Items that CTAs share come together too
-// slowly to be worth it (78 us).  f16, 1001 rows at 4000 keys, 32 heads on 8: 256 us (kv4_chunk.cu, whose errors would be 2.5 times f16's rounding: 115).
+// slowly to be worth it (78 us).  f16, 1001 rows at 4000 keys, 32 heads on 8: 264 us (kv4_chunk.cu, whose errors would be 2.5 times f16's rounding: 119).
 #include "kv4_rows.cuh"
 
 #include <algorithm>

@@ -138,6 +138,28 @@ template <typename I> __device__ __forceinline__ I share(I x, int a, int b) {
   }
 }
 
+// Rows times keys of the sequences of many rows, by all THREADS of the CTA.  (Out of the way of the kernels' code.)
+template <int THREADS> __device__ __noinline__ unsigned long long many_work(const Kv4Params &p, long long *sums) {
+  const int room = p.a.table_stride * p.page;
+  unsigned long long work = 0;
+  for (int s = threadIdx.x; s < p.a.n_seqs; s += THREADS) {
+    const int rows = max(clamp(p.a.row_start[s + 1], 0, p.a.rows) - clamp(p.a.row_start[s], 0, p.a.rows), 0);
+    if (rows >= p.many_rows)
+      work += (unsigned long long)rows * (unsigned)(clamp((long long)p.a.lens[s] - rows, 0, room) + rows / 2);
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+    work += __shfl_xor_sync(0xffffffffu, work, o);
+  if (threadIdx.x % 32 == 0)
+    sums[threadIdx.x / 32] = (long long)work;
+  __syncthreads();
+  work = 0;
+  for (int w = 0; w < THREADS / 32; ++w)
+    work += (unsigned long long)sums[w];
+  __syncthreads();
+  return work;
+}
+
 // An item and the first of its tiles that is meant.
 struct Place {
   int s, slot, rt, tile;
@@ -167,22 +189,7 @@ template <int SHIFT> struct KeyPlan {
     const int per = (n + THREADS - 1) / THREADS, first = min(n, tid * per), last = min(n, first + per);
     int least_rows = p.least_rows, most_rows = p.most_rows;
     if (p.least_work > 0) {   // (both launches come to the same)
-      unsigned long long work = 0;
-      for (int s = first; s < last; ++s) {
-        const int rows = max(clamp(p.a.row_start[s + 1], 0, p.a.rows) - clamp(p.a.row_start[s], 0, p.a.rows), 0);
-        if (rows >= p.many_rows)
-          work += (unsigned long long)rows * (unsigned)(clamp((long long)p.a.lens[s] - rows, 0, room) + rows / 2);
-      }
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1)
-        work += __shfl_xor_sync(0xffffffffu, work, o);
-      if (lane == 0)
-        sums[warp] = (long long)work;
-      __syncthreads();
-      work = 0;
-      for (int w = 0; w < THREADS / 32; ++w)
-        work += (unsigned long long)sums[w];
-      __syncthreads();
+      const unsigned long long work = many_work<THREADS>(p, sums);
       if (work < (unsigned long long)p.least_work) {
         least_rows = p.many ? INT_MAX : 0;
         most_rows = INT_MAX;
