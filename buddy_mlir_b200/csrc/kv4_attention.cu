@@ -26,8 +26,8 @@ constexpr int kRows = 8;            // query rows of an item: a position's heads
 constexpr int kSlots = 4;           // tiles that a warp has in flight or in hand
 constexpr int kChunkRows = 64;     // query vectors of a sequence and kv head from which on tcgen05 has them
 constexpr int kLeastKeys = 512, kSplit = 1000;     // of a CTA, where there are not more CTAs than that asks for
-// of a lane's sum of weights: a key that has more of it is one of few (short f16 contexts: errors 2.1e-4, as with 0.25, where a step of 200 sequences takes 5 % longer; all
-// rounded 3.0e-4 and 8 % shorter)
+// Of a lane's sum of weights: a key that has more of it is one of few.  (Short f16 contexts: errors 2.1e-4, as with 0.25, where a step of 200 sequences takes
+// 5 % longer; all weights rounded: 3.0e-4, and 8 % shorter.)
 constexpr float kFew = 0.9f;
 constexpr float kLeastScale = 5.9604645e-8f;   // (f16's smallest: a group of equal values has the scale 0)
 
@@ -272,7 +272,8 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
         s[n][e] = ex2(s[n][e] - r[e & 1]);
         l[e & 1] += s[n][e];
       }
-      // Weights are rounded to f16, as the result is; of many keys that averages out.  Where a key is most of a lane's, what the rounding left counts too.  (bf16 results are rounded eight times as far, f32 weights have two terms.)
+      // Weights are rounded to f16, as the result is; of many keys that averages out.  Where a key is most of a lane's, what the rounding left counts too.
+      // (bf16 results are rounded eight times as far, f32 weights have two terms.)
       bool few = false;
       if constexpr (TYPE == B200_F16)
         few = __any_sync(0xffffffffu, fmaxf(s[n][0], s[n][2]) > kFew * l[0] || fmaxf(s[n][1], s[n][3]) > kFew * l[1]);
