@@ -8,7 +8,8 @@
 // f16: nibbles 0 and 1 of a half-word are the subnormal numbers c 2^-24 and c 2^-20, which the tensor cores multiply exactly.
 //
 // The reference r of a row's weights is not its largest score but the largest of score + log2 of the key's larger V scale, so that the weights
-// that meet codes, p s, are at most 2^12 and near 2^8 where they count, whatever the scales are; sums and totals carry the same factor.
+// that meet codes, p s, are at most 2^12 and near 2^8 where they count, whatever the scales are; sums and totals carry the same factor.  (By their
+// magnitude: a group whose minimum was rounded to above its maximum has a negative one.)
 //
 // Sixteen warps of a CTA share an item's tiles, each with four tiles on their way (cp.async), and join in shared memory.  64 rows of 2000 to 4096 keys, 32
 // heads on 8 of 128 dims, bf16: 62 us, 3.7 TB/s, 0.56 of a copy's rate.  A tile is some 290 instructions of a warp, 114 clocks of an SM; issue slots are
@@ -29,7 +30,7 @@ constexpr int kLeastKeys = 512, kSplit = 1000;     // of a CTA, where there are 
 // Of a lane's sum of weights: a key that has more of it is one of few.  (Short f16 contexts: errors 2.1e-4, as with 0.25, where a step of 200 sequences takes
 // 5 % longer; all weights rounded: 3.0e-4, and 8 % shorter.)
 constexpr float kFew = 0.9f;
-constexpr float kLeastScale = 5.9604645e-8f;   // (f16's smallest: a group of equal values has the scale 0)
+constexpr float kLeastScale = 5.9604645e-8f;   // (f16's smallest: a group of equal values that f16 holds has the scale 0)
 
 __host__ __device__ constexpr int part_floats(int D) { return kRows * (D + 4) + 2 * kRows; }   // sums in rows of D + 4, maxima, totals
 
@@ -221,7 +222,7 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
         float largest = kLeastScale;
 #pragma unroll
         for (int gr = 0; gr < GROUPS; ++gr)
-          largest = fmaxf(largest, halves(vp[h][gr]).x);
+          largest = fmaxf(largest, fabsf(halves(vp[h][gr]).x));
         const float height = lg2(largest);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {

@@ -1,0 +1,83 @@
+"""b200_kv4_attention where a cache's groups are of unusual magnitude: constant ones (whose minimum, rounded to f16, may lie above all of them: a negative scale) and any
+finite pair.  Bounds are relative to the largest value of the output's own group."""
+import numpy as np
+import pytest
+
+import kv4_util as u
+from test_gpu_kv4 import Batch, bound, dev, rows_of
+from test_gpu_kv4_rows import Rows
+
+pytestmark = pytest.mark.gpu
+KINDS = pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+FORMS = pytest.mark.parametrize("many", [False, True])
+
+
+def batch(many, D, kind, seed, q_scale=1.0):
+    """Sequences of one key to some hundred; many: beside a long prompt, so that the form for many rows has the second."""
+    if many:
+        return Rows([1, 150, 40], [1, 90, 1], 4, 2, D, 16, kind, seed, q_scale=q_scale)
+    return Batch([1, 40, 300, 17], [1, 1, 3, 2], 4, 2, D, 16, kind, seed, q_scale=q_scale)
+
+
+def refill(b, make):
+    """K and V of all positions of every sequence: make(n) gives V [n, heads, D]."""
+    for s in range(len(b.lens) - isinstance(b, Rows)):
+        n, H, D = b.lens[s], b.host.heads, b.host.D
+        slots = np.array([int(b.table[s, j // b.host.page]) * b.host.page + j % b.host.page for j in range(n)], np.int64)
+        k, v = rows_of(b.rng, n, H, D), np.ascontiguousarray(make(n), np.float32)
+        u.write(b.cache, dev(k.reshape(n, -1)), dev(v.reshape(n, -1)), "f32", dev(slots))
+    b.host.pool = b.pool.cpu().numpy()
+
+
+def check_groups(b, every=1):
+    """Every output against f64, within what its own group of 64 dims allows (values of 16 bits as operands: bf16 rows of many only)."""
+    out = b.run().float().cpu().numpy()
+    for s in range(len(b.lens) - isinstance(b, Rows)):
+        n, c, page = b.lens[s], b.counts[s], b.host.page
+        many = b.kind == "bf16" and c * b.q_heads // b.host.heads >= 64
+        for i in sorted(set(range(0, c, every)) | {c - 1}):
+            seen = n - c + i + 1
+            k, v = b.host.rows([int(b.table[s, j // page]) * page + j % page for j in range(seen)])
+            r = b.row_start[s] + i
+            want, S, _ = u.attend(b.q[r], k, v, np.ones(seen, bool), b.scale)
+            got = out[r].reshape(want.shape)
+            for g in range(0, b.host.D, 64):
+                most = bound(b.kind, S, np.abs(v[:, :, g:g + 64]).max(), seen, many)
+                far = np.abs(got[:, g:g + 64] - want[:, g:g + 64]).max()
+                assert far <= most, (s, i, g, far, most)
+
+
+@KINDS
+@FORMS
+@pytest.mark.parametrize("value", [3.0012, 1000.3, 0.3, -1000.2, 3.25])
+@pytest.mark.parametrize("D,which", [(64, (0,)), (128, (0, 1)), (128, (0,)), (128, (1,))])
+def test_constant_groups(kind, many, value, D, which):
+    b = batch(many, D, kind, 61)
+
+    def make(n):
+        v = rows_of(b.rng, n, 2, D)
+        for g in which:
+            v[..., 64 * g:64 * g + 64] = value
+        return v
+    refill(b, make)
+    if value == 1000.3:                                                   # (what the case is about)
+        pairs = np.ascontiguousarray(b.host._parts(int(b.table[0, 0]) * 16, 1)[0][:, 17 * D:17 * D + D // 16]).view(np.float16)
+        assert pairs.reshape(2, -1, 2)[0, which[0], 0] < 0
+    check_groups(b, 7)
+
+
+@KINDS
+@FORMS
+@pytest.mark.parametrize("D", [64, 128])
+def test_any_finite_pair(kind, many, D):
+    """Scales of either sign with any codes, as another writer may leave them: a value is lo + scale * code whatever they are."""
+    b = batch(many, D, kind, 62)
+    for s in range(len(b.lens) - many):
+        for j in range(b.lens[s]):
+            for which in (0, 1):
+                tile, _, _, pair = b.host._parts(int(b.table[s, j // 16]) * 16 + j % 16, which)
+                p = np.ascontiguousarray(tile[:, pair]).view(np.float16).reshape(b.host.heads, -1, 2)
+                p[..., 0] *= b.rng.choice([-1.0, -1.0, 1.0, 0.0], p.shape[:-1]).astype(np.float16)
+                tile[:, pair] = p.reshape(b.host.heads, -1).view(np.uint8)
+    b.pool.copy_(dev(b.host.pool))
+    check_groups(b, 7)
