@@ -260,12 +260,15 @@ int b200_kv_overflow(float **kv_dev, int n_buffers, int kv_heads, int max_len,
  * and V.  A position's K row (and V row) of one head is cut into groups of 64
  * dims.  With x' = x clamped to +-65504 (the largest f16), a group has
  *   lo = f16(min x'),  scale = f16((max x' - lo) / 15)
- *   code = rint((x' - lo) / scale) within 0..15 (0 where the scale is 0)
+ *   code = rint((x' - lo) / scale) within 0..15 (0 where the scale is not positive)
  * each operation rounded to f32 (nearest, ties to even), and stands for
  *   value = lo + scale * code            (rounded to f32 once).
- * So |value - x'| is at most half a step and what lo's rounding adds, and the
- * bytes are the same wherever they are computed.  Infinities are held as
- * +-65504; a NaN makes its group NaN.  4.5 bits a value.
+ * So |value - x'| is at most half a step and what the roundings of lo and, fifteen times,
+ * of scale add, and the bytes are the same wherever they are computed.  (A group narrower
+ * than its minimum's rounding can have lo above all of it, and then a scale below zero,
+ * held as it is, with codes of 0: 64 values of 1000.3 are 1000.5.  Readers take any finite
+ * pair at its word, whatever its codes.)  Infinities are held as +-65504; a NaN makes its
+ * group NaN.  4.5 bits a value.
  *
  * Layout.  Sixteen positions of a head are a tile of 16 * (D + D / 8) bytes; the
  * pool is [n_pages][kv_heads][page / 16] tiles.  In a tile, in this order:

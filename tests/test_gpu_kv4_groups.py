@@ -81,3 +81,25 @@ def test_any_finite_pair(kind, many, D):
                 tile[:, pair] = p.reshape(b.host.heads, -1).view(np.uint8)
     b.pool.copy_(dev(b.host.pool))
     check_groups(b, 7)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_how_a_group_narrower_than_its_minimums_rounding_is_held(D):
+    """Where the scale is not positive every code is 0 and the value is lo, bit for bit: (values, lo, the scale's sign)."""
+    rows = [(1000.3, 1000.5, -1), (3.0012, 3.001953125, -1), (-1000.2, -1000.0, -1), (3.25, 3.25, 0), (1000.2, 1000.0, 1), (65503.0, 65504.0, -1), (1e-9, 0.0, 0)]
+    x = np.repeat(np.array([r[0] for r in rows], np.float32)[:, None], D, 1)
+    host = u.Cache(1, 1, D, 16)
+    pool = dev(host.pool)
+    cache = u.cache_arg(pool, 1, 1, D, 16)
+    slots = np.arange(len(rows), dtype=np.int64)
+    u.write(cache, dev(x), dev(x), "f32", dev(slots))
+    host.pool = pool.cpu().numpy()
+    for j, (value, lo, sign) in enumerate(rows):
+        for which in (0, 1):
+            tile, byte, high, pair = host._parts(j, which)
+            p = np.ascontiguousarray(tile[0, pair]).view(np.float16).reshape(-1, 2)
+            assert (p[:, 1] == np.float16(lo)).all() and (np.sign(p[:, 0]) == sign).all(), (value, p)
+            codes = tile[0, byte] >> (4 * high) & 15
+            assert (codes == (15 if sign > 0 else 0)).all()
+        k, _ = host.read(j)
+        assert sign > 0 or (k == np.float32(lo)).all()
