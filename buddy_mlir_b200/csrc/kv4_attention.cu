@@ -238,13 +238,13 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
         }
       }
     }
-    if (__any_sync(0xffffffffu, top[0] > r[0] + (kKv4Top + kKv4Lag) || top[1] > r[1] + (kKv4Top + kKv4Lag))) {
+    if (__any_sync(0xffffffffu, kv4_moves(top[0], r[0]) || kv4_moves(top[1], r[1]))) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1)
           top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
-        top[e] = top[e] > r[e] + (kKv4Top + kKv4Lag) ? top[e] - kKv4Top : r[e];   // (each row for itself)
+        top[e] = kv4_moves(top[e], r[e]) ? kv4_reference(top[e]) : r[e];   // (each row for itself)
         const float keep = ex2(r[e] - top[e]);
         r[e] = top[e];
         l[e] *= keep;

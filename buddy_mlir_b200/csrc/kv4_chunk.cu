@@ -138,6 +138,7 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel
       const bool any = mine > 0;
       const uint32_t n = g.b1 - g.b0;
       float r = kKv4Seed, l = 0.f, factor = 0.f;
+      bool far = false;                         // a row of this warp has its reference far from zero
       bool marks[GROUPS] = {};                  // V groups that become NaN
       const int token = row / p.G, seen_by = any && token < min(mine, half) ? clamp((long long)g.base + g.first + set * half + token + 1, 0, room) : 0;
       const bool live = any && token < min(mine, half);
@@ -196,9 +197,9 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel
         };
         // a row's reference moves, at the keys 32 c and on
         auto move = [&](float top, int c) {
-          const bool moves = top > r + (kKv4Top + kKv4Lag);
-          const float to = moves ? ceilf(top) - kKv4Top : r, keep = ex2(r - to);   // (each row for itself)
+          const float to = kv4_moves(top, r) ? kv4_reference(ceilf(top)) : r, keep = ex2(r - to);   // (each row for itself)
           r = to;
+          far = __any_sync(0xffffffffu, fabsf(r) >= kKv4Far / 2 && r != kKv4Seed);
           l *= keep;
           auto times = [&](uint32_t at, bool pairs) {
             uint32_t w[32];
@@ -245,10 +246,19 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel
               x[k / 2 & 3] = max3(x[k / 2 & 3], __uint_as_float(w[k]), __uint_as_float(w[k + 1]));
             }
             const float top = fmaxf(max3(x[0], x[1], x[2]), x[3]) * factor;
-            if (__any_sync(0xffffffffu, top > r + (kKv4Top + kKv4Lag)))
+            if (__any_sync(0xffffffffu, kv4_moves(top, r)))
               move(top, c);
+            // Scores less the reference are one fma each.  Far out its exact product and the rounded one that made the reference are steps of f32 apart, and
+            // those are whole powers of two of a weight: scores are rounded first.
+            float by = factor;
+            if (far) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                w[k] = __float_as_uint(__uint_as_float(w[k]) * factor);
+              by = 1.f;
+            }
             uint32_t out[16];
-            const uint64_t ff = pack2(factor, factor), rr = pack2(-r, -r);
+            const uint64_t ff = pack2(by, by), rr = pack2(-r, -r);
             uint64_t sum[2] = {};
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {

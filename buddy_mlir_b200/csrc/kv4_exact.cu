@@ -292,9 +292,8 @@ template <int D, int TYPE> __global__ void __launch_bounds__(kThreads, 1) kv4_ex
         pair_meets();
         top = fmaxf(top, bars.top[block & 1][1 - side][row]);
         // ---- a row's reference moves (both threads know it, and have half of the sums each)
-        if (__any_sync(0xffffffffu, top > r + (kKv4Top + kKv4Lag))) {
-          const bool moves = top > r + (kKv4Top + kKv4Lag);
-          const float to = moves ? ceilf(top) - kKv4Top : r, keep = ex2(r - to);   // (each row for itself)
+        if (__any_sync(0xffffffffu, kv4_moves(top, r))) {
+          const float to = kv4_moves(top, r) ? kv4_reference(ceilf(top)) : r, keep = ex2(r - to);   // (each row for itself)
           r = to;
           l *= keep;
 #pragma unroll

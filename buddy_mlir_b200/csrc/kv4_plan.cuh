@@ -13,7 +13,9 @@ constexpr int kKv4Many = 4096;
 constexpr int kKv4Item = 48;           // keys that take as long as beginning and ending an item
 constexpr float kKv4Top = 8.f;         // powers of two: what the largest weight that meets codes is at when a row's reference is set,
 constexpr float kKv4Lag = 4.f;         // and how far above that one may come before it is set again
-constexpr float kKv4Seed = -1.0e30f;   // a row's reference before its first key
+constexpr float kKv4Seed = -3.402823466e38f;   // a row's reference before its first key: no finite score lies below
+// Scores from here on are their own reference: a step of f32 is as large as kKv4Top there, and weights must neither vanish nor leave f16 by how a sum was rounded.
+constexpr float kKv4Far = 16777216.f;
 
 struct Kv4Params {
   const uint8_t *pool;
@@ -39,6 +41,9 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Whether a row's reference moves for a score of `top`, and where to.  (By their difference, which is exact where they are near each other.)
+__device__ __forceinline__ bool kv4_moves(float top, float r) { return top - r > kKv4Top + kKv4Lag; }
+__device__ __forceinline__ float kv4_reference(float top) { return fabsf(top) < kKv4Far ? top - kKv4Top : top; }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

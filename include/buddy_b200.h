@@ -356,7 +356,9 @@ int b200_page_step(const b200_page_step_args *a, void *stream);
  * sequence is a decode step, several are drafted tokens, many a chunk of a prompt;
  * all can stand in one call.  q head h reads kv head h / (q_heads / kv_heads).
  *   out = softmax(scale * q K^T) V   with the values of the cache,
- * scores, sums and products with f32 accumulators, rounded to `dtype` once.
+ * scores, sums and products with f32 accumulators, rounded to `dtype` once.  Scores may lie
+ * anywhere in f32, in units of 1 / log2 e (16-bit q below 2^117 in magnitude); one that leaves it
+ * downwards has no weight.
  * Codes count exactly.  dtype f32: q and the weights to 2^-22 of themselves.  bf16
  * and f16: q exactly (elements down to 2^-28 of their row's largest), the weights
  * to 2^-11 (f16: those that are most of a sum to 2^-22).  bf16 sequences with 64 or
