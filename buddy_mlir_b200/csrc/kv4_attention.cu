@@ -9,7 +9,9 @@
 //
 // The reference r of a row's weights is not its largest score but the largest of score + log2 of the key's larger V scale, so that the weights
 // that meet codes, p s, are at most 2^12 and near 2^8 where they count, whatever the scales are; sums and totals carry the same factor.  (By their
-// magnitude: a group whose minimum was rounded to above its maximum has a negative one.)
+// magnitude: a group whose minimum was rounded to above its maximum has a negative one.)  f16 ends at 2^-24, 2^-32 of that: where the other group's weights are
+// far smaller (kNear), those of f32 and their sums carry a power of two of their own, set when the reference moves and lowered when a weight outgrows it (a group at
+// 2^-20 of the other would keep 13 bits).  The 16-bit types, whose one term keeps its 11 bits down to 2^-22 of the other group, go without: that took them 5 to 14 % longer.
 //
 // Sixteen warps of a CTA share an item's tiles, each with four tiles on their way (cp.async), and join in shared memory.  64 rows of 2000 to 4096 keys, 32
 // heads on 8 of 128 dims, bf16: 62 us, 3.7 TB/s, 0.56 of a copy's rate.  A tile is some 290 instructions of a warp, 114 clocks of an SM; issue slots are
@@ -30,6 +32,8 @@ constexpr int kLeastKeys = 512, kSplit = 1000;     // of a CTA, where there are 
 // Of a lane's sum of weights: a key that has more of it is one of few.  (Short f16 contexts: errors 2.1e-4, as with 0.25, where a step of 200 sequences takes
 // 5 % longer; all weights rounded: 3.0e-4, and 8 % shorter.)
 constexpr float kFew = 0.9f;
+constexpr float kNear = 6.f, kApart = 64.f;   // log2 of how much smaller a group's largest weight may be than the other's before it is raised; that ratio
+constexpr int kMostLift = 40;
 constexpr float kLeastScale = 5.9604645e-8f;   // (f16's smallest: a group of equal values that f16 holds has the scale 0)
 
 __host__ __device__ constexpr int part_floats(int D) { return kRows * (D + 4) + 2 * kRows; }   // sums in rows of D + 4, maxima, totals
@@ -93,14 +97,56 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
   static constexpr bool EXACT = TYPE == B200_F32;
   static constexpr int TERMS = EXACT ? 2 : 1;
   static constexpr int KT = EXACT ? 1 : 2;  // tiles at a time
+  static constexpr bool LIFTS = EXACT && GROUPS == 2;
   static constexpr float LOW = EXACT ? 1.f : 5.9604645e-8f, HIGH = EXACT ? 16.f : 9.5367432e-7f;   // units of the codes' operands
   uint32_t q[TERMS][STEPS][2];
   float qs[GROUPS][2];                      // sums of q over a group, times the scores' scale, of rows 2 t and 2 t + 1 (t: lane % 4)
   float unit[2];                            // the scores' scale over the row's power of two and the codes' unit
   float o[STEPS][4];                        // dims 16 i + g (+ 8), rows 2 t (+ 1) (g: lane / 4)
   float bias[GROUPS][2], r[2], l[2];        // sums over this lane's keys: p (lo + 8 s), p
+  uint32_t lift;                            // LIFTS: byte 2 group + row: log2 of what that group's weights and o are raised by
 
+  __device__ __forceinline__ int lift_of(int gr, int e) const { return lift >> 8 * (2 * gr + e) & 255; }
+  __device__ __forceinline__ void times(int gr, int e, float f) {
+#pragma unroll
+    for (int i = 4 * gr; i < 4 * gr + 4; ++i) {
+      o[i][e] *= f;
+      o[i][2 + e] *= f;
+    }
+  }
+  // The powers of two of both groups' weights, from the largest score + log2 of scale of these keys: set where the keys are among those that count most for the
+  // row, otherwise only lowered as far as f16 asks for.
+  __device__ __forceinline__ void settle(const uint8_t *tiles, const float (&s)[KT][4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < KT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint2 pairs = *reinterpret_cast<const uint2 *>(tiles + n * BYTES + kv4_v_pairs(D) + (g + 8 * h) * 8);
+          most[0] = fmaxf(most[0], s[n][2 * h + e] + lg2(fabsf(halves(pairs.x).x)));
+          most[1] = fmaxf(most[1], s[n][2 * h + e] + lg2(fabsf(halves(pairs.y).x)));
+        }
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        most[0] = fmaxf(most[0], __shfl_xor_sync(0xffffffffu, most[0], x));
+        most[1] = fmaxf(most[1], __shfl_xor_sync(0xffffffffu, most[1], x));
+      }
+      const bool counts = fmaxf(most[0], most[1]) > r[e] + kKv4Top - kNear;
+#pragma unroll
+      for (int gr = 0; gr < 2; ++gr) {
+        const int have = lift_of(gr, e);
+        const float less = r[e] + kKv4Top - most[gr];   // (a group of scales 0 asks for nothing)
+        const int to = !(less < 1000.f) ? have : counts ? (less > kNear ? min((int)less, kMostLift) : 0) : min(have, max((int)(less + kNear), 0));
+        lift += (uint32_t)(to - have) << 8 * (2 * gr + e);
+        times(gr, e, power(to - have));
+      }
+    }
+  }
   __device__ __forceinline__ void clear() {
+    lift = 0;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
@@ -238,6 +284,7 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
         }
       }
     }
+    bool raised = LIFTS && __any_sync(0xffffffffu, lift != 0);
     if (__any_sync(0xffffffffu, kv4_moves(top[0], r[0]) || kv4_moves(top[1], r[1]))) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -249,15 +296,29 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
         r[e] = top[e];
         l[e] *= keep;
 #pragma unroll
-        for (int gr = 0; gr < GROUPS; ++gr)
+        for (int gr = 0; gr < GROUPS; ++gr) {
           bias[gr][e] *= keep;
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-          o[i][e] *= keep;
-          o[i][2 + e] *= keep;
+          times(gr, e, keep);
         }
       }
+      if constexpr (LIFTS) {
+        bool apart = false;   // keys that are seen, and whose groups are
+#pragma unroll
+        for (int n = 0; n < KT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint2 pairs = *reinterpret_cast<const uint2 *>(tiles + n * BYTES + kv4_v_pairs(D) + (g + 8 * h) * 8);
+            const float a = fabsf(halves(pairs.x).x), b = fabsf(halves(pairs.y).x), least = fminf(a, b);
+            apart = apart || (least > 0.f && least * kApart < fmaxf(a, b) && fmaxf(s[n][2 * h], s[n][2 * h + 1]) > -INFINITY);
+          }
+        raised = raised || __any_sync(0xffffffffu, apart);
+      }
     }
+    if constexpr (LIFTS)
+      if (raised) {
+        settle(tiles, s);
+        raised = __any_sync(0xffffffffu, lift != 0);
+      }
 #pragma unroll
     for (int n = 0; n < KT; ++n) {
       const uint8_t *tile = tiles + n * BYTES;
@@ -297,6 +358,10 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
             bias[gr][e] = b;
           }
         }
+        if (LIFTS && raised)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] *= power(lift_of(gr, k & 1));
         uint32_t b0[TERMS], b1[TERMS];
         split<TERMS>(w[0], w[1], b0);
         split<TERMS>(w[2], w[3], b1);
@@ -357,8 +422,9 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
       }
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
-        o[i][e] = fmaf(o[i][e], 1.f / LOW, bias[i * 16 / kKv4Group][e]);
-        o[i][2 + e] = fmaf(o[i][2 + e], 1.f / HIGH, bias[i * 16 / kKv4Group][e]);
+        const float lower = LIFTS ? power(-lift_of(i * 16 / kKv4Group, e)) : 1.f;
+        o[i][e] = fmaf(o[i][e] * lower, 1.f / LOW, bias[i * 16 / kKv4Group][e]);
+        o[i][2 + e] = fmaf(o[i][2 + e] * lower, 1.f / HIGH, bias[i * 16 / kKv4Group][e]);
       }
     }
   }

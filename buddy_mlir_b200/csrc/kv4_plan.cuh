@@ -44,6 +44,7 @@ __device__ __forceinline__ float ex2(float x) {
 // Whether a row's reference moves for a score of `top`, and where to.  (By their difference, which is exact where they are near each other.)
 __device__ __forceinline__ bool kv4_moves(float top, float r) { return top - r > kKv4Top + kKv4Lag; }
 __device__ __forceinline__ float kv4_reference(float top) { return fabsf(top) < kKv4Far ? top - kKv4Top : top; }
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

@@ -69,7 +69,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 __device__ __forceinline__ bool finite_pair(uint32_t pair) { return (pair & 0x7c00u) != 0x7c00u && (pair & 0x7c000000u) != 0x7c000000u; }
-__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 // A CTA's share of an item: blocks b0 .. b1 - 1 of `all`.
 struct Segment {
   Place at;
