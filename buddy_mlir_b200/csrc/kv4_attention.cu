@@ -105,6 +105,7 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
   float o[STEPS][4];                        // dims 16 i + g (+ 8), rows 2 t (+ 1) (g: lane / 4)
   float bias[GROUPS][2], r[2], l[2];        // sums over this lane's keys: p (lo + 8 s), p
   uint32_t lift;                            // LIFTS: byte 2 group + row: log2 of what that group's weights and o are raised by
+  bool raised;                              // any of the warp's is
 
   __device__ __forceinline__ int lift_of(int gr, int e) const { return lift >> 8 * (2 * gr + e) & 255; }
   __device__ __forceinline__ void times(int gr, int e, float f) {
@@ -147,6 +148,7 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
   }
   __device__ __forceinline__ void clear() {
     lift = 0;
+    raised = false;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
@@ -284,7 +286,6 @@ template <int D, int TYPE> struct Tile {   // of a warp: one item's sums
         }
       }
     }
-    bool raised = LIFTS && __any_sync(0xffffffffu, lift != 0);
     if (__any_sync(0xffffffffu, kv4_moves(top[0], r[0]) || kv4_moves(top[1], r[1]))) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
