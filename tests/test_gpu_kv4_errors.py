@@ -1,0 +1,53 @@
+"""How exact b200_kv4_attention is by root mean square, where the bounds of single outputs are too wide to tell its forms from one another."""
+import numpy as np
+import pytest
+
+import kv4_util as u
+from test_gpu_kv4 import Batch, bound
+from test_gpu_kv4_rows import Rows
+
+pytestmark = pytest.mark.gpu
+# The rounding of a result alone: off by at most half a step, evenly, so by half a step over sqrt(3) where a value is just above a power of two, less elsewhere.
+ROUNDED = {"f32": 2.0 ** -24 / 3 ** 0.5, "f16": 2.0 ** -11 / 3 ** 0.5, "bf16": 2.0 ** -8 / 3 ** 0.5}
+
+
+def errors(b, last, every):
+    """(rms of the error over rms of the result, largest S) over rows of the sequences before `last`; every row also within its bound, without the allowance for values
+    held as 16-bit operands where the type has none."""
+    out = b.run().float().cpu().numpy()
+    far = size = most_S = 0.0
+    for s in range(last):
+        n, c, page = b.lens[s], b.counts[s], b.host.page
+        for i in range(0, c, every):
+            seen = n - c + i + 1
+            k, v = b.host.rows([int(b.table[s, j // page]) * page + j % page for j in range(seen)])
+            r = b.row_start[s] + i
+            want, S, V = u.attend(b.q[r], k, v, np.ones(seen, bool), b.scale)
+            off = out[r].reshape(want.shape) - want
+            assert np.abs(off).max() <= bound(b.kind, S, V, seen, b.kind == "bf16" and c * b.q_heads // b.host.heads >= 64), (s, i)
+            far, size, most_S = far + (off ** 2).sum(), size + (want ** 2).sum(), max(most_S, S)
+    return (far / size) ** 0.5, most_S
+
+
+# f32: scores of which 2^-20 S is rounded (test_gpu_kv4.py), 2^-20 for the rest.  f16: the result's rounding, a hundredth for all else: values and weights are not
+# rounded to 16 bits there.  bf16: values, q and weights as f16, half a step of which is an eighth of bf16's each (2^-11 S of a score; S averages out to its root mean
+# square over 64 dims and more, an eighth of it).
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q_heads,kv_heads,D", [(8, 2, 128), (6, 2, 64), (12, 2, 128)])
+def test_sequences_of_many_rows(kind, q_heads, kv_heads, D):
+    b = Rows([300, 700], [140, 100], q_heads, kv_heads, D, 16, kind, 81)
+    rms, S = errors(b, 2, 5)
+    limit = {"f32": 2.0 ** -20 * (1 + S), "f16": 1.01 * ROUNDED["f16"], "bf16": np.hypot(ROUNDED["bf16"], 2.0 ** -11 * (2 + S / 8))}[kind]
+    assert rms <= limit, (rms, limit, S)
+
+
+# Few rows: weights of 16-bit types are one f16, each off by as much as an f16 result; rows of few keys have them side by side with the result's own rounding.
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("longest", [4, 60, 600])
+def test_sequences_of_few_rows(kind, longest):
+    rng = np.random.default_rng(longest)
+    lens = [int(x) for x in rng.integers(1, longest + 1, 40)]
+    b = Batch(lens, [1] * 40, 8, 2, 128, 16, kind, 82)
+    rms, S = errors(b, 40, 1)
+    limit = {"f32": 2.0 ** -20 * (1 + S), "f16": 2 ** 0.5 * ROUNDED["f16"], "bf16": np.hypot(ROUNDED["bf16"], ROUNDED["f16"])}[kind]
+    assert rms <= limit, (rms, limit, S)
