@@ -2281,7 +2281,11 @@ int b200_batch_remove(b200_batch *b, int seq) {
     std::vector<int32_t> add((size_t)b->max_seqs, 0);
     add[(size_t)seq] = -1;
     if (int rc = batch_step4(b, add, 0)) return rc;
+    int32_t status = 0;
+    B200_CUDA(cudaMemcpyAsync(&status, b->d_status, 4, cudaMemcpyDeviceToHost, b->m->stream));
     B200_CUDA(cudaStreamSynchronize(b->m->stream));
+    if (status != 0)
+      return fail(B200_ESTATE, "batch: the page allocator refused a step (%d)", status);
     b->cur ^= 1;
     b->free4 += pages;
     b->len[seq] = -1;

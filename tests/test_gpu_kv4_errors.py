@@ -51,3 +51,19 @@ def test_sequences_of_few_rows(kind, longest):
     rms, S = errors(b, 40, 1)
     limit = {"f32": 2.0 ** -20 * (1 + S), "f16": 2 ** 0.5 * ROUNDED["f16"], "bf16": np.hypot(ROUNDED["bf16"], ROUNDED["f16"])}[kind]
     assert rms <= limit, (rms, limit, S)
+
+
+def test_a_wait_that_gave_up_is_reported_until_the_workspace_is_zeroed():
+    """The word behind the counters is what a bounded wait leaves; written from the host here."""
+    import torch
+    from buddy_mlir_b200 import _lib
+    from gpu_util import stream
+    status = _lib.load().b200_kv4_attention_status
+    for b in (Batch([40, 7], [1, 3], 4, 2, 64, 16, "f32", 83), Rows([300], [140], 8, 2, 128, 16, "bf16", 84)):
+        before = b.run().clone()
+        assert status(b.ws.data_ptr(), stream()) == 0
+        b.ws[4 * 148:4 * 149].view(torch.int32).fill_(731)
+        b.run()
+        assert status(b.ws.data_ptr(), stream()) == -2 and "731" in _lib.load().b200_last_error().decode()
+        b.ws.zero_()
+        assert (b.run() == before).all() and status(b.ws.data_ptr(), stream()) == 0
