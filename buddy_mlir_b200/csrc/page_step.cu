@@ -24,6 +24,9 @@ __device__ __forceinline__ Sums up(Sums a, int o) {
   return {__shfl_up_sync(0xffffffffu, a.rows, o), __shfl_up_sync(0xffffffffu, a.taken, o), __shfl_up_sync(0xffffffffu, a.given, o)};
 }
 
+// (positions and a page's size: 2^31 - 1 each at most)
+__device__ __forceinline__ int pages_of(int positions, int page) { return (int)(((uint32_t)positions + (uint32_t)page - 1) / (uint32_t)page); }
+
 // The last i of 0 .. n - 1 with first[i] <= x (first does not decrease, first[0] <= x < first[n]): never a sequence without any.
 __device__ __forceinline__ int owner(const int32_t *first, int n, int x) {
   int lo = 0, hi = n;   // first[lo] <= x < first[hi]
@@ -99,7 +102,7 @@ __global__ void __launch_bounds__(kThreads) page_step_kernel(const __grid_consta
   if (ok) {   // (then all sums fit 32 bits)
     Sums at = {before.rows + sum.rows - mine.rows, before.taken + sum.taken - mine.taken, before.given + sum.given - mine.given};
     for (int s = first; s < last; ++s) {
-      const int held = s_held[s], add = p.add[s], have = (held + p.page - 1) / p.page;
+      const int held = s_held[s], add = p.add[s], have = pages_of(held, p.page);
       s_row[s] = (int32_t)at.rows;
       s_take[s] = (int32_t)at.taken;
       s_give[s] = (int32_t)at.given;
@@ -123,15 +126,15 @@ __global__ void __launch_bounds__(kThreads) page_step_kernel(const __grid_consta
     const int at = top - 1 - i;
     return at < n_free ? p.free_pages[at] : returned(at - n_free);
   };
-  const int at0 = blockIdx.x * threads + tid, step = gridDim.x * threads;
+  const uint32_t at0 = blockIdx.x * threads + tid, step = gridDim.x * threads;   // (counted without sign: the last step of a loop may pass 2^31)
   if (what & 1) {
-    for (int r = at0; r < p.max_rows; r += step) {
+    for (uint32_t r = at0; r < (uint32_t)p.max_rows; r += step) {
       int64_t slot = -1;
       int seq = -1, pos = -1;
-      if (r < rows) {
-        seq = owner(s_row, n, r);
-        pos = s_held[seq] + r - s_row[seq];
-        const int have = (s_held[seq] + p.page - 1) / p.page, at = pos / p.page;
+      if (r < (uint32_t)rows) {
+        seq = owner(s_row, n, (int)r);
+        pos = s_held[seq] + (int)r - s_row[seq];
+        const int have = pages_of(s_held[seq], p.page), at = pos / p.page;
         const int page = at < have ? p.block_table[(int64_t)seq * p.table_stride + at] : new_page(s_take[seq] + at - have);
         slot = (int64_t)page * p.page + pos % p.page;
       }
@@ -141,19 +144,19 @@ __global__ void __launch_bounds__(kThreads) page_step_kernel(const __grid_consta
       if (p.row_pos != nullptr)
         p.row_pos[r] = pos;
     }
-    for (int i = at0; i < taken; i += step) {
-      const int s = owner(s_take, n, i), have = (s_held[s] + p.page - 1) / p.page;
-      p.block_table[(int64_t)s * p.table_stride + have + i - s_take[s]] = new_page(i);
+    for (uint32_t i = at0; i < (uint32_t)taken; i += step) {
+      const int s = owner(s_take, n, (int)i), have = pages_of(s_held[s], p.page);
+      p.block_table[(int64_t)s * p.table_stride + have + (int)i - s_take[s]] = new_page((int)i);
     }
-    for (int i = at0; i < given - taken; i += step)   // what stays on the stack of them
-      p.free_pages[n_free + i] = returned(i);
-    for (int s = at0; s <= n; s += step)
+    for (uint32_t i = at0; (int64_t)i < (int64_t)given - taken; i += step)   // what stays on the stack of them
+      p.free_pages[n_free + (int)i] = returned((int)i);
+    for (uint32_t s = at0; s <= (uint32_t)n; s += step)
       p.row_start[s] = ok ? s_row[s] : 0;
     if (at0 == 0)
       *p.status = status;
   }
   if (what & 2) {
-    for (int s = at0; s < n; s += step)
+    for (uint32_t s = at0; s < (uint32_t)n; s += step)
       p.held_out[s] = !ok ? s_held[s] : s_row[s + 1] > s_row[s] ? s_held[s] + s_row[s + 1] - s_row[s] : p.add[s] < 0 ? 0 : s_held[s];
     if (at0 == 0)
       *p.n_free_out = ok ? top - taken : n_free;
@@ -169,7 +172,7 @@ int page_step_launch(const b200_page_step_args &a, cudaStream_t st) {
   if (int rc = raise_shared_limit(g_raised, (const void *)page_step_kernel, 4 * (4 * B200_PAGE_STEP_MAX_SEQS + 3)))
     return rc;
   // one CTA up to 2048 rows, a small one for a few sequences, then one for every 1024
-  const int ctas = a.max_rows <= 2048 ? 1 : std::min(kMostCtas, (a.max_rows + kThreads - 1) / kThreads);
+  const int ctas = a.max_rows <= 2048 ? 1 : std::min(kMostCtas, (a.max_rows - 1) / kThreads + 1);
   const int threads = ctas == 1 && a.n_seqs <= 256 && a.max_rows <= 512 ? 256 : kThreads;
   const bool apart = ctas > 1 && (a.held_out == a.held || a.n_free_out == a.n_free);
   if (int rc = launch_after(page_step_kernel, dim3(ctas), threads, bytes, st, a, apart ? 1 : 3))
