@@ -66,7 +66,8 @@ template <bool PAGED, int V> __global__ void __launch_bounds__(kRopeThreads) rop
   extern __shared__ float s_angle[];   // [D / 2] cosines, then sines
   kernel_go();
   const int half = p.D / 2, D = p.D, m = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // what the kernel before does not write: the angles, the page
+  // What the kernel before does not write: the angles, the page.  (The page allocator, a kernel, has written a 4-bit batch's row maps: embed_rows_launch comes
+  // between the two in a pass, and what is launched behind it finds all before it complete.)
   const int pos = PAGED ? p.row_pos[m] : p.pos0 + m;
   for (int j = threadIdx.x; j < half; j += kRopeThreads) {
     const float th = __fmul_rn(p.inv_freq[j], (float)pos);
@@ -696,6 +697,7 @@ int argmax_rows_launch(const float *v, int64_t n, int rows, int32_t *out, cudaSt
 int embed_rows_launch(const float *table, const int32_t *tokens_dev, float *x, int64_t H, int M, cudaStream_t st) {
   if (H % 4 != 0)
     return fail(B200_EINVAL, "embed_rows: hidden size must be a multiple of 4");
+  // An ordinary launch: rope_rows_kernel reads what was written before this one without waiting.
   embed_rows_kernel<<<M, 128, 0, st>>>(table, tokens_dev, x, H);
   B200_LAUNCH_CHECK();
   return B200_OK;
