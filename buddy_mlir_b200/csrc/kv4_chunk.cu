@@ -149,7 +149,7 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel
         if (live && p.wide_q16) {
 #pragma unroll
           for (int c = 0; c < D / 8; ++c)
-            *reinterpret_cast<uint4 *>(w + 4 * c) = __ldg(reinterpret_cast<const uint4 *>((const uint16_t *)p.a.q + q_row) + c);
+            *reinterpret_cast<uint4 *>(w + 4 * c) = *(reinterpret_cast<const uint4 *>((const uint16_t *)p.a.q + q_row) + c);
         } else {
 #pragma unroll
           for (int c = 0; c < D / 2; ++c)
@@ -344,16 +344,16 @@ template <int D> __global__ void __launch_bounds__(kThreads, 1) kv4_chunk_kernel
       for (int h = 0; h < 2; ++h) {
         const int j = gq + 8 * h;
         if constexpr (D == 128) {
-          *reinterpret_cast<uint4 *>(x.k[h]) = __ldg(reinterpret_cast<const uint4 *>(tile + j * 64 + t * 16));
-          *reinterpret_cast<uint4 *>(x.v + 4 * h) = __ldg(reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + h * 512 + lane * 16));
-          *reinterpret_cast<uint2 *>(x.kp[h]) = __ldg(reinterpret_cast<const uint2 *>(tile + kv4_k_pairs(D) + j * 8));
-          *reinterpret_cast<uint4 *>(x.vp[h]) = __ldg(reinterpret_cast<const uint4 *>(tile + kv4_v_pairs(D) + (2 * t + 8 * h) * 8));
+          *reinterpret_cast<uint4 *>(x.k[h]) = *reinterpret_cast<const uint4 *>(tile + j * 64 + t * 16);
+          *reinterpret_cast<uint4 *>(x.v + 4 * h) = *reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + h * 512 + lane * 16);
+          *reinterpret_cast<uint2 *>(x.kp[h]) = *reinterpret_cast<const uint2 *>(tile + kv4_k_pairs(D) + j * 8);
+          *reinterpret_cast<uint4 *>(x.vp[h]) = *reinterpret_cast<const uint4 *>(tile + kv4_v_pairs(D) + (2 * t + 8 * h) * 8);
         } else {
-          *reinterpret_cast<uint2 *>(x.k[h]) = __ldg(reinterpret_cast<const uint2 *>(tile + j * 32 + t * 8));
+          *reinterpret_cast<uint2 *>(x.k[h]) = *reinterpret_cast<const uint2 *>(tile + j * 32 + t * 8);
           if (h == 0)
-            *reinterpret_cast<uint4 *>(x.v) = __ldg(reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + lane * 16));
-          x.kp[h][0] = __ldg(reinterpret_cast<const uint32_t *>(tile + kv4_k_pairs(D) + j * 4));
-          *reinterpret_cast<uint2 *>(x.vp[h]) = __ldg(reinterpret_cast<const uint2 *>(tile + kv4_v_pairs(D) + (2 * t + 8 * h) * 4));
+            *reinterpret_cast<uint4 *>(x.v) = *reinterpret_cast<const uint4 *>(tile + kv4_v_codes(D) + lane * 16);
+          x.kp[h][0] = *reinterpret_cast<const uint32_t *>(tile + kv4_k_pairs(D) + j * 4);
+          *reinterpret_cast<uint2 *>(x.vp[h]) = *reinterpret_cast<const uint2 *>(tile + kv4_v_pairs(D) + (2 * t + 8 * h) * 4);
         }
       }
     };

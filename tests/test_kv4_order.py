@@ -15,3 +15,11 @@ def test_an_ordinary_launch_stands_between_the_allocator_and_who_reads_its_row_m
     rows = re.search(r"static int batch_rows\(.*?\n\}", open(os.path.join(CSRC, "engine.cu")).read(), re.S).group(0)
     assert rows.index("batch_step4(") < rows.index("embed_rows_launch(") < rows.index("rope_kv_paged_launch(")
     assert rows.count("batch_step4(") == rows.count("embed_rows_launch(") == 1
+
+
+def test_the_cache_is_not_read_as_constant_data():
+    """The writer, or the kernel that makes q, may run when the attention starts: loads for data that nobody writes meanwhile are not for those."""
+    for name in sorted(os.listdir(CSRC)):
+        if name.startswith("kv4") or name == "page_step.cu":
+            text = re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, name)).read())
+            assert not re.search(r"__ldg\b|ld\.global\.nc|__restrict__", text), name
