@@ -29,9 +29,9 @@ constexpr int kRows = 8;            // query rows of an item: a position's heads
 constexpr int kSlots = 4;           // tiles that a warp has in flight or in hand
 constexpr int kChunkRows = 64;     // query vectors of a sequence and kv head from which on tcgen05 has them
 constexpr int kLeastKeys = 512, kSplit = 1000;     // of a CTA, where there are not more CTAs than that asks for
-// Of a lane's sum of weights: a key that has more of it is one of few.  (Short f16 contexts: errors 2.1e-4, as with 0.25, where a step of 200 sequences takes
-// 5 % longer; all weights rounded: 3.0e-4, and 8 % shorter.)
-constexpr float kFew = 0.9f;
+// Of a lane's sum of weights: a key that has more of it is one of few.  (f16, steps of 200 sequences of up to 600 keys, twelve seeds: errors 2.0 to 2.3e-4, where the
+// result's own rounding is 2.0 to 2.1e-4; with 0.9 2.2 to 2.65e-4 and 2 % shorter; all weights rounded: 3.0e-4.)
+constexpr float kFew = 0.25f;
 constexpr float kNear = 6.f, kApart = 64.f;   // log2 of how much smaller a group's largest weight may be than the other's before it is raised; that ratio
 constexpr int kMostLift = 40;
 constexpr float kLeastScale = 5.9604645e-8f;   // (f16's smallest: a group of equal values that f16 holds has the scale 0)

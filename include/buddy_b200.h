@@ -361,7 +361,7 @@ int b200_page_step(const b200_page_step_args *a, void *stream);
  * downwards has no weight.
  * Codes count exactly.  dtype f32: q and the weights to 2^-22 of themselves.  bf16
  * and f16: q exactly (elements down to 2^-28 of their row's largest), the weights
- * to 2^-11 (f16: those that are most of a sum to 2^-22).  Products of a weight and a V scale
+ * to 2^-11 (f16: those that are a quarter of a sum and more to 2^-22).  Products of a weight and a V scale
  * end at 2^-32 of their row's largest: f32 of their own group of dims, else of both, so that
  * a group 2^-22 of its neighbour has fewer bits there.  bf16 sequences with 64 or
  * more query vectors per kv head (rows times q heads that share it) may take the

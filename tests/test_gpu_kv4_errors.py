@@ -67,3 +67,29 @@ def test_a_wait_that_gave_up_is_reported_until_the_workspace_is_zeroed():
         assert status(b.ws.data_ptr(), stream()) == -2 and "731" in _lib.load().b200_last_error().decode()
         b.ws.zero_()
         assert (b.run() == before).all() and status(b.ws.data_ptr(), stream()) == 0
+
+
+@pytest.mark.parametrize("share", [0.5, 0.6, 0.7])
+def test_f16_rows_whose_weight_lies_on_few_keys(share):
+    """What is left of a weight's rounding counts too where a key has a quarter of its lane's sum.  A lane of one tile has two keys, eight apart: with shares of 0.3 and
+    more none is rounded.  Their values nearly cancel, so that the result's own rounding does not hide it: 2^-12 of the larger weights would be 30 times the bound."""
+    from test_gpu_kv4 import dev
+    b = Batch([16] * 6, [1] * 6, 2, 2, 128, 16, "f16", 85)
+    b.scale = 1.0
+    b.q[:] = 0.0
+    b.q[:, :, 0] = 1.0
+    k = np.zeros((16, 2, 128), np.float32)
+    k[:8, :, :64] = np.float16(np.log(share / (1 - share)))               # (held exactly)
+    for s in range(6):
+        v = b.rng.standard_normal((16, 2, 128)).astype(np.float32)
+        v[8:] = -share / (1 - share) * v[:8]
+        slots = int(b.table[s, 0]) * 16 + np.arange(16)
+        u.write(b.cache, dev(k.reshape(16, -1)), dev(v.reshape(16, -1)), "f32", dev(slots.astype(np.int64)))
+    b.host.pool = b.pool.cpu().numpy()
+    out = b.run().double().cpu().numpy().reshape(6, 2, 128)
+    for s in range(6):
+        kk, vv = b.host.rows([int(b.table[s, 0]) * 16 + j for j in range(16)])
+        want, S, V = u.attend(b.q[s], kk, vv, np.ones(16, bool), 1.0)
+        # scores, sums, exponentials and weights of two terms as f32 rows have them; the result's own rounding
+        most = bound("f32", S, V, 16) + 2.0 ** -11 * np.abs(want)
+        assert (np.abs(out[s] - want) <= most).all(), (s, np.abs(out[s] - want).max(), most.min())
