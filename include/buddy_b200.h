@@ -360,7 +360,8 @@ int b200_page_step(const b200_page_step_args *a, void *stream);
  * anywhere in f32, in units of 1 / log2 e (16-bit q below 2^117 in magnitude); one that leaves it
  * downwards has no weight.
  * Codes count exactly.  dtype f32: q and the weights to 2^-22 of themselves.  bf16
- * and f16: q exactly (elements down to 2^-28 of their row's largest), the weights
+ * and f16: q exactly (bf16 elements down to 2^-27 of their row's largest, f16 down to 2^-24;
+ * smaller ones to 2^-35 of it), the weights
  * to 2^-11 (f16: those that are a quarter of a sum and more to 2^-22).  Products of a weight and a V scale
  * end at 2^-32 of their row's largest: f32 of their own group of dims, else of both, so that
  * a group 2^-22 of its neighbour has fewer bits there.  bf16 sequences with 64 or
