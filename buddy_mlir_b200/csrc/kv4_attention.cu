@@ -854,6 +854,9 @@ int b200_kv4_attention(const b200_kv4_cache *c, const b200_kv4_attention_args *a
   // leave it open, and both see from the lengths whose the sequences are.
   // (Few rows, many rows, us; 1000 keys, f32 12 heads on 2, else 32 on 8: f32 20 x 22 rows 54 / 59, 20 x 43 96 / 59; bf16 20 x 16 53 / 71, 20 x 32 88 / 73; f16 20 x 32
   // 91 / 103, 20 x 64 162 / 150; one sequence of 11 rows of f32 18 / 49.)
+  // Only where there are 24 query vectors of a kv head for every sequence (or place for one): other calls are decode steps, mostly, which would pay for the second
+  // launch and its look at the lengths (128 rows of 32 to 4000 keys, 32 heads on 8: bf16 79 us, 98 with it; f16 91 either way; f32 117, 133).  A chunk beside many of them is
+  // the price: 512 rows at 4000 keys and 127 rows take 282 us in bf16, 328 in f16, 471 in f32, where tcgen05 would have 210, 275 and 304; beside 63 they have it (182, 238, 257).
   const bool exact = a->dtype != B200_BF16;   // (a bf16 result is rounded eight times as far as f16 operands are)
   const double work = a->dtype == B200_F32 ? 5.5e6 : exact ? 30e6 : 15e6, vectors = (double)a->rows * a->q_heads;
   if ((exact ? kv4_exact_takes(p.G, a->n_seqs) : kv4_chunk_takes(p.G, a->n_seqs)) && (int64_t)a->rows * p.G >= kChunkRows &&

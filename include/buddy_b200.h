@@ -360,17 +360,18 @@ int b200_page_step(const b200_page_step_args *a, void *stream);
  * anywhere in f32, in units of 1 / log2 e (16-bit q below 2^117 in magnitude); one that leaves it
  * downwards has no weight.
  * Codes count exactly.  dtype f32: q and the weights to 2^-22 of themselves.  bf16
- * and f16: q exactly (bf16 elements down to 2^-27 of their row's largest, f16 down to 2^-24;
- * smaller ones to 2^-35 of it), the weights
- * to 2^-11 (f16: those that are a quarter of a sum and more to 2^-22).  Products of a weight and a V scale
- * end at 2^-32 of their row's largest: f32 of their own group of dims, else of both, so that
- * a group 2^-22 of its neighbour has fewer bits there.  bf16 sequences with 64 or
- * more query vectors per kv head (rows times q heads that share it) may take the
- * cache's values rounded to f16 as well, 2^-11 each.  A row that sees no position is zero, and so are the rows before
+ * and f16: q exactly (bf16 elements down to 2^-27 of their row's largest, f16 down to
+ * 2^-24; smaller ones to 2^-35 of it), the weights to 2^-11 (f16: those that are a quarter
+ * of a sum and more to 2^-22).  Products of a weight and a V scale end at 2^-32 of their
+ * row's largest: f32 of their own group of dims, else of both, so that a group 2^-22 of
+ * its neighbour has fewer bits there.  bf16 sequences with 64 or more query vectors per
+ * kv head (rows times q heads that share it) may take the cache's values rounded to f16 as
+ * well, 2^-11 each.  A row that sees no position is zero, and so are the rows before
  * row_start[0] and behind the last sequence's.  Positions beyond
  * table_stride * page, and those whose table entry is no page of the pool, are
- * not seen.  Nothing that a row does not see (infinities and NaN included)
- * changes it.  workspace: b200_kv4_attention_workspace_bytes() bytes, 256-byte
+ * not seen.  Nothing that a row does not see (infinities and NaN included) reaches it;
+ * what other rows of its sequence in the call see may decide how it is rounded, within the
+ * above, and what no row sees changes no bit.  workspace: b200_kv4_attention_workspace_bytes() bytes, 256-byte
  * aligned, zeroed once by the caller (every call leaves its counters zero);
  * calls that can overlap on the GPU need one each.  Results do not depend on what runs
  * beside them: the same inputs on the same device give the same bits.  q and out must not overlap.
