@@ -14,7 +14,7 @@
 // 2^-20 of the other would keep 13 bits).  The 16-bit types, whose one term keeps its 11 bits down to 2^-22 of the other group, go without: that took them 5 to 14 % longer.
 //
 // Sixteen warps of a CTA share an item's tiles, each with four tiles on their way (cp.async), and join in shared memory.  64 rows of 2000 to 4096 keys, 32
-// heads on 8 of 128 dims, bf16: 62 us, 3.7 TB/s, 0.56 of a copy's rate.  A tile is some 290 instructions of a warp, 114 clocks of an SM; issue slots are
+// heads on 8 of 128 dims, bf16: 62 us, 3.7 TB/s, 0.56 of a copy's rate (f32, one tile at a time and twice the products: 93 us).  A tile is some 290 instructions of a warp, 114 clocks of an SM; issue slots are
 // half full and the tensor pipe a quarter, so chains of latencies bound it at four warps a scheduler (128 registers a thread: q, sums and two tiles).
 #include "kv4_plan.cuh"
 

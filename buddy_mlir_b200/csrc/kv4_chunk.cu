@@ -11,7 +11,7 @@
 // Two sets of 128 rows take turns: one's products run under the other's softmax.  (S 2 x 128 columns, O 2 x D.)
 // A key's values that are not finite are zero in the operands, and what sees them becomes NaN afterwards: nothing reaches rows that do not.
 //
-// 1001 rows at 4000 keys, 32 heads on 8 of 128 dims, bf16: 119 us, 481 TFLOP/s, 0.29 of a dense product's rate.  A block of 128 keys takes an SM 7000 clocks,
+// 1001 rows at 4000 keys, 32 heads on 8 of 128 dims, bf16: 120 us, 479 TFLOP/s, 0.29 of a dense product's rate.  A block of 128 keys takes an SM 7000 clocks,
 // 1500 of them for its products: a set's softmax (3400) and the way of its weights through both products (2400) follow each other.  The softmax goes through its scores
 // in a loop of 32 at a time: straight code with the next 32 on their way took 4 % longer.
 #include "kv4_rows.cuh"

@@ -11,10 +11,10 @@
 // do the softmax, two threads per row: scores of half a block each, the larger of their maxima (through shared memory) decides whether the row's
 // reference moves, weights.  Scores of two blocks have their own columns (2 x 128), O and its sum D each.
 //
-// A prompt of 1000 f32 rows, 12 heads on 2 of 128 dims: 53 us (the few-rows form 70), errors 2.8e-7 of the result; 4000 rows: 412 us, 119 TFLOP/s.  A block takes some
+// A prompt of 1000 f32 rows, 12 heads on 2 of 128 dims: 53 us (the few-rows form 70), errors 3 to 4e-7 of the result; 4000 rows: 415 us, 118 TFLOP/s.  A block takes some
 // 8000 clocks, 5400 of them the softmax, and 2300 for the products: a tile's K takes a maker 2300, its V 1450, and of seven makers one has two tiles.  Eight
 // (17 warps of 96 registers) spill, 63 us; one thread per row and eight makers take as long here and 13 % longer at 4000 rows.  Items that CTAs share come together too
-// slowly to be worth it (78 us).  f16, 1001 rows at 4000 keys, 32 heads on 8: 264 us (kv4_chunk.cu, whose errors would be 2.5 times f16's rounding: 119).
+// slowly to be worth it (78 us).  f16, 1001 rows at 4000 keys, 32 heads on 8: 265 us (kv4_chunk.cu, whose errors would be 2.5 times f16's rounding: 120).
 #include "kv4_rows.cuh"
 
 #include <algorithm>

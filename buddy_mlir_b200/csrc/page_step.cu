@@ -4,7 +4,7 @@
 // the outputs; a row, a page or a place of the stack finds its sequence by binary search.  Table entries and places of the stack that are read
 // (below a sequence's old end, below the old top) are not those that are written; lengths and the top may be written where they were read, by
 // one CTA, after the others where there are any: a second launch of its own.
-// 24 sequences that grow by one: 4.6 us; 2000, a tenth of them by prompts of up to 500 rows (102 thousand places of the row maps): 10.3 us.  Latencies bound the
+// 24 sequences that grow by one: 4.5 us; 2000, a tenth of them by prompts of up to 500 rows (102 thousand places of the row maps): 9.8 us.  Latencies bound the
 // one, the searches' instructions the other.
 #include "kv4.cuh"
 

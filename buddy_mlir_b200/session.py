@@ -264,7 +264,10 @@ class BatchSession:
     them by one token per step.  Not part of buddy-mlir's interface (its
     sessions are single-sequence); per sequence the results are those of
     ModelSession.  kv_bits=4 holds the cache in 4 bits (b200_batch_create_kv4: a
-    seventh of the memory, results with the rounding of its keys and values)."""
+    seventh of the memory, results with the rounding of its keys and values;
+    steps of long contexts are faster, of short ones slower: the 1.5B int8
+    model's 24 sequences of 32..700 positions 2.26 ms instead of 1.97, 64 of
+    4000 3.13 instead of 7.18)."""
 
     def __init__(self, model: ModelSession, max_seqs: int, page_size: int, n_pages: int, max_context: int, kv_bits: int = 32):
         if kv_bits not in (4, 32):

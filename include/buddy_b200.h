@@ -370,9 +370,10 @@ int b200_page_step(const b200_page_step_args *a, void *stream);
  * row_start[0] and behind the last sequence's.  Positions beyond
  * table_stride * page, and those whose table entry is no page of the pool, are
  * not seen.  Nothing that a row does not see (infinities and NaN included) reaches it;
- * what other rows of its sequence in the call see may decide how it is rounded, within the
- * above, and what no row sees changes no bit.  workspace: b200_kv4_attention_workspace_bytes() bytes, 256-byte
- * aligned, zeroed once by the caller (every call leaves its counters zero);
+ * how long the call's sequences are, how many rows they have, and what the other rows of
+ * its own see may decide how it is rounded, within the above; what no row sees changes no
+ * bit.  workspace: b200_kv4_attention_workspace_bytes() bytes, 256-byte aligned, zeroed
+ * once by the caller (every call leaves its counters zero);
  * calls that can overlap on the GPU need one each.  Results do not depend on what runs
  * beside them: the same inputs on the same device give the same bits.  q and out must not overlap.
  * n_seqs up to B200_KV4_ATTENTION_MAX_SEQS, table_stride * page up to 2^30. */
